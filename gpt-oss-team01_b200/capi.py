@@ -15,8 +15,8 @@ CSRC = PKG_DIR / "csrc"
 # GPTOSS_B200_LIB points the binding at another build of the same C ABI (e.g. a tuning variant)
 LIB_PATH = Path(os.environ.get("GPTOSS_B200_LIB", CSRC / "libgptoss_b200.so"))
 SOURCES = ["routing.cu", "router.cu", "grouped_gemm.cu", "grouped_gemm_pair.cu", "comm.cu", "convert.cu", "capi.cu", "model_kernels.cu",
-           "model.cu"]
-HEADERS = ["common.cuh", "kernels.cuh", "tcgen05.cuh", "gemm_tile.cuh", "../../include/gptoss_b200.h"]
+           "model.cu", "tree_attention.cu", "lora.cu", "expert_choice.cu"]
+HEADERS = ["common.cuh", "kernels.cuh", "serving.cuh", "tcgen05.cuh", "gemm_tile.cuh", "../../include/gptoss_b200.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "--threads", "4"]
 
@@ -46,7 +46,8 @@ EXPORTS = [
     "gptoss_moe_dispatch_route", "gptoss_moe_dispatch_rows", "gptoss_moe_dispatch_push", "gptoss_moe_forward_dispatch",
     "gptoss_launch_count", "gptoss_argmax_rows", "gptoss_model_step_rows", "gptoss_model_step_seqs",
     "gptoss_moe_forward_host_submit", "gptoss_moe_forward_host_sliced_submit", "gptoss_moe_forward_host_wait",
-    "gptoss_model_layer_moe_dispatch",
+    "gptoss_model_layer_moe_dispatch", "gptoss_serving_last_error", "gptoss_tree_attention_workspace", "gptoss_tree_attention",
+    "gptoss_cache_commit", "gptoss_lora_workspace", "gptoss_lora_apply", "gptoss_expert_choice", "gptoss_moe_forward_routed",
 ]
 
 
@@ -62,6 +63,26 @@ class ModelConfig(C.Structure):
 class MoEDims(C.Structure):
     _fields_ = [("hidden", C.c_int), ("intermediate", C.c_int), ("n_experts", C.c_int),
                 ("top_k", C.c_int), ("n_layers", C.c_int), ("swiglu_limit", C.c_float)]
+
+
+class TreeAttentionArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k_cache", "v_cache", "out", "offsets", "ctx_len", "rows", "mask", "depth",
+                                          "sinks", "workspace")] + \
+               [("workspace_bytes", C.c_uint64), ("q_stride", C.c_int64), ("out_stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("n_tokens", "n_seqs", "max_nodes", "max_ctx", "mask_words", "cache_rows", "max_seq",
+                                       "n_q_heads", "n_kv_heads", "head_dim", "window")] + [("scale", C.c_float)]
+
+
+class LoraArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "a", "b", "scale", "ids", "y", "out", "workspace")] + \
+               [("workspace_bytes", C.c_uint64)] + [(n, C.c_int64) for n in ("x_stride", "y_stride", "out_stride")] + \
+               [(n, C.c_int) for n in ("T", "K", "n_out", "rank", "n_adapters")]
+
+
+class ExpertChoiceArgs(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("logits", "bias", "topk_w", "topk_i")] + [("stride", C.c_int64)] + \
+               [(n, C.c_int) for n in ("T", "E", "k", "scoring", "n_groups", "topk_groups", "group_top", "renormalize")] + \
+               [("weight_scale", C.c_float)]
 
 
 def needs_build() -> bool:
@@ -168,6 +189,14 @@ def load() -> C.CDLL:
         "gptoss_moe_forward_host_submit": ([ctxp, i32, i32, vp, vp], i32),
         "gptoss_moe_forward_host_sliced_submit": ([ctxp, i32, i32, vp, vp], i32),
         "gptoss_moe_forward_host_wait": ([ctxp], i32),
+        "gptoss_serving_last_error": ([], C.c_char_p),
+        "gptoss_tree_attention_workspace": ([C.POINTER(TreeAttentionArgs)], u64),
+        "gptoss_tree_attention": ([C.POINTER(TreeAttentionArgs), vp], i32),
+        "gptoss_cache_commit": ([vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp], i32),
+        "gptoss_lora_workspace": ([C.POINTER(LoraArgs)], u64),
+        "gptoss_lora_apply": ([C.POINTER(LoraArgs), vp], i32),
+        "gptoss_expert_choice": ([C.POINTER(ExpertChoiceArgs), vp], i32),
+        "gptoss_moe_forward_routed": ([ctxp, i32, i32, vp, vp, vp, vp, vp], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

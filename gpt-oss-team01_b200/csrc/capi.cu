@@ -839,6 +839,31 @@ int gptoss_moe_forward(gptoss_ctx *ctx, int layer, int T, const void *t_dev_bf16
   return gptoss_moe_add_delta(ctx, x_dev, stream);
 }
 
+// The block with the caller's routing: the rows take the place of what the router kernels would have written, and
+// everything behind them (grouping, expert GEMMs, slot-ordered sum) runs as in gptoss_moe_forward.
+int gptoss_moe_forward_routed(gptoss_ctx *ctx, int layer, int T, const void *t_dev_bf16, const int *topk_i_dev,
+                              const float *topk_w_dev, float *x_dev, void *stream) {
+  int rc = check_layer(ctx, layer, true);
+  if (rc) return rc;
+  if ((rc = check_T(ctx, T))) return rc;
+  if (ctx->world != 1) return ctx->fail(GPTOSS_ERR_UNSUPPORTED, "routing by the caller is for single-GPU contexts");
+  if (!t_dev_bf16 || !topk_i_dev || !topk_w_dev || !x_dev) return ctx->fail(GPTOSS_ERR_BAD_ARG, "null pointer");
+  if ((reinterpret_cast<uintptr_t>(t_dev_bf16) | reinterpret_cast<uintptr_t>(x_dev)) & 15u)
+    return ctx->fail(GPTOSS_ERR_BAD_ARG, "activations must be 16-byte aligned");
+  CK(cudaSetDevice(ctx->device));
+  ctx->cur_T = T;
+  if (T == 0) return GPTOSS_OK;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const size_t bytes = (size_t)T * ctx->d.k * 4;
+  CK(cudaMemcpyAsync(ctx->rb.topk_i, topk_i_dev, bytes, cudaMemcpyDeviceToDevice, s));
+  CK(cudaMemcpyAsync(ctx->rb.topk_w, topk_w_dev, bytes, cudaMemcpyDeviceToDevice, s));
+  CK(launch_pair_hist(ctx->rb.topk_i, T, ctx->d, ctx->rb.blk_hist, s));
+  if ((rc = route_group(ctx, T, t_dev_bf16, s))) return rc;
+  if ((rc = gptoss_moe_mlp1_swiglu(ctx, layer, stream))) return rc;
+  if ((rc = gptoss_moe_mlp2(ctx, layer, stream))) return rc;
+  return gptoss_moe_combine(ctx, T, x_dev, 1, stream);
+}
+
 int gptoss_moe_forward_partial(gptoss_ctx *ctx, int layer, int T, const void *t_dev_bf16, float *partial_dev,
                                void *stream) {
   if (!ctx) return GPTOSS_ERR_BAD_ARG;

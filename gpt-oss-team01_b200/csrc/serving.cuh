@@ -1,0 +1,14 @@
+// What the serving operators (tree_attention.cu, lora.cu, expert_choice.cu) share: the message of the last failing call
+// of a host thread, and the launchers that the model step calls.
+#pragma once
+
+#include "kernels.cuh"
+
+namespace gptoss {
+
+// Remembers `msg` for gptoss_serving_last_error() of this host thread and returns `code`.
+int serving_fail(int code, const char *msg, cudaError_t e = cudaSuccess);
+
+inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace gptoss

@@ -164,6 +164,15 @@ class MoEBlock:
         assert t.shape == (T, self.H) and x.shape == (T, self.H)
         self._check(self.lib.gptoss_moe_forward(self._ctx, layer, T, _ptr(t), _ptr(x), _stream(stream)))
 
+    def forward_routed(self, layer, t, topk_w, topk_i, x, stream=None):
+        """x += MoE(t) with the caller's routing (e.g. of ``serving.route_experts``): topk_w fp32 [T,k], topk_i int32 [T,k];
+        ids outside [0, n_experts) take no part."""
+        T = t.shape[0]
+        assert t.dtype == torch.bfloat16 and x.dtype == torch.float32 and t.shape == x.shape == (T, self.H)
+        assert topk_w.dtype == torch.float32 and topk_i.dtype == torch.int32 and topk_w.shape == topk_i.shape == (T, self.k)
+        self._check(self.lib.gptoss_moe_forward_routed(self._ctx, layer, T, _ptr(t), _ptr(topk_i), _ptr(topk_w), _ptr(x),
+                                                       _stream(stream)))
+
     def forward_partial(self, layer, t, partial, stream=None):
         T = t.shape[0]
         assert t.dtype == torch.bfloat16 and partial.dtype == torch.float32

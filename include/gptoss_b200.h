@@ -276,6 +276,100 @@ int gptoss_moe_build_offsets_noalloc(int T, int n_experts, int top_k, const int 
 /* Message of the last failing gptoss_moe_build_offsets_noalloc call on this host thread ("" if none). */
 const char *gptoss_noalloc_last_error(void);
 
+/* ---- serving operators on caller-supplied device buffers -----------------------------------------------------------
+ * What a serving loop needs beside the reference's one-token greedy step (getp-csrc/submit/getp_run_submit.cpp:60-96):
+ * verification of drafted tokens, adapters per request, other routing rules.  No context: they work on the CURRENT
+ * device, are asynchronous on `stream`, allocate nothing, keep nothing between calls and can be captured into a CUDA
+ * graph.  Arguments are checked on the host; counts and indices that live on the device are bounded by the kernels, so
+ * that a bad one never reaches memory outside the tensors, but what it yields is not specified beyond what is said here.
+ * A workspace belongs to one call at a time: two calls (or captured graphs) that may overlap need two. */
+/* Message of the last failing call of these operators on this host thread ("" if none). */
+const char *gptoss_serving_last_error(void);
+
+/* Attention of drafted tokens over the KV cache.  Sequence b has the ctx_len[b] cached tokens of cache row rows[b], and
+ * a tree of n_b = offsets[b+1] - offsets[b] drafted tokens (rows offsets[b].. of q and out), whose K and V already stand
+ * in the cache, drafted token i in slot ctx_len[b] + i.  Query i attends to every cached token and to the drafted tokens
+ * j whose bit is set in its mask (bit j & 31 of word j >> 5; its own bit included, if it shall see itself).  With a
+ * window > 0 it attends only to tokens less than `window` positions before its own, the position of a drafted token
+ * being ctx_len[b] + depth (run.cpp:582).  Softmax in fp32, the sink joins the denominator only (run.cpp:588-591); a
+ * query that attends to nothing gets zeros.  K and V rows that no query of the tree attends to, and masked ones, may
+ * hold anything, NaN included.  Rows of out behind offsets[n_seqs] are left as they were.
+ * bf16: q [n_tokens][n_q_heads][head_dim], token stride q_stride elements (a multiple of 8); caches
+ * [cache_rows][n_kv_heads][max_seq][head_dim]; out like q.  All 16-byte aligned.  head_dim 32 or 64, 1 to 8 query heads
+ * per kv head, up to GPTOSS_TREE_MAX_NODES drafted tokens per sequence, ctx_len[b] + n_b <= max_seq.
+ * max_nodes must not be below the largest n_b (further tokens of a sequence are not computed); max_ctx sizes the launch:
+ * the result is right for any ctx_len, the work is spread best when max_ctx is the largest. */
+#define GPTOSS_TREE_MAX_NODES 256
+typedef struct {
+  const void *q, *k_cache, *v_cache;
+  void *out;
+  const int *offsets;   /* [n_seqs + 1] */
+  const int *ctx_len;   /* [n_seqs] */
+  const int *rows;      /* [n_seqs] cache row of each sequence; NULL: sequence b in row b */
+  const int *mask;      /* [n_tokens][mask_words] */
+  const int *depth;     /* [n_tokens] 0 for a child of the last cached token; read only with a window */
+  const float *sinks;   /* [n_q_heads], or NULL for none */
+  void *workspace;      /* gptoss_tree_attention_workspace() bytes, 16-byte aligned (NULL if 0) */
+  uint64_t workspace_bytes;
+  int64_t q_stride, out_stride;
+  int n_tokens, n_seqs, max_nodes, max_ctx, mask_words;
+  int cache_rows, max_seq, n_q_heads, n_kv_heads, head_dim;
+  int window;           /* 0: none */
+  float scale;          /* of the scores, 1/sqrt(head_dim) as a rule */
+} gptoss_tree_attention_args;
+uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *args);
+int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream);
+
+/* Moves the accepted path of each tree into place: path[offsets[b] + j], ascending, is the drafted token that becomes the
+ * j-th new token of sequence b; its K and V move from slot ctx_len[b] + path to slot ctx_len[b] + j in every layer of the
+ * caches [n_layers][cache_rows][n_kv_heads][max_seq][head_dim] (bf16).  Other slots are left as they were.  No path is
+ * longer than max_path.  Sequences must name distinct cache rows. */
+int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_rows, int n_kv_heads, int max_seq, int head_dim,
+                        int n_seqs, const int *rows, const int *ctx_len, const int *offsets, const int *path, int max_path,
+                        void *stream);
+
+/* Adapters beside a shared projection: out[t] = y[t] + scale[a] * B_a (A_a x[t]) with a = ids[t]; a token whose id is
+ * outside [0, n_adapters) has no adapter (out[t] = y[t]).  x [T][K] bf16, a [n_adapters][rank][K] bf16,
+ * b [n_adapters][n_out][rank] bf16, scale [n_adapters] fp32 or NULL for 1, y and out [T][n_out] fp32; out may be y.
+ * Products accumulate in fp32 and the intermediate A x is not rounded.  K and n_out multiples of 8, rank a
+ * multiple of 8 up to GPTOSS_LORA_MAX_RANK (adapters of lower rank: zero rows of A, zero columns of B). */
+#define GPTOSS_LORA_MAX_RANK 128
+typedef struct {
+  const void *x, *a, *b;
+  const float *scale;
+  const int *ids;       /* [T], any order */
+  const float *y;
+  float *out;
+  void *workspace;      /* gptoss_lora_workspace() bytes, 16-byte aligned */
+  uint64_t workspace_bytes;
+  int64_t x_stride, y_stride, out_stride; /* elements from row to row */
+  int T, K, n_out, rank, n_adapters;
+} gptoss_lora_args;
+uint64_t gptoss_lora_workspace(const gptoss_lora_args *args);
+int gptoss_lora_apply(const gptoss_lora_args *args, void *stream);
+
+/* Experts of each token from router logits [T][E] fp32 (row stride `stride`): scores = softmax over the E logits, or
+ * sigmoid; choice = score + bias (NULL: 0).  With n_groups > 1 the experts form equal groups of neighbours, a group is
+ * worth the sum of its group_top (1 or 2) largest choices, and only the topk_groups best groups take part.  The k largest
+ * choices are taken, in descending order; of equal ones, of groups and of experts, the lowest index comes first.
+ * topk_w = their scores (without the bias), divided by their sum with renormalize, times weight_scale.
+ * A NaN logit scores 0, a NaN choice counts as -infinity.  Compared in fp64.  E <= 256, k <= 8, n_groups <= 32. */
+#define GPTOSS_SCORE_SOFTMAX 0
+#define GPTOSS_SCORE_SIGMOID 1
+typedef struct {
+  const float *logits, *bias;
+  float *topk_w;        /* [T][k] */
+  int *topk_i;          /* [T][k] */
+  int64_t stride;
+  int T, E, k, scoring, n_groups, topk_groups, group_top, renormalize;
+  float weight_scale;
+} gptoss_expert_choice_args;
+int gptoss_expert_choice(const gptoss_expert_choice_args *args, void *stream);
+/* gptoss_moe_forward with the caller's routing instead of the layer's router: topk_i [T][k], topk_w [T][k] on the device,
+ * in any order, experts may repeat, ids outside [0, n_experts) take no part.  Single-GPU contexts only. */
+int gptoss_moe_forward_routed(gptoss_ctx *ctx, int layer, int T, const void *t_dev_bf16, const int *topk_i_dev,
+                              const float *topk_w_dev, float *x_dev, void *stream);
+
 /* ---- taps (debug/parity; the reference's DEBUG printDebug, getp-csrc/src/model.cpp:205-450) -------- */
 #define GPTOSS_TAP_SCORES 0    /* fp32 [T,E]   router scores incl. bias                            */
 #define GPTOSS_TAP_TOPK_W 1    /* fp32 [T,k]   gate weights                                        */
