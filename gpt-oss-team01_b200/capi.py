@@ -46,7 +46,7 @@ EXPORTS = [
     "gptoss_moe_dispatch_route", "gptoss_moe_dispatch_rows", "gptoss_moe_dispatch_push", "gptoss_moe_forward_dispatch",
     "gptoss_launch_count", "gptoss_argmax_rows", "gptoss_model_step_rows", "gptoss_model_step_seqs",
     "gptoss_moe_forward_host_submit", "gptoss_moe_forward_host_sliced_submit", "gptoss_moe_forward_host_wait",
-    "gptoss_model_layer_moe_dispatch", "gptoss_serving_last_error", "gptoss_tree_attention_workspace", "gptoss_tree_attention",
+    "gptoss_model_layer_moe_dispatch", "gptoss_serving_last_error", "gptoss_serving_status", "gptoss_tree_attention_workspace", "gptoss_tree_attention",
     "gptoss_cache_commit", "gptoss_lora_workspace", "gptoss_lora_apply", "gptoss_expert_choice", "gptoss_moe_forward_routed",
 ]
 
@@ -190,6 +190,7 @@ def load() -> C.CDLL:
         "gptoss_moe_forward_host_sliced_submit": ([ctxp, i32, i32, vp, vp], i32),
         "gptoss_moe_forward_host_wait": ([ctxp], i32),
         "gptoss_serving_last_error": ([], C.c_char_p),
+        "gptoss_serving_status": ([], i32),
         "gptoss_tree_attention_workspace": ([C.POINTER(TreeAttentionArgs)], u64),
         "gptoss_tree_attention": ([C.POINTER(TreeAttentionArgs), vp], i32),
         "gptoss_cache_commit": ([vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp], i32),

@@ -2,10 +2,12 @@
 // place.  Both replace nothing in the reference, which decodes one token per sequence and step
 // (getp-csrc/src/model.cpp:6-151); the attention is that of run.cpp:565-607 (learned sink in the denominator, sliding
 // window) for many queries per sequence under a mask.
-#include <cfloat>
+#include <cmath>
 #include <cstdio>
+#include <cstring>
 
 #include "serving.cuh"
+#include "tcgen05.cuh"
 
 namespace gptoss {
 
@@ -13,79 +15,454 @@ namespace {
 
 thread_local char g_serving_error[256] = "";
 
-// One warp per (drafted token, query head); lane = cached position.  The plain statement of the operator.
+// ---- kernel ---------------------------------------------------------------------------------------------------------
+// One CTA per (sequence, kv head, tile of up to 128 query rows, share of the context).  A query row is a (drafted token,
+// head of the group) pair, so a tree of n tokens with g heads per kv head gives n g rows that all read the same K and V.
+// Per tile of 128 slots:   S = Q K^T   (tcgen05, accumulator in TMEM)
+//                          P = 2^(c S - m), c = scale log2(e), in the registers of one thread per row, bf16 to TMEM
+//                          O += P V    (tcgen05, A operand from TMEM; V as it lies in the cache, K-index outermost)
+// m is a running reference, not the running maximum: it moves (and O is rescaled in TMEM) only when the maximum has grown
+// by more than 2^8, so that most tiles leave O alone; P and O stay below 2^8 times their usual range.  P is rounded to
+// bf16, the type of V (both operands of the product have the same type); the denominator adds the unrounded values.
+// S is read into registers at once, which frees its TMEM columns for the next tile's QK^T while this tile's exponentials
+// run; with 256 of the 512 TMEM columns and under 114 KiB of shared memory two CTAs share an SM, so the exponentials of
+// one overlap the products of the other.
+//
+// Tiles that every row sees whole skip all masking.  In the others (the window's edge, the drafted slots, the end) each
+// thread builds a 128-bit mask of its row.  What a row must not see still goes through P V as 0 * V, so in those tiles
+// the non-finite elements of V are replaced by zeros in shared memory; the epilogue adds them back to the rows that do
+// see them.
+constexpr int kAttRows = 128, kAttTile = 128;     // query rows per CTA, slots per tile
+constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 bytes (head_dim 32: the upper half is zero-filled)
+constexpr int kAttKStages = 3, kAttVStages = 2;
+constexpr int kAttThreads = 192;                  // 4 softmax warps, the copy warp, the MMA warp
+constexpr int kMaxPoison = 768;                   // slots of masked tiles that can hold a non-finite V element
+constexpr uint32_t kTmemS = 0, kTmemP = 128, kTmemO = 192, kAttTmemCols = 256;
+
+struct AttCtrl {
+  uint64_t k_full[kAttKStages], k_empty[kAttKStages], v_full[kAttVStages], v_empty[kAttVStages];
+  uint64_t s_full, s_empty, p_full, pv_done, mma_done;
+  uint32_t tmem_base;
+  int abort, depth_lo, depth_hi, n_poison;
+  int poison[kMaxPoison];
+};
+constexpr size_t kAttSmem = kAttTileBytes * (1 + kAttKStages + kAttVStages) + 1024 + sizeof(AttCtrl);
+
+struct AttParams {
+  CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 128, 1}
+  gptoss_tree_attention_args a;
+  int group, nodes_per_tile, q_tiles, n_splits, tiles_per_split;
+  float c;                   // scale * log2(e)
+};
+
+__device__ int g_serving_status[kStatusWords];
+
+// Slots [slot0, slot0 + 32) that a row sees, one bit each.
+struct RowView {
+  int ctx, n_keys, lo, window, depth, words;
+  const int *mask, *depths;  // of this row's token; of the sequence's first token
+  __device__ __forceinline__ uint32_t word(int slot0) const {
+    uint32_t w = 0;
+    const int a = max(lo - slot0, 0), z = min(ctx - slot0, 32);
+    if (z > a) w = (z == 32 ? 0xffffffffu : (1u << z) - 1u) & ~((1u << a) - 1u);
+    const int nb = slot0 - ctx;  // drafted token of bit 0
+    if (nb > -32 && nb < n_keys) {
+      const int i = nb >> 5;
+      const uint32_t w0 = i >= 0 && i < words ? (uint32_t)mask[i] : 0u, w1 = i + 1 < words ? (uint32_t)mask[i + 1] : 0u;
+      uint32_t bits = __funnelshift_r(w0, w1, nb & 31);
+      if (n_keys - nb < 32) bits &= (1u << (n_keys - nb)) - 1u;
+      if (window > 0 && depth >= window)  // a path longer than the window
+        for (uint32_t left = bits; left; left &= left - 1) {
+          const int j = __ffs(left) - 1;
+          if (depths[nb + j] <= depth - window) bits &= ~(1u << j);
+        }
+      w |= bits;
+    }
+    return w;
+  }
+};
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float *r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]), "=f"(r[9]),
+        "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]), "=f"(r[17]), "=f"(r[18]),
+        "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]), "=f"(r[25]), "=f"(r[26]), "=f"(r[27]),
+        "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+        "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// D[tmem] (+)= A[tmem] * B[smem], bf16, M = 128, K = 16
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Descriptor of a V tile as the B operand with its N index (dims) innermost: 64 dims are one 128-byte swizzle row, groups
+// of 8 slots are 1024 bytes apart; the stride between swizzle rows along N is not used.
+__device__ __forceinline__ uint64_t smem_desc_v(uint32_t addr) {
+  const uint32_t lo = ((addr & 0x3FFFFu) >> 4) | ((1024u >> 4) << 16);
+  const uint32_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+  return ((uint64_t)hi << 32) | lo;
+}
+constexpr uint32_t kIdescTransposeB = 1u << 16;
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ bool bf16_nonfinite(uint32_t pair) {
+  return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
+}
+__device__ __forceinline__ uint32_t bf16_finite_part(uint32_t pair) {
+  return pair & ((pair & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((pair & 0x7f800000u) == 0x7f800000u ? 0x0000ffffu : ~0u);
+}
+
+// mbar_wait in line: around a call the compiler would spill the row of scores that a softmax thread holds.
+__device__ __forceinline__ void wait_here(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
+  const uint32_t addr = smem_u32(bar);
+  volatile int *ab = abort_flag;
+  uint32_t i = 0;
+  while (!mbar_try_wait(addr, parity)) {
+    if (*ab) return;
+    if (++i == kSpinLimit) {
+      *ab = 1;
+      if (atomicCAS(g_serving_status, 0, kDevErrTimeout) == 0) g_serving_status[1] = site, g_serving_status[2] = (int)blockIdx.x;
+      return;
+    }
+  }
+}
+
 template <int HD>
-__global__ void __launch_bounds__(128) tree_attention_kernel(gptoss_tree_attention_args a) {
-  constexpr int DL = HD / 32;  // dims of the output per lane
-  __shared__ float q_s[4][HD];
+__global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __grid_constant__ AttParams p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t q_s = (raw + 1023u) & ~1023u, k_s = q_s + kAttTileBytes, v_s = k_s + kAttKStages * kAttTileBytes;
+  uint8_t *const smem = smem_raw + (q_s - raw);
+  AttCtrl *ctrl = reinterpret_cast<AttCtrl *>(smem + kAttTileBytes * (1 + kAttKStages + kAttVStages));
+  const gptoss_tree_attention_args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int b = blockIdx.x / a.max_nodes, i = blockIdx.x % a.max_nodes;
-  const int h = blockIdx.y * 4 + warp;
+  int x = blockIdx.x;
+  const int qt = x % p.q_tiles;
+  x /= p.q_tiles;
+  const int split = x % p.n_splits;
+  x /= p.n_splits;
+  const int kvh = x % a.n_kv_heads, b = x / a.n_kv_heads;
   pdl_wait();
-  pdl_launch_dependents();
-  if (h >= a.n_q_heads) return;
   const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
-  if (first < 0 || i >= n) return;
-  const int tok = first + i;
+  const int n0 = qt * p.nodes_per_tile, nodes = min(n - n0, p.nodes_per_tile);
+  if (first < 0 || nodes <= 0) {
+    pdl_launch_dependents();
+    return;
+  }
   const int row = a.rows ? a.rows[b] : b;
   int ctx = min(max(a.ctx_len[b], 0), a.max_seq);
   int len = min(ctx + n, a.max_seq);
   if (row < 0 || row >= a.cache_rows) ctx = len = 0;
-  const int pos = a.window > 0 ? ctx + a.depth[tok] : 0;
-  const int lo = a.window > 0 ? max(0, min(pos - a.window + 1, ctx)) : 0;
-  const int kvh = h / (a.n_q_heads / a.n_kv_heads);
-  const uint16_t *kb = static_cast<const uint16_t *>(a.k_cache) + ((size_t)row * a.n_kv_heads + kvh) * a.max_seq * HD;
-  const uint16_t *vb = static_cast<const uint16_t *>(a.v_cache) + ((size_t)row * a.n_kv_heads + kvh) * a.max_seq * HD;
-  const uint16_t *qp = static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + h * HD;
-  for (int d = lane; d < HD; d += 32) q_s[warp][d] = __uint_as_float((uint32_t)qp[d] << 16);
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, o[DL];
+  const int slab = row * a.n_kv_heads + kvh;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kAttKStages; ++i) mbar_init(smem_u32(&ctrl->k_full[i]), 1), mbar_init(smem_u32(&ctrl->k_empty[i]), 1);
+    for (int i = 0; i < kAttVStages; ++i) mbar_init(smem_u32(&ctrl->v_full[i]), 1), mbar_init(smem_u32(&ctrl->v_empty[i]), 1);
+    mbar_init(smem_u32(&ctrl->s_full), 1);
+    mbar_init(smem_u32(&ctrl->s_empty), 4);
+    mbar_init(smem_u32(&ctrl->p_full), 4);
+    mbar_init(smem_u32(&ctrl->pv_done), 1);
+    mbar_init(smem_u32(&ctrl->mma_done), 1);
+    ctrl->abort = 0, ctrl->n_poison = 0, ctrl->depth_lo = 0x3fffffff, ctrl->depth_hi = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 5) {
+    tmem_alloc(smem_u32(&ctrl->tmem_base), kAttTmemCols);
+    tmem_relinquish();
+  }
+  // query rows into shared memory, in the layout a 128-byte-swizzled copy would give them (rows beyond the tree hold
+  // whatever lies there: a row of the products depends on its own row of Q only)
+  const int r = threadIdx.x, node = r / p.group, head = kvh * p.group + r % p.group;
+  const bool valid = r < kAttRows && node < nodes;
+  const int tok = first + n0 + (valid ? node : 0);
+  if (valid) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
 #pragma unroll
-  for (int d = 0; d < DL; ++d) o[d] = 0.f;
-  for (int j0 = lo; j0 < len; j0 += 32) {
-    const int j = j0 + lane;
-    bool seen = j < len;
-    if (seen && j >= ctx) {
-      const int node = j - ctx;
-      seen = (a.mask[(size_t)tok * a.mask_words + (node >> 5)] >> (node & 31)) & 1;
-      if (a.window > 0) seen = seen && ctx + a.depth[first + node] > pos - a.window;
+    for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + r * 128 + ((c ^ (r & 7)) << 4)) = src[c];
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const int depth = a.window > 0 && valid ? min(max(a.depth[tok], 0), kMaxPoison) : 0;
+  if (a.window > 0) {
+    if (valid) atomicMin(&ctrl->depth_lo, depth), atomicMax(&ctrl->depth_hi, depth);
+    __syncthreads();
+  }
+  const uint32_t tmem = ctrl->tmem_base;
+  const int lo_min = a.window > 0 ? min(max(ctx + ctrl->depth_lo - a.window + 1, 0), ctx) : 0;
+  const int lo_max = a.window > 0 ? min(max(ctx + ctrl->depth_hi - a.window + 1, 0), ctx) : 0;
+  const int tiles = (len - lo_min + kAttTile - 1) / kAttTile;
+  const int t_begin = min(tiles, split * p.tiles_per_split);
+  const int n_tiles = (split == p.n_splits - 1 ? tiles : min(tiles, t_begin + p.tiles_per_split)) - t_begin;
+  const int slot_first = lo_min + t_begin * kAttTile;
+
+  if (warp == 4) {
+    // ===================== copies =====================
+    if (lane == 0) {
+      int i = 0;
+      for (; i < n_tiles; ++i) {
+        const int ks = i % kAttKStages, vs = i % kAttVStages;
+        bool ok = mbar_wait(smem_u32(&ctrl->k_empty[ks]), ((i / kAttKStages) & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2000 | ks);
+        if (!ok) break;
+        mbar_expect_tx(smem_u32(&ctrl->k_full[ks]), kAttTileBytes);
+        tma_load_3d(k_s + ks * kAttTileBytes, &p.map_k, smem_u32(&ctrl->k_full[ks]), 0, slot_first + i * kAttTile, slab);
+        ok = mbar_wait(smem_u32(&ctrl->v_empty[vs]), ((i / kAttVStages) & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2100 | vs);
+        mbar_expect_tx(smem_u32(&ctrl->v_full[vs]), kAttTileBytes);
+        tma_load_3d(v_s + vs * kAttTileBytes, &p.map_v, smem_u32(&ctrl->v_full[vs]), 0, slot_first + i * kAttTile, slab);
+        if (!ok) {
+          ++i;
+          break;
+        }
+      }
+      if (i < n_tiles || *reinterpret_cast<volatile int *>(&ctrl->abort)) {
+        // gave up: the copies in flight have to land before the CTA's shared memory is given away
+        for (int j = max(0, i - kAttKStages); j < i; ++j)
+          for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->k_full[j % kAttKStages]), (j / kAttKStages) & 1); ++w) {}
+        for (int j = max(0, i - kAttVStages); j < i; ++j)
+          for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->v_full[j % kAttVStages]), (j / kAttVStages) & 1); ++w) {}
+      }
     }
-    float s = -INFINITY;
-    if (seen) {
-      s = 0.f;
-      for (int d = 0; d < HD; ++d) s = fmaf(q_s[warp][d], __uint_as_float((uint32_t)kb[(size_t)j * HD + d] << 16), s);
-      s *= a.scale;
+  } else if (warp == 5) {
+    // ===================== products =====================
+    if (lane == 0) {
+      const uint32_t idesc_s = umma_idesc(kAttTile), idesc_o = umma_idesc(HD) | kIdescTransposeB;
+      const uint64_t dq = smem_desc_sw128(q_s);
+      auto scores = [&](int i) {
+        const int ks = i % kAttKStages;
+        mbar_wait(smem_u32(&ctrl->k_full[ks]), (i / kAttKStages) & 1, &ctrl->abort, g_serving_status, 0x2200 | ks);
+        mbar_wait(smem_u32(&ctrl->s_empty), (i & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2300);
+        tc_fence_after();
+        const uint64_t dk = smem_desc_sw128(k_s + ks * kAttTileBytes);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) umma_bf16(tmem + kTmemS, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, k > 0);
+        umma_commit(smem_u32(&ctrl->s_full));
+        umma_commit(smem_u32(&ctrl->k_empty[ks]));
+      };
+      if (n_tiles > 0) scores(0);
+      for (int i = 0; i < n_tiles; ++i) {
+        if (i + 1 < n_tiles) scores(i + 1);
+        const int vs = i % kAttVStages;
+        mbar_wait(smem_u32(&ctrl->v_full[vs]), (i / kAttVStages) & 1, &ctrl->abort, g_serving_status, 0x2400 | vs);
+        mbar_wait(smem_u32(&ctrl->p_full), i & 1, &ctrl->abort, g_serving_status, 0x2500);
+        tc_fence_after();
+        const uint64_t dv = smem_desc_v(v_s + vs * kAttTileBytes);
+#pragma unroll
+        for (int k = 0; k < kAttTile / 16; ++k)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V
+          umma_bf16_ts(tmem + kTmemO, tmem + kTmemP + 8 * k, dv + (uint64_t)(128 * k), idesc_o, (i | k) != 0);
+        umma_commit(smem_u32(&ctrl->pv_done));
+        umma_commit(smem_u32(&ctrl->v_empty[vs]));
+      }
+      if (*reinterpret_cast<volatile int *>(&ctrl->abort)) {  // what was issued has to retire before TMEM is given up
+        umma_commit(smem_u32(&ctrl->mma_done));
+        for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->mma_done), 0); ++w) {}
+      }
     }
-    float mx = s;
+  } else {
+    // ===================== softmax, a thread per query row =====================
+    RowView view{ctx, len - ctx, a.window > 0 ? min(max(ctx + depth - a.window + 1, 0), ctx) : 0, a.window, depth, a.mask_words,
+                 a.mask + (size_t)tok * a.mask_words, a.depth + first};
+    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+    const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < n_tiles; ++i) {
+      const int t0 = slot_first + i * kAttTile;
+      const bool masked = t0 < lo_max || t0 + kAttTile > ctx;
+      uint32_t bits[4];
+      if (masked) {
 #pragma unroll
-    for (int x = 16; x >= 1; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-    const float m_new = fmaxf(m, mx);
-    const float base = m_new == -INFINITY ? 0.f : m_new;
-    const float corr = expf(m - base);
-    const float p = seen ? expf(s - base) : 0.f;
-    l = l * corr + p;
-    m = m_new;
+        for (int w = 0; w < 4; ++w) bits[w] = valid ? view.word(t0 + 32 * w) : 0u;
+        // slot r of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
+        const int vs = i % kAttVStages;
+        wait_here(&ctrl->v_full[vs], (i / kAttVStages) & 1, &ctrl->abort, 0x2700);
+        uint4 *vr = reinterpret_cast<uint4 *>(smem + (1 + kAttKStages + vs) * kAttTileBytes + r * 128);
+        bool bad = false;
 #pragma unroll
-    for (int d = 0; d < DL; ++d) o[d] *= corr;
-    uint32_t some = __ballot_sync(0xffffffffu, seen);
-    while (some) {
-      const int x = __ffs(some) - 1;
-      some &= some - 1;
-      const float px = __shfl_sync(0xffffffffu, p, x);
+        for (int c = 0; c < 8; ++c) {
+          uint4 v = vr[(c + r) & 7];
+          if (bf16_nonfinite(v.x) || bf16_nonfinite(v.y) || bf16_nonfinite(v.z) || bf16_nonfinite(v.w)) {
+            bad = true;
+            v.x = bf16_finite_part(v.x), v.y = bf16_finite_part(v.y), v.z = bf16_finite_part(v.z), v.w = bf16_finite_part(v.w);
+            vr[(c + r) & 7] = v;
+          }
+        }
+        if (bad && t0 + r < len) {
+          const int at = atomicAdd(&ctrl->n_poison, 1);
+          if (at < kMaxPoison) ctrl->poison[at] = t0 + r;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      }
+      float s[kAttTile];
+      wait_here(&ctrl->s_full, i & 1, &ctrl->abort, 0x2600);
+      tc_fence_after();
+      if (live) {
 #pragma unroll
-      for (int d = 0; d < DL; ++d)
-        o[d] = fmaf(px, __uint_as_float((uint32_t)vb[(size_t)(j0 + x) * HD + lane * DL + d] << 16), o[d]);
+        for (int j = 0; j < kAttTile; j += 32) tmem_ld32(tmem + lane_addr + kTmemS + j, s + j);
+        tmem_ld_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctrl->s_empty));
+      bool move = false;
+      float corr = 1.f;
+      if (live) {
+        if (masked) {
+#pragma unroll
+          for (int j = 0; j < kAttTile; ++j) s[j] = (bits[j >> 5] >> (j & 31) & 1u) ? s[j] : -INFINITY;
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < kAttTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c;
+        move = top > m + 8.f;
+        if (move) {
+          corr = ex2(m - top);
+          m = top;
+        }
+      }
+      // the product before this one has read P and written O (warps without rows wait too: nobody may arrive for this
+      // tile's P before the last one's has been taken)
+      if (i > 0) wait_here(&ctrl->pv_done, (i - 1) & 1, &ctrl->abort, 0x2800);
+      tc_fence_after();
+      if (live) {
+        if (i > 0 && __any_sync(0xffffffffu, move)) {
+#pragma unroll
+          for (int h = 0; h < HD; h += 16) {
+            uint32_t o[16];
+            tmem_ld16(tmem + lane_addr + kTmemO + h, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+            tmem_st16(tmem + lane_addr + kTmemO + h, o);
+          }
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < kAttTile; h += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float e0 = ex2(fmaf(s[h + j], p.c, -base)), e1 = ex2(fmaf(s[h + j + 1], p.c, -base));
+            sum[(j >> 1) & 3] += e0 + e1;
+            pk[j >> 1] = pack_bf16(e0, e1);
+          }
+          tmem_st16(tmem + lane_addr + kTmemP + (h >> 1), pk);
+        }
+        l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full));
+    }
+    // ---- result of this share of the context ----
+    if (n_tiles > 0) wait_here(&ctrl->pv_done, (n_tiles - 1) & 1, &ctrl->abort, 0x2900);
+    asm volatile("bar.sync 1, 128;" ::: "memory");  // every note of a non-finite element is in place
+    tc_fence_after();
+    if (live) {
+      float o[HD];
+#pragma unroll
+      for (int j = 0; j < HD; ++j) o[j] = 0.f;
+      if (n_tiles > 0) {
+#pragma unroll
+        for (int h = 0; h < HD; h += 32) tmem_ld32(tmem + lane_addr + kTmemO + h, o + h);
+        tmem_ld_wait();
+      }
+      if (valid) {
+        const int bad = min(ctrl->n_poison, kMaxPoison);
+        for (int i = 0; i < bad; ++i) {
+          const int slot = ctrl->poison[i];
+          if (!(view.word(slot) & 1u)) continue;
+          const uint16_t *v = static_cast<const uint16_t *>(a.v_cache) + ((size_t)slab * a.max_seq + slot) * HD;
+#pragma unroll
+          for (int j = 0; j < HD; ++j)
+            if ((v[j] & 0x7f80u) == 0x7f80u) o[j] += __uint_as_float((uint32_t)v[j] << 16);
+        }
+        if (p.n_splits == 1) {
+          const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
+          const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+          const float w = ex2(m - base), total = fmaf(l, w, ex2(sink - base));
+          const float inv = total == 0.f ? 0.f : w / total;
+          uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (size_t)tok * a.out_stride + (size_t)head * HD);
+#pragma unroll
+          for (int j = 0; j < HD; j += 8)
+            dst[j >> 3] = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
+                                     pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+        } else {
+          const size_t at = ((size_t)split * a.n_tokens + tok) * a.n_q_heads + head;
+          float4 *dst = static_cast<float4 *>(a.workspace) + at * (HD / 4);
+#pragma unroll
+          for (int j = 0; j < HD; j += 4) dst[j >> 2] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+          float2 *ml = reinterpret_cast<float2 *>(static_cast<float *>(a.workspace) + (size_t)p.n_splits * a.n_tokens * a.n_q_heads * HD);
+          ml[at] = make_float2(m, l);
+        }
+      }
     }
   }
-#pragma unroll
-  for (int x = 16; x >= 1; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  const float sink = a.sinks ? a.sinks[h] : -INFINITY;
-  const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
-  const float c = expf(m - base), total = l * c + expf(sink - base);
-  const float inv = total > 0.f ? c / total : (total == 0.f ? 0.f : total);
-  __nv_bfloat16 *op = static_cast<__nv_bfloat16 *>(a.out) + (size_t)tok * a.out_stride + h * HD + lane * DL;
-#pragma unroll
-  for (int d = 0; d < DL; ++d) op[d] = __float2bfloat16_rn(o[d] * inv);
+  pdl_launch_dependents();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, kAttTmemCols);
+  }
+}
+
+// Joins the shares of the context: out = sum_s O_s 2^(m_s - M) / (sum_s l_s 2^(m_s - M) + 2^(sink - M)).  HD / 4 threads
+// per (drafted token, head); the shares are added in their order, whatever order they finished in.
+template <int HD>
+__global__ void __launch_bounds__(256) tree_merge_kernel(gptoss_tree_attention_args a, int n_splits) {
+  constexpr int TPR = HD / 4;
+  const int h = blockIdx.y * (256 / TPR) + threadIdx.x / TPR, d4 = threadIdx.x % TPR;
+  const int b = blockIdx.x / a.max_nodes, i = blockIdx.x % a.max_nodes;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int first = a.offsets[b], n = min(a.offsets[b + 1], a.n_tokens) - first;
+  if (first < 0 || i >= n || h >= a.n_q_heads) return;
+  const int tok = first + i;
+  const size_t step = (size_t)a.n_tokens * a.n_q_heads, at = (size_t)tok * a.n_q_heads + h;
+  const float4 *o = static_cast<const float4 *>(a.workspace) + at * TPR + d4;
+  const float2 *ml = reinterpret_cast<const float2 *>(static_cast<const float *>(a.workspace) + (size_t)n_splits * step * HD) + at;
+  const float sink = a.sinks ? a.sinks[h] * 1.44269504f : -INFINITY;
+  float top = sink;
+  for (int s = 0; s < n_splits; ++s) top = fmaxf(top, ml[s * step].x);
+  const float base = top == -INFINITY ? 0.f : top;
+  float total = ex2(sink - base);
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < n_splits; ++s) {
+    const float2 x = ml[s * step];
+    const float w = ex2(x.x - base);
+    const float4 v = o[s * step * TPR];
+    total = fmaf(x.y, w, total);
+    acc.x = fmaf(v.x, w, acc.x), acc.y = fmaf(v.y, w, acc.y), acc.z = fmaf(v.z, w, acc.z), acc.w = fmaf(v.w, w, acc.w);
+  }
+  const float inv = total == 0.f ? 0.f : 1.f / total;
+  *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (size_t)tok * a.out_stride + (size_t)h * HD + 4 * d4) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
 }
 
 // One warp per (layer, sequence, kv head).  Row path[j] moves to row j of the drafted rows; path ascends, so path[j] >= j
@@ -141,9 +518,70 @@ using namespace gptoss;
 
 extern "C" const char *gptoss_serving_last_error(void) { return g_serving_error; }
 
+namespace {
+
+// How a call is cut: query tiles, and shares of the context when the (sequence, kv head, query tile) items alone would not
+// fill two CTAs on every SM.
+struct AttPlan {
+  int group, nodes_per_tile, q_tiles, n_splits, tiles_per_split;
+};
+AttPlan plan_of(const gptoss_tree_attention_args &a) {
+  AttPlan p;
+  p.group = a.n_q_heads / a.n_kv_heads;
+  p.nodes_per_tile = kAttRows / p.group;
+  p.q_tiles = (a.max_nodes + p.nodes_per_tile - 1) / p.nodes_per_tile;
+  int device = 0, sms = kSmCountFallback;
+  if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  const long long items = (long long)a.n_seqs * a.n_kv_heads * p.q_tiles;
+  // the cached tokens that a tree can reach: with a window, as many as its first token sees
+  const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
+  const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
+  long long splits = items > 0 ? (2ll * sms + items - 1) / items : 1;
+  if (splits > tiles) splits = tiles;
+  if (splits < 1) splits = 1;
+  p.tiles_per_split = (int)((tiles + splits - 1) / splits);
+  p.n_splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
+  return p;
+}
+
+bool countable(const gptoss_tree_attention_args &a) {
+  return a.n_seqs > 0 && a.n_tokens > 0 && a.max_nodes > 0 && a.max_nodes <= GPTOSS_TREE_MAX_NODES && a.max_ctx >= 0 && a.n_kv_heads > 0 &&
+         a.n_q_heads > 0 && a.n_q_heads % a.n_kv_heads == 0 && a.n_q_heads / a.n_kv_heads <= 8 && (a.head_dim == 32 || a.head_dim == 64);
+}
+
+uint64_t workspace_of(const gptoss_tree_attention_args &a, int n_splits) {
+  return n_splits <= 1 ? 0 : (uint64_t)n_splits * a.n_tokens * a.n_q_heads * (a.head_dim + 2) * sizeof(float);
+}
+
+template <int HD>
+cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
+  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
+  if (e != cudaSuccess) return e;
+  const dim3 grid((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_tiles * p.n_splits));
+  e = launch_chain(tree_attention_kernel<HD>, grid, dim3(kAttThreads), kAttSmem, s, p);
+  if (e != cudaSuccess || p.n_splits == 1) return e;
+  const int heads = 256 / (HD / 4);
+  return launch_chain(tree_merge_kernel<HD>, dim3(p.a.n_seqs * p.a.max_nodes, (p.a.n_q_heads + heads - 1) / heads), dim3(256), 0, s,
+                      p.a, p.n_splits);
+}
+
+}  // namespace
+
 extern "C" uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *a) {
-  (void)a;
-  return 0;
+  return a && countable(*a) ? workspace_of(*a, plan_of(*a).n_splits) : 0;
+}
+
+extern "C" int gptoss_serving_status(void) {
+  int st[kStatusWords];
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(st, g_serving_status, sizeof st);
+  if (e != cudaSuccess) return serving_fail(GPTOSS_ERR_CUDA, "gptoss_serving_status", e);
+  if (st[0] == 0) return GPTOSS_OK;
+  char msg[128];
+  snprintf(msg, sizeof msg, "device-side bounded wait gave up in a serving operator (site 0x%x)", st[1]);
+  memset(st, 0, sizeof st);
+  cudaMemcpyToSymbol(g_serving_status, st, sizeof st);
+  return serving_fail(GPTOSS_ERR_TIMEOUT, msg);
 }
 
 extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream) {
@@ -162,15 +600,27 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
   if (!a.q || !a.k_cache || !a.v_cache || !a.offsets || !a.ctx_len || !a.mask || !a.out)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "null pointer");
   if (a.window < 0 || (a.window > 0 && !a.depth)) return serving_fail(GPTOSS_ERR_BAD_ARG, "a window needs the depths of the drafted tokens");
+  if (!(a.scale >= 0.f) || std::isinf(a.scale)) return serving_fail(GPTOSS_ERR_BAD_ARG, "scale must be finite and not negative");
   if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out) || a.q_stride % 8 || a.out_stride % 8)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "q, caches and out must be 16-byte aligned, token strides multiples of 8 elements");
   if (a.q_stride < (int64_t)a.n_q_heads * a.head_dim || a.out_stride < (int64_t)a.n_q_heads * a.head_dim)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "token stride below n_q_heads * head_dim");
-  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff) return serving_fail(GPTOSS_ERR_BAD_ARG, "too many drafted tokens");
-  const dim3 grid(a.n_seqs * a.max_nodes, (a.n_q_heads + 3) / 4);
-  const cudaError_t e = a.head_dim == 64
-                            ? launch_chain(tree_attention_kernel<64>, grid, dim3(128), 0, static_cast<cudaStream_t>(stream), a)
-                            : launch_chain(tree_attention_kernel<32>, grid, dim3(128), 0, static_cast<cudaStream_t>(stream), a);
+  const AttPlan plan = plan_of(a);
+  const uint64_t need = workspace_of(a, plan.n_splits);
+  if (need && (!a.workspace || !aligned16(a.workspace) || a.workspace_bytes < need))
+    return serving_fail(GPTOSS_ERR_BAD_ARG, "workspace missing, misaligned or below gptoss_tree_attention_workspace()");
+  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff || (int64_t)a.n_seqs * a.n_kv_heads * plan.q_tiles * plan.n_splits > 0x7fffffff ||
+      (int64_t)a.cache_rows * a.n_kv_heads > 0x7fffffff)
+    return serving_fail(GPTOSS_ERR_BAD_ARG, "too many drafted tokens or cache rows");
+  AttParams p;
+  p.a = a;
+  p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.q_tiles = plan.q_tiles;
+  p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
+  p.c = a.scale * 1.44269504f;
+  const uint64_t slabs = (uint64_t)a.cache_rows * a.n_kv_heads;
+  cudaError_t e = encode_weight_map(&p.map_k, a.k_cache, a.head_dim, a.max_seq, slabs);
+  if (e == cudaSuccess) e = encode_weight_map(&p.map_v, a.v_cache, a.head_dim, a.max_seq, slabs);
+  if (e == cudaSuccess) e = a.head_dim == 64 ? launch_tree<64>(p, static_cast<cudaStream_t>(stream)) : launch_tree<32>(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? GPTOSS_OK : serving_fail(GPTOSS_ERR_CUDA, "tree attention launch", e);
 }
 

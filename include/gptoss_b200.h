@@ -285,6 +285,9 @@ const char *gptoss_noalloc_last_error(void);
  * A workspace belongs to one call at a time: two calls (or captured graphs) that may overlap need two. */
 /* Message of the last failing call of these operators on this host thread ("" if none). */
 const char *gptoss_serving_last_error(void);
+/* Synchronises the current device: GPTOSS_OK, or GPTOSS_ERR_TIMEOUT if a kernel of these operators gave up on a bounded
+ * wait since the last call (its result is then meaningless). */
+int gptoss_serving_status(void);
 
 /* Attention of drafted tokens over the KV cache.  Sequence b has the ctx_len[b] cached tokens of cache row rows[b], and
  * a tree of n_b = offsets[b+1] - offsets[b] drafted tokens (rows offsets[b].. of q and out), whose K and V already stand
@@ -315,7 +318,7 @@ typedef struct {
   int n_tokens, n_seqs, max_nodes, max_ctx, mask_words;
   int cache_rows, max_seq, n_q_heads, n_kv_heads, head_dim;
   int window;           /* 0: none */
-  float scale;          /* of the scores, 1/sqrt(head_dim) as a rule */
+  float scale;          /* of the scores, 1/sqrt(head_dim) as a rule; finite, not negative */
 } gptoss_tree_attention_args;
 uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *args);
 int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream);
