@@ -448,12 +448,16 @@ cudaError_t launch_grouped_amax(const GemmArgs &a, int sm_count, cudaStream_t s)
 }
 
 cudaError_t encode_weight_map(CUtensorMap *m, const void *base, uint64_t K, uint64_t rows, uint64_t slabs) {
+  return encode_map_3d(m, base, K, rows, slabs, (uint32_t)kTileF);
+}
+
+cudaError_t encode_map_3d(CUtensorMap *m, const void *base, uint64_t K, uint64_t rows, uint64_t slabs, uint32_t box_rows) {
   EncodeTiledFn fn;
   cudaError_t e = get_encode_fn(&fn);
   if (e != cudaSuccess) return e;
   const cuuint64_t dims[3] = {K, rows, slabs};
   const cuuint64_t strides[2] = {K * 2, K * rows * 2};
-  const cuuint32_t box[3] = {(cuuint32_t)kBlockK, (cuuint32_t)kTileF, 1};
+  const cuuint32_t box[3] = {(cuuint32_t)kBlockK, (cuuint32_t)box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,

@@ -145,6 +145,8 @@ cudaError_t launch_grouped_amax(const GemmArgs &a, int sm_count, cudaStream_t s)
 // weights: base of [slabs][rows][K] bf16;  activations: base of [rows][K] bf16.
 cudaError_t encode_weight_map(CUtensorMap *m, const void *base, uint64_t K, uint64_t rows, uint64_t slabs);
 cudaError_t encode_act_map(CUtensorMap *m, const void *base, uint64_t K, uint64_t rows);
+// [slabs][rows][K] bf16 with the 128-byte swizzle and boxes of box_rows rows (<= 256)
+cudaError_t encode_map_3d(CUtensorMap *m, const void *base, uint64_t K, uint64_t rows, uint64_t slabs, uint32_t box_rows);
 
 // model_kernels.cu — the kernels around the MoE block that a decode step needs
 cudaError_t launch_embed(const int *tokens, const __nv_bfloat16 *table, int B, int H, int vocab, float *x, cudaStream_t s);

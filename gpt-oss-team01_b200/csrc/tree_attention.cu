@@ -32,24 +32,25 @@ thread_local char g_serving_error[256] = "";
 // thread builds a 128-bit mask of its row.  What a row must not see still goes through P V as 0 * V, so in those tiles
 // the non-finite elements of V are replaced by zeros in shared memory; the epilogue adds them back to the rows that do
 // see them.
-constexpr int kAttRows = 128, kAttTile = 128;     // query rows per CTA, slots per tile
+constexpr int kAttRows = 128, kAttTile = 64;      // query rows per CTA, slots per tile
+constexpr int kAttQBytes = kAttRows * 128;
 constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 bytes (head_dim 32: the upper half is zero-filled)
-constexpr int kAttKStages = 3, kAttVStages = 2;
-constexpr int kAttThreads = 192;                  // 4 softmax warps, the copy warp, the MMA warp
+constexpr int kAttStages = 2;
+constexpr int kAttThreads = 160;                  // 4 softmax warps, one warp for the copies and the products
+constexpr int kAttCtasPerSm = 4;
 constexpr int kMaxPoison = 768;                   // slots of masked tiles that can hold a non-finite V element
-constexpr uint32_t kTmemS = 0, kTmemP = 128, kTmemO = 192, kAttTmemCols = 256;
+constexpr uint32_t kTmemS = 0, kTmemP = 0, kTmemO = 64, kAttTmemCols = 128;
 
 struct AttCtrl {
-  uint64_t k_full[kAttKStages], k_empty[kAttKStages], v_full[kAttVStages], v_empty[kAttVStages];
-  uint64_t s_full, s_empty, p_full, pv_done, mma_done;
+  uint64_t k_full[kAttStages], v_full[kAttStages], s_full, p_full, done;
   uint32_t tmem_base;
   int abort, depth_lo, depth_hi, n_poison;
   int poison[kMaxPoison];
 };
-constexpr size_t kAttSmem = kAttTileBytes * (1 + kAttKStages + kAttVStages) + 1024 + sizeof(AttCtrl);
+constexpr size_t kAttSmem = kAttQBytes + kAttTileBytes * 2 * kAttStages + 1024 + sizeof(AttCtrl);
 
 struct AttParams {
-  CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 128, 1}
+  CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 64, 1}
   gptoss_tree_attention_args a;
   int group, nodes_per_tile, q_tiles, n_splits, tiles_per_split;
   float c;                   // scale * log2(e)
@@ -128,6 +129,23 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// two fp32 operations per instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
 __device__ __forceinline__ bool bf16_nonfinite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
@@ -135,14 +153,26 @@ __device__ __forceinline__ uint32_t bf16_finite_part(uint32_t pair) {
   return pair & ((pair & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((pair & 0x7f800000u) == 0x7f800000u ? 0x0000ffffu : ~0u);
 }
 
+constexpr uint32_t kPollLimit = 1u << 22;
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // mbar_wait in line: around a call the compiler would spill the row of scores that a softmax thread holds.
 __device__ __forceinline__ void wait_here(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
   const uint32_t addr = smem_u32(bar);
   volatile int *ab = abort_flag;
   uint32_t i = 0;
-  while (!mbar_try_wait(addr, parity)) {
+  while (!mbar_test_wait(addr, parity)) {
     if (*ab) return;
-    if (++i == kSpinLimit) {
+    if (++i == kPollLimit) {
       *ab = 1;
       if (atomicCAS(g_serving_status, 0, kDevErrTimeout) == 0) g_serving_status[1] = site, g_serving_status[2] = (int)blockIdx.x;
       return;
@@ -150,13 +180,18 @@ __device__ __forceinline__ void wait_here(uint64_t *bar, uint32_t parity, int *a
   }
 }
 
+__device__ __forceinline__ void wait_warp(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
+  wait_here(bar, parity, abort_flag, site);
+  __syncwarp();
+}
+
 template <int HD>
-__global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __grid_constant__ AttParams p) {
+__global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_kernel(const __grid_constant__ AttParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t q_s = (raw + 1023u) & ~1023u, k_s = q_s + kAttTileBytes, v_s = k_s + kAttKStages * kAttTileBytes;
+  const uint32_t q_s = (raw + 1023u) & ~1023u, k_s = q_s + kAttQBytes, v_s = k_s + kAttStages * kAttTileBytes;
   uint8_t *const smem = smem_raw + (q_s - raw);
-  AttCtrl *ctrl = reinterpret_cast<AttCtrl *>(smem + kAttTileBytes * (1 + kAttKStages + kAttVStages));
+  AttCtrl *ctrl = reinterpret_cast<AttCtrl *>(smem + kAttQBytes + 2 * kAttStages * kAttTileBytes);
   const gptoss_tree_attention_args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int x = blockIdx.x;
@@ -179,17 +214,14 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
   const int slab = row * a.n_kv_heads + kvh;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kAttKStages; ++i) mbar_init(smem_u32(&ctrl->k_full[i]), 1), mbar_init(smem_u32(&ctrl->k_empty[i]), 1);
-    for (int i = 0; i < kAttVStages; ++i) mbar_init(smem_u32(&ctrl->v_full[i]), 1), mbar_init(smem_u32(&ctrl->v_empty[i]), 1);
+    for (int i = 0; i < kAttStages; ++i) mbar_init(smem_u32(&ctrl->k_full[i]), 1), mbar_init(smem_u32(&ctrl->v_full[i]), 1);
     mbar_init(smem_u32(&ctrl->s_full), 1);
-    mbar_init(smem_u32(&ctrl->s_empty), 4);
     mbar_init(smem_u32(&ctrl->p_full), 4);
-    mbar_init(smem_u32(&ctrl->pv_done), 1);
-    mbar_init(smem_u32(&ctrl->mma_done), 1);
+    mbar_init(smem_u32(&ctrl->done), 1);
     ctrl->abort = 0, ctrl->n_poison = 0, ctrl->depth_lo = 0x3fffffff, ctrl->depth_hi = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == 4) {
     tmem_alloc(smem_u32(&ctrl->tmem_base), kAttTmemCols);
     tmem_relinquish();
   }
@@ -221,64 +253,60 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
   const int slot_first = lo_min + t_begin * kAttTile;
 
   if (warp == 4) {
-    // ===================== copies =====================
-    if (lane == 0) {
-      int i = 0;
-      for (; i < n_tiles; ++i) {
-        const int ks = i % kAttKStages, vs = i % kAttVStages;
-        bool ok = mbar_wait(smem_u32(&ctrl->k_empty[ks]), ((i / kAttKStages) & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2000 | ks);
-        if (!ok) break;
-        mbar_expect_tx(smem_u32(&ctrl->k_full[ks]), kAttTileBytes);
-        tma_load_3d(k_s + ks * kAttTileBytes, &p.map_k, smem_u32(&ctrl->k_full[ks]), 0, slot_first + i * kAttTile, slab);
-        ok = mbar_wait(smem_u32(&ctrl->v_empty[vs]), ((i / kAttVStages) & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2100 | vs);
-        mbar_expect_tx(smem_u32(&ctrl->v_full[vs]), kAttTileBytes);
-        tma_load_3d(v_s + vs * kAttTileBytes, &p.map_v, smem_u32(&ctrl->v_full[vs]), 0, slot_first + i * kAttTile, slab);
-        if (!ok) {
-          ++i;
-          break;
-        }
-      }
-      if (i < n_tiles || *reinterpret_cast<volatile int *>(&ctrl->abort)) {
-        // gave up: the copies in flight have to land before the CTA's shared memory is given away
-        for (int j = max(0, i - kAttKStages); j < i; ++j)
-          for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->k_full[j % kAttKStages]), (j / kAttKStages) & 1); ++w) {}
-        for (int j = max(0, i - kAttVStages); j < i; ++j)
-          for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->v_full[j % kAttVStages]), (j / kAttVStages) & 1); ++w) {}
-      }
-    }
-  } else if (warp == 5) {
-    // ===================== products =====================
-    if (lane == 0) {
+    // ===================== copies and products =====================
+    // Products run in the order of their issue, and the completion that a commit signals covers all before it.  So P of
+    // tile i being there (p_full) says that the softmax threads saw S of tile i, hence that Q K^T of tile i and P V of
+    // tile i - 1 are complete: their K and V tiles can be overwritten.
+    if (lane == 0 && n_tiles > 0) {
       const uint32_t idesc_s = umma_idesc(kAttTile), idesc_o = umma_idesc(HD) | kIdescTransposeB;
       const uint64_t dq = smem_desc_sw128(q_s);
+      auto copy = [&](const CUtensorMap *map, uint32_t dst, uint64_t *bar, int i) {
+        const uint32_t full = smem_u32(bar + i % kAttStages);
+        mbar_expect_tx(full, kAttTileBytes);
+        tma_load_3d(dst + (i % kAttStages) * kAttTileBytes, map, full, 0, slot_first + i * kAttTile, slab);
+      };
       auto scores = [&](int i) {
-        const int ks = i % kAttKStages;
-        mbar_wait(smem_u32(&ctrl->k_full[ks]), (i / kAttKStages) & 1, &ctrl->abort, g_serving_status, 0x2200 | ks);
-        mbar_wait(smem_u32(&ctrl->s_empty), (i & 1) ^ 1, &ctrl->abort, g_serving_status, 0x2300);
-        tc_fence_after();
-        const uint64_t dk = smem_desc_sw128(k_s + ks * kAttTileBytes);
+        const uint64_t dk = smem_desc_sw128(k_s + (i % kAttStages) * kAttTileBytes);
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) umma_bf16(tmem + kTmemS, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, k > 0);
         umma_commit(smem_u32(&ctrl->s_full));
-        umma_commit(smem_u32(&ctrl->k_empty[ks]));
       };
-      if (n_tiles > 0) scores(0);
+      auto landed = [&](uint64_t *bar, int i, int site) {
+        wait_here(bar + i % kAttStages, (i / kAttStages) & 1, &ctrl->abort, site);
+      };
+      int k_sent = 0, v_sent = 0;
+      for (; k_sent < min(kAttStages, n_tiles); ++k_sent) {
+        copy(&p.map_k, k_s, ctrl->k_full, k_sent);
+        copy(&p.map_v, v_s, ctrl->v_full, v_sent++);
+      }
+      landed(ctrl->k_full, 0, 0x2200);
+      tc_fence_after();
+      scores(0);
       for (int i = 0; i < n_tiles; ++i) {
-        if (i + 1 < n_tiles) scores(i + 1);
-        const int vs = i % kAttVStages;
-        mbar_wait(smem_u32(&ctrl->v_full[vs]), (i / kAttVStages) & 1, &ctrl->abort, g_serving_status, 0x2400 | vs);
-        mbar_wait(smem_u32(&ctrl->p_full), i & 1, &ctrl->abort, g_serving_status, 0x2500);
+        // from P to the next S nothing but the products stands in the way: their tiles are waited for before, the next
+        // copies are issued after
+        const bool more = i + 1 < n_tiles;
+        landed(ctrl->v_full, i, 0x2400);
+        if (more) landed(ctrl->k_full, i + 1, 0x2300);
+        const uint64_t dv = smem_desc_v(v_s + (i % kAttStages) * kAttTileBytes);
+        wait_here(&ctrl->p_full, i & 1, &ctrl->abort, 0x2500);
         tc_fence_after();
-        const uint64_t dv = smem_desc_v(v_s + vs * kAttTileBytes);
 #pragma unroll
         for (int k = 0; k < kAttTile / 16; ++k)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V
           umma_bf16_ts(tmem + kTmemO, tmem + kTmemP + 8 * k, dv + (uint64_t)(128 * k), idesc_o, (i | k) != 0);
-        umma_commit(smem_u32(&ctrl->pv_done));
-        umma_commit(smem_u32(&ctrl->v_empty[vs]));
+        if (more) scores(i + 1);
+        if (*reinterpret_cast<volatile int *>(&ctrl->abort)) break;
+        if (k_sent < n_tiles) copy(&p.map_k, k_s, ctrl->k_full, k_sent++);                     // tile i + kAttStages
+        if (i > 0 && v_sent < n_tiles) copy(&p.map_v, v_s, ctrl->v_full, v_sent++);  // tile i - 1 + kAttStages
       }
-      if (*reinterpret_cast<volatile int *>(&ctrl->abort)) {  // what was issued has to retire before TMEM is given up
-        umma_commit(smem_u32(&ctrl->mma_done));
-        for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->mma_done), 0); ++w) {}
+      umma_commit(smem_u32(&ctrl->done));
+      if (*reinterpret_cast<volatile int *>(&ctrl->abort)) {
+        // gave up: what was issued has to retire before shared memory and TMEM are given away
+        for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->done), 0); ++w) {}
+        for (int j = max(0, k_sent - kAttStages); j < k_sent; ++j)
+          for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->k_full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
+        for (int j = max(0, v_sent - kAttStages); j < v_sent; ++j)
+          for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->v_full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
       }
     }
   } else {
@@ -291,44 +319,39 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
     for (int i = 0; i < n_tiles; ++i) {
       const int t0 = slot_first + i * kAttTile;
       const bool masked = t0 < lo_max || t0 + kAttTile > ctx;
-      uint32_t bits[4];
+      uint32_t bits[2];
       if (masked) {
 #pragma unroll
-        for (int w = 0; w < 4; ++w) bits[w] = valid ? view.word(t0 + 32 * w) : 0u;
-        // slot r of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
-        const int vs = i % kAttVStages;
-        wait_here(&ctrl->v_full[vs], (i / kAttVStages) & 1, &ctrl->abort, 0x2700);
-        uint4 *vr = reinterpret_cast<uint4 *>(smem + (1 + kAttKStages + vs) * kAttTileBytes + r * 128);
+        for (int w = 0; w < 2; ++w) bits[w] = valid ? view.word(t0 + 32 * w) : 0u;
+        // half of slot r / 2 of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
+        const int vs = i % kAttStages;
+        wait_warp(&ctrl->v_full[vs], (i / kAttStages) & 1, &ctrl->abort, 0x2700);
+        uint4 *vr = reinterpret_cast<uint4 *>(smem + kAttQBytes + (kAttStages + vs) * kAttTileBytes + r * 64);
         bool bad = false;
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          uint4 v = vr[(c + r) & 7];
+        for (int c = 0; c < 4; ++c) {
+          uint4 v = vr[c];
           if (bf16_nonfinite(v.x) || bf16_nonfinite(v.y) || bf16_nonfinite(v.z) || bf16_nonfinite(v.w)) {
             bad = true;
             v.x = bf16_finite_part(v.x), v.y = bf16_finite_part(v.y), v.z = bf16_finite_part(v.z), v.w = bf16_finite_part(v.w);
-            vr[(c + r) & 7] = v;
+            vr[c] = v;
           }
         }
-        if (bad && t0 + r < len) {
+        const bool other_half = __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;  // every lane takes part
+        bad |= other_half;
+        if (bad && !(r & 1) && t0 + (r >> 1) < len) {
           const int at = atomicAdd(&ctrl->n_poison, 1);
-          if (at < kMaxPoison) ctrl->poison[at] = t0 + r;
+          if (at < kMaxPoison) ctrl->poison[at] = t0 + (r >> 1);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
       float s[kAttTile];
-      wait_here(&ctrl->s_full, i & 1, &ctrl->abort, 0x2600);
+      wait_warp(&ctrl->s_full, i & 1, &ctrl->abort, 0x2600);
       tc_fence_after();
       if (live) {
 #pragma unroll
         for (int j = 0; j < kAttTile; j += 32) tmem_ld32(tmem + lane_addr + kTmemS + j, s + j);
         tmem_ld_wait();
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctrl->s_empty));
-      bool move = false;
-      float corr = 1.f;
-      if (live) {
         if (masked) {
 #pragma unroll
           for (int j = 0; j < kAttTile; ++j) s[j] = (bits[j >> 5] >> (j & 31) & 1u) ? s[j] : -INFINITY;
@@ -337,18 +360,13 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
 #pragma unroll
         for (int j = 0; j < kAttTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c;
-        move = top > m + 8.f;
+        const bool move = top > m + 8.f;
+        float corr = 1.f;
         if (move) {
           corr = ex2(m - top);
           m = top;
         }
-      }
-      // the product before this one has read P and written O (warps without rows wait too: nobody may arrive for this
-      // tile's P before the last one's has been taken)
-      if (i > 0) wait_here(&ctrl->pv_done, (i - 1) & 1, &ctrl->abort, 0x2800);
-      tc_fence_after();
-      if (live) {
-        if (i > 0 && __any_sync(0xffffffffu, move)) {
+        if (i > 0 && __any_sync(0xffffffffu, move)) {  // P V of the tile before is complete, as S of this tile is
 #pragma unroll
           for (int h = 0; h < HD; h += 16) {
             uint32_t o[16];
@@ -360,19 +378,21 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+        const float2 c2 = make_float2(p.c, p.c), base2 = make_float2(-base, -base);
 #pragma unroll
         for (int h = 0; h < kAttTile; h += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
-            const float e0 = ex2(fmaf(s[h + j], p.c, -base)), e1 = ex2(fmaf(s[h + j + 1], p.c, -base));
-            sum[(j >> 1) & 3] += e0 + e1;
-            pk[j >> 1] = pack_bf16(e0, e1);
+            const float2 x = fma2(make_float2(s[h + j], s[h + j + 1]), c2, base2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+            pk[j >> 1] = pack_bf16(e.x, e.y);
           }
           tmem_st16(tmem + lane_addr + kTmemP + (h >> 1), pk);
         }
-        l = l * corr + ((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        l = l * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
         tmem_st_wait();
       }
       tc_fence_before();
@@ -380,7 +400,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
       if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full));
     }
     // ---- result of this share of the context ----
-    if (n_tiles > 0) wait_here(&ctrl->pv_done, (n_tiles - 1) & 1, &ctrl->abort, 0x2900);
+    if (n_tiles > 0) wait_warp(&ctrl->done, 0, &ctrl->abort, 0x2900);
     asm volatile("bar.sync 1, 128;" ::: "memory");  // every note of a non-finite element is in place
     tc_fence_after();
     if (live) {
@@ -426,7 +446,7 @@ __global__ void __launch_bounds__(kAttThreads, 2) tree_attention_kernel(const __
   pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == 4) {
     tc_fence_after();
     tmem_dealloc(tmem, kAttTmemCols);
   }
@@ -536,7 +556,7 @@ AttPlan plan_of(const gptoss_tree_attention_args &a) {
   // the cached tokens that a tree can reach: with a window, as many as its first token sees
   const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
-  long long splits = items > 0 ? (2ll * sms + items - 1) / items : 1;
+  long long splits = items > 0 ? ((long long)kAttCtasPerSm * sms + items - 1) / items : 1;
   if (splits > tiles) splits = tiles;
   if (splits < 1) splits = 1;
   p.tiles_per_split = (int)((tiles + splits - 1) / splits);
@@ -618,8 +638,8 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
   p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
   p.c = a.scale * 1.44269504f;
   const uint64_t slabs = (uint64_t)a.cache_rows * a.n_kv_heads;
-  cudaError_t e = encode_weight_map(&p.map_k, a.k_cache, a.head_dim, a.max_seq, slabs);
-  if (e == cudaSuccess) e = encode_weight_map(&p.map_v, a.v_cache, a.head_dim, a.max_seq, slabs);
+  cudaError_t e = encode_map_3d(&p.map_k, a.k_cache, a.head_dim, a.max_seq, slabs, kAttTile);
+  if (e == cudaSuccess) e = encode_map_3d(&p.map_v, a.v_cache, a.head_dim, a.max_seq, slabs, kAttTile);
   if (e == cudaSuccess) e = a.head_dim == 64 ? launch_tree<64>(p, static_cast<cudaStream_t>(stream)) : launch_tree<32>(p, static_cast<cudaStream_t>(stream));
   return e == cudaSuccess ? GPTOSS_OK : serving_fail(GPTOSS_ERR_CUDA, "tree attention launch", e);
 }
