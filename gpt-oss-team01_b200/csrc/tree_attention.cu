@@ -35,14 +35,16 @@ thread_local char g_serving_error[256] = "";
 constexpr int kAttRows = 128, kAttTile = 64;      // query rows per CTA, slots per tile
 constexpr int kAttQBytes = kAttRows * 128;
 constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 bytes (head_dim 32: the upper half is zero-filled)
-constexpr int kAttStages = 2;
-constexpr int kAttThreads = 160;                  // 4 softmax warps, one warp for the copies and the products
-constexpr int kAttCtasPerSm = 4;
+constexpr int kAttStages = 4;
+constexpr int kAttHalf = kAttTile / 2;            // slots of a tile that one softmax thread works on
+constexpr int kAttSoftmax = 2 * kAttRows;         // 8 softmax warps
+constexpr int kAttThreads = kAttSoftmax + 32;     // and one warp for the copies and the products
+constexpr int kAttCtasPerSm = 2;
 constexpr int kMaxPoison = 768;                   // slots of masked tiles that can hold a non-finite V element
-constexpr uint32_t kTmemS = 0, kTmemP = 0, kTmemO = 64, kAttTmemCols = 128;
+constexpr uint32_t kTmemS = 0, kTmemO = 128, kAttTmemCols = 256;  // two tiles of S; O of each half
 
 struct AttCtrl {
-  uint64_t k_full[kAttStages], v_full[kAttStages], s_full, p_full, done;
+  uint64_t k_full[kAttStages], v_full[kAttStages], s_full[2], p_full[2], pv_done, retired;
   uint32_t tmem_base;
   int abort, depth_lo, depth_hi, n_poison;
   int poison[kMaxPoison];
@@ -146,6 +148,27 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
       : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+// largest of three, NaN if any is
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x for finite x below 127 (below -126: 2^-126): x = n + f with n the nearest integer, taken from the low bits of
+// x + 1.5 * 2^23, and 2^f by the polynomial of degree 4 with the smallest largest relative error on [-1/2, 1/2]
+// (Remez exchange: 2^-18.5), its exponent then raised by n.
+__device__ __forceinline__ float2 ex2_poly(float2 x) {
+  constexpr float kShift = 12582912.f;
+  x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
+  const float2 t = add2(x, make_float2(kShift, kShift));
+  const float2 f = fma2(add2(t, make_float2(-kShift, -kShift)), make_float2(-1.f, -1.f), x);
+  float2 y = fma2(f, make_float2(0.009570102f, 0.009570102f), make_float2(0.05591786f, 0.05591786f));
+  y = fma2(f, y, make_float2(0.24024744f, 0.24024744f));
+  y = fma2(f, y, make_float2(0.6931218f, 0.6931218f));
+  y = fma2(f, y, make_float2(0.9999993f, 0.9999993f));
+  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
 __device__ __forceinline__ bool bf16_nonfinite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
 }
@@ -215,22 +238,22 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAttStages; ++i) mbar_init(smem_u32(&ctrl->k_full[i]), 1), mbar_init(smem_u32(&ctrl->v_full[i]), 1);
-    mbar_init(smem_u32(&ctrl->s_full), 1);
-    mbar_init(smem_u32(&ctrl->p_full), 4);
-    mbar_init(smem_u32(&ctrl->done), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctrl->s_full[i]), 1), mbar_init(smem_u32(&ctrl->p_full[i]), 8);
+    mbar_init(smem_u32(&ctrl->pv_done), 1);
+    mbar_init(smem_u32(&ctrl->retired), 1);
     ctrl->abort = 0, ctrl->n_poison = 0, ctrl->depth_lo = 0x3fffffff, ctrl->depth_hi = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) {
+  if (warp == 8) {
     tmem_alloc(smem_u32(&ctrl->tmem_base), kAttTmemCols);
     tmem_relinquish();
   }
   // query rows into shared memory, in the layout a 128-byte-swizzled copy would give them (rows beyond the tree hold
   // whatever lies there: a row of the products depends on its own row of Q only)
-  const int r = threadIdx.x, node = r / p.group, head = kvh * p.group + r % p.group;
-  const bool valid = r < kAttRows && node < nodes;
+  const int r = threadIdx.x % kAttRows, half = threadIdx.x / kAttRows, node = r / p.group, head = kvh * p.group + r % p.group;
+  const bool valid = half < 2 && node < nodes;
   const int tok = first + n0 + (valid ? node : 0);
-  if (valid) {
+  if (valid && half == 0) {
     const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
 #pragma unroll
     for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + r * 128 + ((c ^ (r & 7)) << 4)) = src[c];
@@ -252,11 +275,13 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const int n_tiles = (split == p.n_splits - 1 ? tiles : min(tiles, t_begin + p.tiles_per_split)) - t_begin;
   const int slot_first = lo_min + t_begin * kAttTile;
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ===================== copies and products =====================
-    // Products run in the order of their issue, and the completion that a commit signals covers all before it.  So P of
-    // tile i being there (p_full) says that the softmax threads saw S of tile i, hence that Q K^T of tile i and P V of
-    // tile i - 1 are complete: their K and V tiles can be overwritten.
+    // Products run in the order of their issue, and the completion that a commit signals covers all before it.  Two tiles
+    // of S are under way: while the softmax threads work on one, Q K^T of the next is done.  P of tile i being there
+    // (p_full) says that the softmax threads saw S of tile i, hence that Q K^T of tile i and P V of tile i - 2 are
+    // complete: their K and V tiles can be overwritten.  P of tile i is read by P V before Q K^T of tile i + 2, issued
+    // behind it, overwrites it.
     if (lane == 0 && n_tiles > 0) {
       const uint32_t idesc_s = umma_idesc(kAttTile), idesc_o = umma_idesc(HD) | kIdescTransposeB;
       const uint64_t dq = smem_desc_sw128(q_s);
@@ -267,9 +292,10 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
       };
       auto scores = [&](int i) {
         const uint64_t dk = smem_desc_sw128(k_s + (i % kAttStages) * kAttTileBytes);
+        const uint32_t d = tmem + kTmemS + (i & 1) * kAttTile;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) umma_bf16(tmem + kTmemS, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, k > 0);
-        umma_commit(smem_u32(&ctrl->s_full));
+        for (int k = 0; k < HD / 16; ++k) umma_bf16(d, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, k > 0);
+        umma_commit(smem_u32(&ctrl->s_full[i & 1]));
       };
       auto landed = [&](uint64_t *bar, int i, int site) {
         wait_here(bar + i % kAttStages, (i / kAttStages) & 1, &ctrl->abort, site);
@@ -279,30 +305,33 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         copy(&p.map_k, k_s, ctrl->k_full, k_sent);
         copy(&p.map_v, v_s, ctrl->v_full, v_sent++);
       }
-      landed(ctrl->k_full, 0, 0x2200);
-      tc_fence_after();
-      scores(0);
+      for (int i = 0; i < min(2, n_tiles); ++i) {
+        landed(ctrl->k_full, i, 0x2200);
+        tc_fence_after();
+        scores(i);
+      }
       for (int i = 0; i < n_tiles; ++i) {
-        // from P to the next S nothing but the products stands in the way: their tiles are waited for before, the next
-        // copies are issued after
-        const bool more = i + 1 < n_tiles;
+        const bool more = i + 2 < n_tiles;
         landed(ctrl->v_full, i, 0x2400);
-        if (more) landed(ctrl->k_full, i + 1, 0x2300);
+        if (more) landed(ctrl->k_full, i + 2, 0x2300);
         const uint64_t dv = smem_desc_v(v_s + (i % kAttStages) * kAttTileBytes);
-        wait_here(&ctrl->p_full, i & 1, &ctrl->abort, 0x2500);
+        const uint32_t tp = tmem + kTmemS + (i & 1) * kAttTile;
+        wait_here(&ctrl->p_full[i & 1], (i >> 1) & 1, &ctrl->abort, 0x2500);
         tc_fence_after();
 #pragma unroll
-        for (int k = 0; k < kAttTile / 16; ++k)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V
-          umma_bf16_ts(tmem + kTmemO, tmem + kTmemP + 8 * k, dv + (uint64_t)(128 * k), idesc_o, (i | k) != 0);
-        if (more) scores(i + 1);
+        for (int k = 0; k < kAttTile / 16; ++k)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V; 2 such steps per half
+          umma_bf16_ts(tmem + kTmemO + (k >> 1) * 64, tp + (k >> 1) * kAttHalf + (k & 1) * 8, dv + (uint64_t)(128 * k), idesc_o,
+                       i > 0 || (k & 1) != 0);
+        umma_commit(smem_u32(&ctrl->pv_done));
+        if (more) scores(i + 2);
         if (*reinterpret_cast<volatile int *>(&ctrl->abort)) break;
         if (k_sent < n_tiles) copy(&p.map_k, k_s, ctrl->k_full, k_sent++);                     // tile i + kAttStages
-        if (i > 0 && v_sent < n_tiles) copy(&p.map_v, v_s, ctrl->v_full, v_sent++);  // tile i - 1 + kAttStages
+        if (i > 1 && v_sent < n_tiles) copy(&p.map_v, v_s, ctrl->v_full, v_sent++);  // tile i - 2 + kAttStages
       }
-      umma_commit(smem_u32(&ctrl->done));
+      umma_commit(smem_u32(&ctrl->retired));
       if (*reinterpret_cast<volatile int *>(&ctrl->abort)) {
         // gave up: what was issued has to retire before shared memory and TMEM are given away
-        for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->done), 0); ++w) {}
+        for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->retired), 0); ++w) {}
         for (int j = max(0, k_sent - kAttStages); j < k_sent; ++j)
           for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->k_full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
         for (int j = max(0, v_sent - kAttStages); j < v_sent; ++j)
@@ -313,140 +342,154 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     // ===================== softmax, a thread per query row =====================
     RowView view{ctx, len - ctx, a.window > 0 ? min(max(ctx + depth - a.window + 1, 0), ctx) : 0, a.window, depth, a.mask_words,
                  a.mask + (size_t)tok * a.mask_words, a.depth + first};
-    const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, to = tmem + lane_addr + kTmemO + half * 64;
     const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
     float m = -INFINITY, l = 0.f;
     for (int i = 0; i < n_tiles; ++i) {
       const int t0 = slot_first + i * kAttTile;
       const bool masked = t0 < lo_max || t0 + kAttTile > ctx;
-      uint32_t bits[2];
+      uint32_t bits = 0;
       if (masked) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) bits[w] = valid ? view.word(t0 + 32 * w) : 0u;
-        // half of slot r / 2 of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
+        if (valid) bits = view.word(t0 + kAttHalf * half);
+        // a quarter of slot threadIdx.x / 4 of this tile: non-finite elements of V become zeros, and the slot is noted if
+        // anyone can see it
         const int vs = i % kAttStages;
         wait_warp(&ctrl->v_full[vs], (i / kAttStages) & 1, &ctrl->abort, 0x2700);
-        uint4 *vr = reinterpret_cast<uint4 *>(smem + kAttQBytes + (kAttStages + vs) * kAttTileBytes + r * 64);
-        bool bad = false;
+        uint4 *vr = reinterpret_cast<uint4 *>(smem + kAttQBytes + (kAttStages + vs) * kAttTileBytes + threadIdx.x * 32);
+        int bad = 0;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint4 v = vr[c];
           if (bf16_nonfinite(v.x) || bf16_nonfinite(v.y) || bf16_nonfinite(v.z) || bf16_nonfinite(v.w)) {
-            bad = true;
+            bad = 1;
             v.x = bf16_finite_part(v.x), v.y = bf16_finite_part(v.y), v.z = bf16_finite_part(v.z), v.w = bf16_finite_part(v.w);
             vr[c] = v;
           }
         }
-        const bool other_half = __shfl_xor_sync(0xffffffffu, (int)bad, 1) != 0;  // every lane takes part
-        bad |= other_half;
-        if (bad && !(r & 1) && t0 + (r >> 1) < len) {
+        __syncwarp();
+        bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
+        bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
+        const int slot = t0 + (threadIdx.x >> 2);
+        if (bad && (lane & 3) == 0 && slot < len) {
           const int at = atomicAdd(&ctrl->n_poison, 1);
-          if (at < kMaxPoison) ctrl->poison[at] = t0 + (r >> 1);
+          if (at < kMaxPoison) ctrl->poison[at] = slot;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      float s[kAttTile];
-      wait_warp(&ctrl->s_full, i & 1, &ctrl->abort, 0x2600);
+      float s[kAttHalf];
+      const uint32_t ts = tmem + lane_addr + kTmemS + (i & 1) * kAttTile + half * kAttHalf;
+      wait_warp(&ctrl->s_full[i & 1], (i >> 1) & 1, &ctrl->abort, 0x2600);
       tc_fence_after();
       if (live) {
-#pragma unroll
-        for (int j = 0; j < kAttTile; j += 32) tmem_ld32(tmem + lane_addr + kTmemS + j, s + j);
+        tmem_ld32(ts, s);
         tmem_ld_wait();
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < kAttTile; ++j) s[j] = (bits[j >> 5] >> (j & 31) & 1u) ? s[j] : -INFINITY;
+          for (int j = 0; j < kAttHalf; ++j) s[j] = (bits >> j & 1u) ? s[j] : -INFINITY;
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        float mx[2] = {max3_nan(s[0], s[1], s[2]), max3_nan(s[3], s[4], s[5])};
 #pragma unroll
-        for (int j = 0; j < kAttTile; ++j) mx[j & 3] = fmaxf(mx[j & 3], s[j]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c;
+        for (int j = 6; j + 1 < kAttHalf; j += 2) mx[(j >> 1) & 1] = max3_nan(mx[(j >> 1) & 1], s[j], s[j + 1]);
+        const float top = max3_nan(mx[0], mx[1], mx[1]) * p.c;
         const bool move = top > m + 8.f;
         float corr = 1.f;
         if (move) {
           corr = ex2(m - top);
           m = top;
         }
-        if (i > 0 && __any_sync(0xffffffffu, move)) {  // P V of the tile before is complete, as S of this tile is
+        if (i > 0 && __any_sync(0xffffffffu, move)) {
+          wait_warp(&ctrl->pv_done, (i - 1) & 1, &ctrl->abort, 0x2800);
+          tc_fence_after();
 #pragma unroll
           for (int h = 0; h < HD; h += 16) {
             uint32_t o[16];
-            tmem_ld16(tmem + lane_addr + kTmemO + h, o);
+            tmem_ld16(to + h, o);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-            tmem_st16(tmem + lane_addr + kTmemO + h, o);
+            tmem_st16(to + h, o);
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         const float2 c2 = make_float2(p.c, p.c), base2 = make_float2(-base, -base);
+        uint32_t pk[kAttHalf / 2];
 #pragma unroll
-        for (int h = 0; h < kAttTile; h += 32) {
-          uint32_t pk[16];
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float2 x = fma2(make_float2(s[h + j], s[h + j + 1]), c2, base2);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
-            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
-            pk[j >> 1] = pack_bf16(e.x, e.y);
-          }
-          tmem_st16(tmem + lane_addr + kTmemP + (h >> 1), pk);
+        for (int j = 0; j < kAttHalf; j += 2) {
+          const float2 x = fma2(make_float2(s[j], s[j + 1]), c2, base2);
+          const float2 e = make_float2(ex2(x.x), ex2(x.y));
+          sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+          pk[j >> 1] = pack_bf16(e.x, e.y);
         }
+        tmem_st16(ts, pk);
         l = l * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
         tmem_st_wait();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full));
+      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full[i & 1]));
     }
     // ---- result of this share of the context ----
-    if (n_tiles > 0) wait_warp(&ctrl->done, 0, &ctrl->abort, 0x2900);
-    asm volatile("bar.sync 1, 128;" ::: "memory");  // every note of a non-finite element is in place
+    if (n_tiles > 0) wait_warp(&ctrl->retired, 0, &ctrl->abort, 0x2900);
     tc_fence_after();
-    if (live) {
-      float o[HD];
+    float o[HD];
 #pragma unroll
-      for (int j = 0; j < HD; ++j) o[j] = 0.f;
-      if (n_tiles > 0) {
+    for (int j = 0; j < HD; ++j) o[j] = 0.f;
+    if (live && n_tiles > 0) {
 #pragma unroll
-        for (int h = 0; h < HD; h += 32) tmem_ld32(tmem + lane_addr + kTmemO + h, o + h);
-        tmem_ld_wait();
+      for (int h = 0; h < HD; h += 32) tmem_ld32(to + h, o + h);
+      tmem_ld_wait();
+    }
+    // the second half of each row goes to the first through shared memory; no copy or product is under way any more
+    float *join = reinterpret_cast<float *>(smem + kAttQBytes) + r;
+    static_assert((HD + 2) * kAttRows * 4 <= 2 * kAttStages * kAttTileBytes, "the halves meet in the ring's memory");
+    if (half == 1) {
+#pragma unroll
+      for (int j = 0; j < HD; ++j) join[j * kAttRows] = o[j];
+      join[HD * kAttRows] = m;
+      join[(HD + 1) * kAttRows] = l;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (half == 0 && valid) {
+      const float m1 = join[HD * kAttRows], top1 = fmaxf(m, m1), base1 = top1 == -INFINITY ? 0.f : top1;
+      const float w0 = ex2(m - base1), w1 = ex2(m1 - base1);
+      l = fmaf(l, w0, join[(HD + 1) * kAttRows] * w1);
+      m = top1;
+#pragma unroll
+      for (int j = 0; j < HD; ++j) o[j] = fmaf(o[j], w0, join[j * kAttRows] * w1);
+      const int bad = min(ctrl->n_poison, kMaxPoison);
+      for (int i = 0; i < bad; ++i) {
+        const int slot = ctrl->poison[i];
+        if (!(view.word(slot) & 1u)) continue;
+        const uint16_t *v = static_cast<const uint16_t *>(a.v_cache) + ((size_t)slab * a.max_seq + slot) * HD;
+#pragma unroll
+        for (int j = 0; j < HD; ++j)
+          if ((v[j] & 0x7f80u) == 0x7f80u) o[j] += __uint_as_float((uint32_t)v[j] << 16);
       }
-      if (valid) {
-        const int bad = min(ctrl->n_poison, kMaxPoison);
-        for (int i = 0; i < bad; ++i) {
-          const int slot = ctrl->poison[i];
-          if (!(view.word(slot) & 1u)) continue;
-          const uint16_t *v = static_cast<const uint16_t *>(a.v_cache) + ((size_t)slab * a.max_seq + slot) * HD;
+      if (p.n_splits == 1) {
+        const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
+        const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
+        const float w = ex2(m - base), total = fmaf(l, w, ex2(sink - base));
+        const float inv = total == 0.f ? 0.f : w / total;
+        uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (size_t)tok * a.out_stride + (size_t)head * HD);
 #pragma unroll
-          for (int j = 0; j < HD; ++j)
-            if ((v[j] & 0x7f80u) == 0x7f80u) o[j] += __uint_as_float((uint32_t)v[j] << 16);
-        }
-        if (p.n_splits == 1) {
-          const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
-          const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
-          const float w = ex2(m - base), total = fmaf(l, w, ex2(sink - base));
-          const float inv = total == 0.f ? 0.f : w / total;
-          uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (size_t)tok * a.out_stride + (size_t)head * HD);
+        for (int j = 0; j < HD; j += 8)
+          dst[j >> 3] = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
+                                   pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
+      } else {
+        const size_t at = ((size_t)split * a.n_tokens + tok) * a.n_q_heads + head;
+        float4 *dst = static_cast<float4 *>(a.workspace) + at * (HD / 4);
 #pragma unroll
-          for (int j = 0; j < HD; j += 8)
-            dst[j >> 3] = make_uint4(pack_bf16(o[j] * inv, o[j + 1] * inv), pack_bf16(o[j + 2] * inv, o[j + 3] * inv),
-                                     pack_bf16(o[j + 4] * inv, o[j + 5] * inv), pack_bf16(o[j + 6] * inv, o[j + 7] * inv));
-        } else {
-          const size_t at = ((size_t)split * a.n_tokens + tok) * a.n_q_heads + head;
-          float4 *dst = static_cast<float4 *>(a.workspace) + at * (HD / 4);
-#pragma unroll
-          for (int j = 0; j < HD; j += 4) dst[j >> 2] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-          float2 *ml = reinterpret_cast<float2 *>(static_cast<float *>(a.workspace) + (size_t)p.n_splits * a.n_tokens * a.n_q_heads * HD);
-          ml[at] = make_float2(m, l);
-        }
+        for (int j = 0; j < HD; j += 4) dst[j >> 2] = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        float2 *ml = reinterpret_cast<float2 *>(static_cast<float *>(a.workspace) + (size_t)p.n_splits * a.n_tokens * a.n_q_heads * HD);
+        ml[at] = make_float2(m, l);
       }
     }
   }
   pdl_launch_dependents();
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem, kAttTmemCols);
   }
