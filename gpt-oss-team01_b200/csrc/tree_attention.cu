@@ -32,29 +32,27 @@ thread_local char g_serving_error[256] = "";
 // thread builds a 128-bit mask of its row.  What a row must not see still goes through P V as 0 * V, so in those tiles
 // the non-finite elements of V are replaced by zeros in shared memory; the epilogue adds them back to the rows that do
 // see them.
-constexpr int kAttRows = 128, kAttTile = 64;      // query rows per CTA, slots per tile
+constexpr int kAttRows = 128, kAttTile = 64;      // query rows per tile of them, slots per tile
 constexpr int kAttQBytes = kAttRows * 128;
 constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 bytes (head_dim 32: the upper half is zero-filled)
 constexpr int kAttStages = 4;
-constexpr int kAttHalf = kAttTile / 2;            // slots of a tile that one softmax thread works on
-constexpr int kAttSoftmax = 2 * kAttRows;         // 8 softmax warps
-constexpr int kAttThreads = kAttSoftmax + 32;     // and one warp for the copies and the products
+constexpr int kAttThreads = 2 * kAttRows + 64;    // two groups of 4 softmax warps, the products' warp, the copies' warp
 constexpr int kAttCtasPerSm = 2;
-constexpr int kMaxPoison = 768;                   // slots of masked tiles that can hold a non-finite V element
-constexpr uint32_t kTmemS = 0, kTmemO = 128, kAttTmemCols = 256;  // two tiles of S; O of each half
+constexpr int kMaxPoison = 1536;                  // slots of masked tiles that can hold a non-finite V element, noted by each group
+constexpr uint32_t kTmemS = 0, kTmemO = 64, kTmemGroup = 128, kAttTmemCols = 256;  // per group: S (P in its first columns), O
 
 struct AttCtrl {
-  uint64_t k_full[kAttStages], v_full[kAttStages], s_full[2], p_full[2], pv_done, retired;
+  uint64_t full[kAttStages], empty[kAttStages], s_full[2], p_full[2], retired;
   uint32_t tmem_base;
   int abort, depth_lo, depth_hi, n_poison;
   int poison[kMaxPoison];
 };
-constexpr size_t kAttSmem = kAttQBytes + kAttTileBytes * 2 * kAttStages + 1024 + sizeof(AttCtrl);
+constexpr size_t kAttSmem = 2 * kAttQBytes + kAttTileBytes * 2 * kAttStages + 1024 + sizeof(AttCtrl);
 
 struct AttParams {
   CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 64, 1}
   gptoss_tree_attention_args a;
-  int group, nodes_per_tile, q_tiles, n_splits, tiles_per_split;
+  int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
   float c;                   // scale * log2(e)
 };
 
@@ -176,60 +174,57 @@ __device__ __forceinline__ uint32_t bf16_finite_part(uint32_t pair) {
   return pair & ((pair & 0x7f80u) == 0x7f80u ? 0xffff0000u : ~0u) & ((pair & 0x7f800000u) == 0x7f800000u ? 0x0000ffffu : ~0u);
 }
 
-constexpr uint32_t kPollLimit = 1u << 22;
-__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // mbar_wait in line: around a call the compiler would spill the row of scores that a softmax thread holds.
-__device__ __forceinline__ void wait_here(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
-  const uint32_t addr = smem_u32(bar);
-  volatile int *ab = abort_flag;
+__device__ __forceinline__ void wait_addr(uint32_t addr, uint32_t parity, volatile int *abort_flag, int site) {
   uint32_t i = 0;
-  while (!mbar_test_wait(addr, parity)) {
-    if (*ab) return;
-    if (++i == kPollLimit) {
-      *ab = 1;
+  while (!mbar_try_wait(addr, parity)) {
+    if (*abort_flag) return;
+    if (++i == kSpinLimit) {
+      *abort_flag = 1;
       if (atomicCAS(g_serving_status, 0, kDevErrTimeout) == 0) g_serving_status[1] = site, g_serving_status[2] = (int)blockIdx.x;
       return;
     }
   }
 }
-
 __device__ __forceinline__ void wait_warp(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
-  wait_here(bar, parity, abort_flag, site);
+  wait_addr(smem_u32(bar), parity, abort_flag, site);
   __syncwarp();
+}
+
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0;
 }
 
 template <int HD>
 __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_kernel(const __grid_constant__ AttParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t q_s = (raw + 1023u) & ~1023u, k_s = q_s + kAttQBytes, v_s = k_s + kAttStages * kAttTileBytes;
+  const uint32_t q_s = (raw + 1023u) & ~1023u, k_s = q_s + 2 * kAttQBytes, v_s = k_s + kAttStages * kAttTileBytes;
   uint8_t *const smem = smem_raw + (q_s - raw);
-  AttCtrl *ctrl = reinterpret_cast<AttCtrl *>(smem + kAttQBytes + 2 * kAttStages * kAttTileBytes);
+  AttCtrl *ctrl = reinterpret_cast<AttCtrl *>(smem + 2 * kAttQBytes + 2 * kAttStages * kAttTileBytes);
   const gptoss_tree_attention_args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int x = blockIdx.x;
-  const int qt = x % p.q_tiles;
-  x /= p.q_tiles;
+  const int pair = x % p.q_pairs;
+  x /= p.q_pairs;
   const int split = x % p.n_splits;
   x /= p.n_splits;
   const int kvh = x % a.n_kv_heads, b = x / a.n_kv_heads;
   pdl_wait();
   const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
-  const int n0 = qt * p.nodes_per_tile, nodes = min(n - n0, p.nodes_per_tile);
+  const int n0 = 2 * pair * p.nodes_per_tile, nodes = n - n0;
   if (first < 0 || nodes <= 0) {
     pdl_launch_dependents();
     return;
   }
+  const bool by_rows = nodes > p.nodes_per_tile;  // a query tile for each group, else the slot tiles are dealt out to them
   const int row = a.rows ? a.rows[b] : b;
   int ctx = min(max(a.ctx_len[b], 0), a.max_seq);
   int len = min(ctx + n, a.max_seq);
@@ -237,9 +232,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const int slab = row * a.n_kv_heads + kvh;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kAttStages; ++i) mbar_init(smem_u32(&ctrl->k_full[i]), 1), mbar_init(smem_u32(&ctrl->v_full[i]), 1);
-    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctrl->s_full[i]), 1), mbar_init(smem_u32(&ctrl->p_full[i]), 8);
-    mbar_init(smem_u32(&ctrl->pv_done), 1);
+    for (int i = 0; i < kAttStages; ++i) mbar_init(smem_u32(&ctrl->full[i]), 1), mbar_init(smem_u32(&ctrl->empty[i]), 1);
+    for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctrl->s_full[i]), 1), mbar_init(smem_u32(&ctrl->p_full[i]), 4);
     mbar_init(smem_u32(&ctrl->retired), 1);
     ctrl->abort = 0, ctrl->n_poison = 0, ctrl->depth_lo = 0x3fffffff, ctrl->depth_hi = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -250,13 +244,15 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   }
   // query rows into shared memory, in the layout a 128-byte-swizzled copy would give them (rows beyond the tree hold
   // whatever lies there: a row of the products depends on its own row of Q only)
-  const int r = threadIdx.x % kAttRows, half = threadIdx.x / kAttRows, node = r / p.group, head = kvh * p.group + r % p.group;
-  const bool valid = half < 2 && node < nodes;
+  const int r = threadIdx.x % kAttRows, g = threadIdx.x / kAttRows;
+  const int tile_node = by_rows ? g * p.nodes_per_tile : 0;  // first node of this group's query tile
+  const int node = tile_node + r / p.group, head = kvh * p.group + r % p.group;
+  const bool valid = g < 2 && r < p.nodes_per_tile * p.group && node < nodes;
   const int tok = first + n0 + (valid ? node : 0);
-  if (valid && half == 0) {
+  if (valid && (by_rows || g == 0)) {
     const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
 #pragma unroll
-    for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + r * 128 + ((c ^ (r & 7)) << 4)) = src[c];
+    for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + g * kAttQBytes + r * 128 + ((c ^ (r & 7)) << 4)) = src[c];
   }
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
@@ -275,90 +271,125 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const int n_tiles = (split == p.n_splits - 1 ? tiles : min(tiles, t_begin + p.tiles_per_split)) - t_begin;
   const int slot_first = lo_min + t_begin * kAttTile;
 
-  if (warp == 8) {
-    // ===================== copies and products =====================
-    // Products run in the order of their issue, and the completion that a commit signals covers all before it.  Two tiles
-    // of S are under way: while the softmax threads work on one, Q K^T of the next is done.  P of tile i being there
-    // (p_full) says that the softmax threads saw S of tile i, hence that Q K^T of tile i and P V of tile i - 2 are
-    // complete: their K and V tiles can be overwritten.  P of tile i is read by P V before Q K^T of tile i + 2, issued
-    // behind it, overwrites it.
-    if (lane == 0 && n_tiles > 0) {
+  if (warp == 9) {
+    // ===================== copies: a stage of the ring holds the K and the V tile of 64 slots =====================
+    int i = 0;
+    for (; i < n_tiles; ++i) {
+      const int st = i % kAttStages;
+      if (i >= kAttStages) wait_warp(&ctrl->empty[st], ((i / kAttStages) & 1) ^ 1, &ctrl->abort, 0x2000 | st);
+      if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int *>(&ctrl->abort))) break;
+      if (elect_one()) {
+        const uint32_t full = smem_u32(&ctrl->full[st]);
+        mbar_expect_tx(full, 2 * kAttTileBytes);
+        tma_load_3d(k_s + st * kAttTileBytes, &p.map_k, full, 0, slot_first + i * kAttTile, slab);
+        tma_load_3d(v_s + st * kAttTileBytes, &p.map_v, full, 0, slot_first + i * kAttTile, slab);
+      }
+      __syncwarp();
+    }
+    if (i < n_tiles || *reinterpret_cast<volatile int *>(&ctrl->abort))  // gave up: what is under way has to land first
+      for (int j = max(0, i - kAttStages); j < i; ++j)
+        for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
+    __syncwarp();
+  } else if (warp == 8) {
+    // ===================== products =====================
+    // They run in the order of their issue, and the completion that a commit signals covers all before it: S of a group's
+    // tile being there says that its P V before is complete too.  While one group's exponentials run, the other group's
+    // products do.
+    // One elected lane does it all (elect.sync tells the compiler that one thread runs; under a plain lane == 0 every issue
+    // becomes a loop over lanes).  Its instructions stand between P and the next S: addresses and descriptors are kept as
+    // running values.
+    if (elect_one()) {
       const uint32_t idesc_s = umma_idesc(kAttTile), idesc_o = umma_idesc(HD) | kIdescTransposeB;
-      const uint64_t dq = smem_desc_sw128(q_s);
-      auto copy = [&](const CUtensorMap *map, uint32_t dst, uint64_t *bar, int i) {
-        const uint32_t full = smem_u32(bar + i % kAttStages);
-        mbar_expect_tx(full, kAttTileBytes);
-        tma_load_3d(dst + (i % kAttStages) * kAttTileBytes, map, full, 0, slot_first + i * kAttTile, slab);
-      };
-      auto scores = [&](int i) {
-        const uint64_t dk = smem_desc_sw128(k_s + (i % kAttStages) * kAttTileBytes);
-        const uint32_t d = tmem + kTmemS + (i & 1) * kAttTile;
+      const uint32_t full = smem_u32(ctrl->full), empty = smem_u32(ctrl->empty), s_full = smem_u32(ctrl->s_full),
+                     p_full = smem_u32(ctrl->p_full);
+      const uint64_t dq = smem_desc_sw128(q_s), dk = smem_desc_sw128(k_s), dv = smem_desc_v(v_s);
+      constexpr uint64_t kStageDesc = kAttTileBytes >> 4;
+      const uint64_t dq1 = by_rows ? dq + (kAttQBytes >> 4) : dq;
+      auto scores = [&](int grp, int stage) {
+        const uint64_t d = dk + stage * kStageDesc, e = grp ? dq1 : dq;
 #pragma unroll
-        for (int k = 0; k < HD / 16; ++k) umma_bf16(d, dq + (uint64_t)(2 * k), dk + (uint64_t)(2 * k), idesc_s, k > 0);
-        umma_commit(smem_u32(&ctrl->s_full[i & 1]));
+        for (int k = 0; k < HD / 16; ++k)
+          umma_bf16(tmem + grp * kTmemGroup + kTmemS, e + (uint64_t)(2 * k), d + (uint64_t)(2 * k), idesc_s, k > 0);
+        umma_commit(s_full + 8 * grp);
       };
-      auto landed = [&](uint64_t *bar, int i, int site) {
-        wait_here(bar + i % kAttStages, (i / kAttStages) & 1, &ctrl->abort, site);
-      };
-      int k_sent = 0, v_sent = 0;
-      for (; k_sent < min(kAttStages, n_tiles); ++k_sent) {
-        copy(&p.map_k, k_s, ctrl->k_full, k_sent);
-        copy(&p.map_v, v_s, ctrl->v_full, v_sent++);
-      }
-      for (int i = 0; i < min(2, n_tiles); ++i) {
-        landed(ctrl->k_full, i, 0x2200);
-        tc_fence_after();
-        scores(i);
-      }
-      for (int i = 0; i < n_tiles; ++i) {
-        const bool more = i + 2 < n_tiles;
-        landed(ctrl->v_full, i, 0x2400);
-        if (more) landed(ctrl->k_full, i + 2, 0x2300);
-        const uint64_t dv = smem_desc_v(v_s + (i % kAttStages) * kAttTileBytes);
-        const uint32_t tp = tmem + kTmemS + (i & 1) * kAttTile;
-        wait_here(&ctrl->p_full[i & 1], (i >> 1) & 1, &ctrl->abort, 0x2500);
-        tc_fence_after();
+      auto output = [&](int grp, int stage, bool add) {
+        const uint64_t d = dv + stage * kStageDesc;
+        const uint32_t t = tmem + grp * kTmemGroup;
 #pragma unroll
-        for (int k = 0; k < kAttTile / 16; ++k)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V; 2 such steps per half
-          umma_bf16_ts(tmem + kTmemO + (k >> 1) * 64, tp + (k >> 1) * kAttHalf + (k & 1) * 8, dv + (uint64_t)(128 * k), idesc_o,
-                       i > 0 || (k & 1) != 0);
-        umma_commit(smem_u32(&ctrl->pv_done));
-        if (more) scores(i + 2);
-        if (*reinterpret_cast<volatile int *>(&ctrl->abort)) break;
-        if (k_sent < n_tiles) copy(&p.map_k, k_s, ctrl->k_full, k_sent++);                     // tile i + kAttStages
-        if (i > 1 && v_sent < n_tiles) copy(&p.map_v, v_s, ctrl->v_full, v_sent++);  // tile i - 2 + kAttStages
+        for (int c = 0; c < kAttTile / 16; ++c)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V
+          umma_bf16_ts(t + kTmemO, t + kTmemS + 8 * c, d + (uint64_t)(128 * c), idesc_o, add || c > 0);
+      };
+      int stage = 0, ahead = 0;          // of tile i; of the next tile whose S is wanted
+      uint32_t ahead_phase = 0;
+      auto advance = [&] {
+        if (++ahead == kAttStages) ahead = 0, ahead_phase ^= 1;
+      };
+      for (int grp = 0; grp < 2 && (by_rows ? 0 : grp) < n_tiles; ++grp) {
+        if (grp == 0 || !by_rows) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2200);
+        tc_fence_after();
+        scores(grp, ahead);
+        if (grp == 1 || !by_rows) advance();
+      }
+      if (by_rows) {
+        for (int i = 0; i < n_tiles; ++i) {
+          const bool more = i + 1 < n_tiles;
+          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2201);
+          wait_addr(p_full, i & 1, &ctrl->abort, 0x2500);
+          tc_fence_after();
+          output(0, stage, i > 0);
+          if (more) scores(0, ahead);
+          wait_addr(p_full + 8, i & 1, &ctrl->abort, 0x2501);
+          tc_fence_after();
+          output(1, stage, i > 0);
+          umma_commit(empty + 8 * stage);
+          if (more) {
+            scores(1, ahead);
+            advance();
+          }
+          stage = stage + 1 == kAttStages ? 0 : stage + 1;
+        }
+      } else {
+        for (int i = 0; i < n_tiles; ++i) {
+          const bool more = i + 2 < n_tiles;
+          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2202);
+          wait_addr(p_full + 8 * (i & 1), (i >> 1) & 1, &ctrl->abort, 0x2502);
+          tc_fence_after();
+          output(i & 1, stage, i > 1);
+          umma_commit(empty + 8 * stage);
+          if (more) {
+            scores(i & 1, ahead);
+            advance();
+          }
+          stage = stage + 1 == kAttStages ? 0 : stage + 1;
+        }
       }
       umma_commit(smem_u32(&ctrl->retired));
-      if (*reinterpret_cast<volatile int *>(&ctrl->abort)) {
-        // gave up: what was issued has to retire before shared memory and TMEM are given away
-        for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->retired), 0); ++w) {}
-        for (int j = max(0, k_sent - kAttStages); j < k_sent; ++j)
-          for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->k_full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
-        for (int j = max(0, v_sent - kAttStages); j < v_sent; ++j)
-          for (uint32_t w = 0; w < kPollLimit && !mbar_test_wait(smem_u32(&ctrl->v_full[j % kAttStages]), (j / kAttStages) & 1); ++w) {}
-      }
+      if (*reinterpret_cast<volatile int *>(&ctrl->abort))  // gave up: what was issued has to retire before TMEM is given away
+        for (uint32_t w = 0; w < kSpinLimit && !mbar_try_wait(smem_u32(&ctrl->retired), 0); ++w) {}
     }
+    __syncwarp();
   } else {
     // ===================== softmax, a thread per query row =====================
     RowView view{ctx, len - ctx, a.window > 0 ? min(max(ctx + depth - a.window + 1, 0), ctx) : 0, a.window, depth, a.mask_words,
                  a.mask + (size_t)tok * a.mask_words, a.depth + first};
-    const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16, to = tmem + lane_addr + kTmemO + half * 64;
+    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * kTmemGroup + kTmemS, to = ts + kTmemO;
     const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
     float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < n_tiles; ++i) {
+    int k = 0;
+    for (int i = by_rows ? 0 : g; i < n_tiles; i += by_rows ? 1 : 2, ++k) {
       const int t0 = slot_first + i * kAttTile;
       const bool masked = t0 < lo_max || t0 + kAttTile > ctx;
-      uint32_t bits = 0;
+      uint32_t bits[2] = {0u, 0u};
       if (masked) {
-        if (valid) bits = view.word(t0 + kAttHalf * half);
-        // a quarter of slot threadIdx.x / 4 of this tile: non-finite elements of V become zeros, and the slot is noted if
-        // anyone can see it
-        const int vs = i % kAttStages;
-        wait_warp(&ctrl->v_full[vs], (i / kAttStages) & 1, &ctrl->abort, 0x2700);
-        uint4 *vr = reinterpret_cast<uint4 *>(smem + kAttQBytes + (kAttStages + vs) * kAttTileBytes + threadIdx.x * 32);
+        if (valid) bits[0] = view.word(t0), bits[1] = view.word(t0 + 32);
+        // half of slot r / 2 of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
+        // (two groups on one tile both look at all of it: what the second still finds, the first has written as well)
+        const int st = i % kAttStages;
+        wait_warp(&ctrl->full[st], (i / kAttStages) & 1, &ctrl->abort, 0x2700);
+        uint4 *vr = reinterpret_cast<uint4 *>(smem + 2 * kAttQBytes + (kAttStages + st) * kAttTileBytes + r * 64);
         int bad = 0;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < 4; ++c) {
           uint4 v = vr[c];
           if (bf16_nonfinite(v.x) || bf16_nonfinite(v.y) || bf16_nonfinite(v.z) || bf16_nonfinite(v.w)) {
             bad = 1;
@@ -368,38 +399,34 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         }
         __syncwarp();
         bad |= __shfl_xor_sync(0xffffffffu, bad, 1);
-        bad |= __shfl_xor_sync(0xffffffffu, bad, 2);
-        const int slot = t0 + (threadIdx.x >> 2);
-        if (bad && (lane & 3) == 0 && slot < len) {
+        if (bad && !(r & 1) && t0 + (r >> 1) < len) {
           const int at = atomicAdd(&ctrl->n_poison, 1);
-          if (at < kMaxPoison) ctrl->poison[at] = slot;
+          if (at < kMaxPoison) ctrl->poison[at] = t0 + (r >> 1);
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      float s[kAttHalf];
-      const uint32_t ts = tmem + lane_addr + kTmemS + (i & 1) * kAttTile + half * kAttHalf;
-      wait_warp(&ctrl->s_full[i & 1], (i >> 1) & 1, &ctrl->abort, 0x2600);
+      float s[kAttTile];
+      wait_warp(&ctrl->s_full[g], k & 1, &ctrl->abort, 0x2600);
       tc_fence_after();
       if (live) {
-        tmem_ld32(ts, s);
+#pragma unroll
+        for (int j = 0; j < kAttTile; j += 32) tmem_ld32(ts + j, s + j);
         tmem_ld_wait();
         if (masked) {
 #pragma unroll
-          for (int j = 0; j < kAttHalf; ++j) s[j] = (bits >> j & 1u) ? s[j] : -INFINITY;
+          for (int j = 0; j < kAttTile; ++j) s[j] = (bits[j >> 5] >> (j & 31) & 1u) ? s[j] : -INFINITY;
         }
-        float mx[2] = {max3_nan(s[0], s[1], s[2]), max3_nan(s[3], s[4], s[5])};
+        float mx[4] = {max3_nan(s[0], s[1], s[2]), max3_nan(s[3], s[4], s[5]), max3_nan(s[6], s[7], s[8]), max3_nan(s[9], s[10], s[11])};
 #pragma unroll
-        for (int j = 6; j + 1 < kAttHalf; j += 2) mx[(j >> 1) & 1] = max3_nan(mx[(j >> 1) & 1], s[j], s[j + 1]);
-        const float top = max3_nan(mx[0], mx[1], mx[1]) * p.c;
+        for (int j = 12; j + 1 < kAttTile; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], s[j], s[j + 1]);
+        const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.c;
         const bool move = top > m + 8.f;
         float corr = 1.f;
         if (move) {
           corr = ex2(m - top);
           m = top;
         }
-        if (i > 0 && __any_sync(0xffffffffu, move)) {
-          wait_warp(&ctrl->pv_done, (i - 1) & 1, &ctrl->abort, 0x2800);
-          tc_fence_after();
+        if (k > 0 && __any_sync(0xffffffffu, move)) {
 #pragma unroll
           for (int h = 0; h < HD; h += 16) {
             uint32_t o[16];
@@ -413,50 +440,56 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         const float base = m == -INFINITY ? 0.f : m;
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         const float2 c2 = make_float2(p.c, p.c), base2 = make_float2(-base, -base);
-        uint32_t pk[kAttHalf / 2];
 #pragma unroll
-        for (int j = 0; j < kAttHalf; j += 2) {
-          const float2 x = fma2(make_float2(s[j], s[j + 1]), c2, base2);
-          const float2 e = make_float2(ex2(x.x), ex2(x.y));
-          sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
-          pk[j >> 1] = pack_bf16(e.x, e.y);
+        for (int h = 0; h < kAttTile; h += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float2 x = fma2(make_float2(s[h + j], s[h + j + 1]), c2, base2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+            pk[j >> 1] = pack_bf16(e.x, e.y);
+          }
+          tmem_st16(ts + (h >> 1), pk);
         }
-        tmem_st16(ts, pk);
         l = l * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
         tmem_st_wait();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full[i & 1]));
+      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full[g]));
     }
     // ---- result of this share of the context ----
-    if (n_tiles > 0) wait_warp(&ctrl->retired, 0, &ctrl->abort, 0x2900);
+    wait_warp(&ctrl->retired, 0, &ctrl->abort, 0x2900);
     tc_fence_after();
     float o[HD];
 #pragma unroll
     for (int j = 0; j < HD; ++j) o[j] = 0.f;
-    if (live && n_tiles > 0) {
+    if (live && k > 0) {
 #pragma unroll
       for (int h = 0; h < HD; h += 32) tmem_ld32(to + h, o + h);
       tmem_ld_wait();
     }
-    // the second half of each row goes to the first through shared memory; no copy or product is under way any more
-    float *join = reinterpret_cast<float *>(smem + kAttQBytes) + r;
-    static_assert((HD + 2) * kAttRows * 4 <= 2 * kAttStages * kAttTileBytes, "the halves meet in the ring's memory");
-    if (half == 1) {
+    // groups that shared out the slot tiles: the second's part of each row goes to the first through shared memory (no copy
+    // or product is under way any more)
+    float *join = reinterpret_cast<float *>(smem + 2 * kAttQBytes) + r;
+    static_assert((HD + 2) * kAttRows * 4 <= 2 * kAttStages * kAttTileBytes, "the groups meet in the ring's memory");
+    if (!by_rows && g == 1) {
 #pragma unroll
       for (int j = 0; j < HD; ++j) join[j * kAttRows] = o[j];
       join[HD * kAttRows] = m;
       join[(HD + 1) * kAttRows] = l;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (half == 0 && valid) {
-      const float m1 = join[HD * kAttRows], top1 = fmaxf(m, m1), base1 = top1 == -INFINITY ? 0.f : top1;
-      const float w0 = ex2(m - base1), w1 = ex2(m1 - base1);
-      l = fmaf(l, w0, join[(HD + 1) * kAttRows] * w1);
-      m = top1;
+    if (valid && (by_rows || g == 0)) {
+      if (!by_rows) {
+        const float m1 = join[HD * kAttRows], top1 = fmaxf(m, m1), base1 = top1 == -INFINITY ? 0.f : top1;
+        const float w0 = ex2(m - base1), w1 = ex2(m1 - base1);
+        l = fmaf(l, w0, join[(HD + 1) * kAttRows] * w1);
+        m = top1;
 #pragma unroll
-      for (int j = 0; j < HD; ++j) o[j] = fmaf(o[j], w0, join[j * kAttRows] * w1);
+        for (int j = 0; j < HD; ++j) o[j] = fmaf(o[j], w0, join[j * kAttRows] * w1);
+      }
       const int bad = min(ctrl->n_poison, kMaxPoison);
       for (int i = 0; i < bad; ++i) {
         const int slot = ctrl->poison[i];
@@ -586,16 +619,16 @@ namespace {
 // How a call is cut: query tiles, and shares of the context when the (sequence, kv head, query tile) items alone would not
 // fill two CTAs on every SM.
 struct AttPlan {
-  int group, nodes_per_tile, q_tiles, n_splits, tiles_per_split;
+  int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
 };
 AttPlan plan_of(const gptoss_tree_attention_args &a) {
   AttPlan p;
   p.group = a.n_q_heads / a.n_kv_heads;
   p.nodes_per_tile = kAttRows / p.group;
-  p.q_tiles = (a.max_nodes + p.nodes_per_tile - 1) / p.nodes_per_tile;
+  p.q_pairs = (a.max_nodes + 2 * p.nodes_per_tile - 1) / (2 * p.nodes_per_tile);
   int device = 0, sms = kSmCountFallback;
   if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  const long long items = (long long)a.n_seqs * a.n_kv_heads * p.q_tiles;
+  const long long items = (long long)a.n_seqs * a.n_kv_heads * p.q_pairs;
   // the cached tokens that a tree can reach: with a window, as many as its first token sees
   const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
@@ -620,7 +653,7 @@ template <int HD>
 cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
   cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_tiles * p.n_splits));
+  const dim3 grid((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_pairs * p.n_splits));
   e = launch_chain(tree_attention_kernel<HD>, grid, dim3(kAttThreads), kAttSmem, s, p);
   if (e != cudaSuccess || p.n_splits == 1) return e;
   const int heads = 256 / (HD / 4);
@@ -672,12 +705,12 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
   const uint64_t need = workspace_of(a, plan.n_splits);
   if (need && (!a.workspace || !aligned16(a.workspace) || a.workspace_bytes < need))
     return serving_fail(GPTOSS_ERR_BAD_ARG, "workspace missing, misaligned or below gptoss_tree_attention_workspace()");
-  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff || (int64_t)a.n_seqs * a.n_kv_heads * plan.q_tiles * plan.n_splits > 0x7fffffff ||
+  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff || (int64_t)a.n_seqs * a.n_kv_heads * plan.q_pairs * plan.n_splits > 0x7fffffff ||
       (int64_t)a.cache_rows * a.n_kv_heads > 0x7fffffff)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "too many drafted tokens or cache rows");
   AttParams p;
   p.a = a;
-  p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.q_tiles = plan.q_tiles;
+  p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.q_pairs = plan.q_pairs;
   p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
   p.c = a.scale * 1.44269504f;
   const uint64_t slabs = (uint64_t)a.cache_rows * a.n_kv_heads;
