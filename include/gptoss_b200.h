@@ -335,7 +335,8 @@ int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_ro
  * outside [0, n_adapters) has no adapter (out[t] = y[t]).  x [T][K] bf16, a [n_adapters][rank][K] bf16,
  * b [n_adapters][n_out][rank] bf16, scale [n_adapters] fp32 or NULL for 1, y and out [T][n_out] fp32; out may be y.
  * Products accumulate in fp32 and the intermediate A x is not rounded.  K and n_out multiples of 8, rank a
- * multiple of 8 up to GPTOSS_LORA_MAX_RANK (adapters of lower rank: zero rows of A, zero columns of B). */
+ * multiple of 8 up to GPTOSS_LORA_MAX_RANK (adapters of lower rank: zero rows of A, zero columns of B), at most 8192
+ * adapters.  What adapters that no token uses and rows of x without an adapter hold does not matter. */
 #define GPTOSS_LORA_MAX_RANK 128
 typedef struct {
   const void *x, *a, *b;
