@@ -10,6 +10,9 @@
 Each call runs on the device of its tensors, asynchronously on ``stream`` (default: that device's current stream); scratch
 comes from torch's allocator, so calls on different streams and captured graphs have their own.  Errors raise
 ``GptossError``.  Nothing is kept between calls.
+
+The calls are short on the GPU (from 2 us), so their host side counts: checks are plain attribute comparisons, and the
+raw stream handle is asked for directly (a ``torch.cuda.Stream`` object costs 3 us, a device context 1.4 us).
 """
 from __future__ import annotations
 
@@ -23,10 +26,12 @@ from .moe import GptossError
 
 TREE_MAX_NODES = 256
 _SCORING = {"softmax": 0, "sigmoid": 1}
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _check(rc):
-    if rc != capi.OK:
+    if rc:
         raise GptossError(rc, capi.load().gptoss_serving_last_error().decode())
 
 
@@ -34,29 +39,33 @@ def _bad(message):
     raise GptossError(capi.ERR_BAD_ARG, message)
 
 
-def _need(name, t, dtype, ndim, device=None):
-    """t is a cuda tensor of that type and rank, contiguous in its last dimension, on `device`."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.dim() != ndim:
-        _bad(f"{name} must be a {dtype} tensor of {ndim} dimensions")
-    if not t.is_cuda:
-        _bad(f"{name} must be a cuda tensor")
-    if device is not None and t.device != device:
-        _bad(f"{name} is on {t.device}, expected {device}")
+def _view(name, t, dtype, ndim, dev=None):
+    """t is a tensor of that type and number of dimensions on cuda device `dev` (default: any); returns its device."""
+    try:
+        at = t.get_device()
+        if t.dtype is dtype and t.dim() == ndim and at >= 0 and (dev is None or at == dev):
+            return at
+    except AttributeError:
+        pass
+    where = "a cuda device" if dev is None else f"cuda:{dev}"
+    _bad(f"{name} must be a {dtype} tensor of {ndim} dimensions on {where}")
 
 
-def _dense(name, t, dtype, ndim, device):
-    _need(name, t, dtype, ndim, device)
+def _dense(name, t, dtype, ndim, dev):
+    _view(name, t, dtype, ndim, dev)
     if not t.is_contiguous():
         _bad(f"{name} must be contiguous")
 
 
-def _launch(device, stream, call):
-    """call(stream handle) with `device` current and, for what it allocates, `stream` as torch's current stream."""
-    with torch.cuda.device(device):
+def _launch(dev, stream, call, *args):
+    """call(stream handle, *args) with device `dev` current and, for what it allocates, `stream` as torch's current one."""
+    if stream is None and _current_device() == dev:
+        return call(_raw_stream(dev), *args)
+    with torch.cuda.device(dev):
         if stream is None:
-            return call(C.c_void_p(torch.cuda.current_stream().cuda_stream))
+            return call(_raw_stream(dev), *args)
         with torch.cuda.stream(stream):
-            return call(C.c_void_p(stream.cuda_stream))
+            return call(stream.cuda_stream, *args)
 
 
 def tree_masks(parents, max_nodes=None):
@@ -92,58 +101,63 @@ def tree_attention(q, k_cache, v_cache, offsets, ctx_len, mask, depth=None, *, m
     offsets int32 [B+1], ctx_len int32 [B], mask int32 [n_tokens, words], depth int32 [n_tokens] (with a window), sinks fp32
     [n_q_heads], cache_rows int32 [B].  max_nodes / max_ctx: upper bounds of the drafted / cached tokens of a sequence.
     Returns out like q (bf16); rows behind the last sequence are not written."""
-    _need("q", q, torch.bfloat16, 3)
-    dev = q.device
+    dev = _view("q", q, _BF16, 3)
     n_tokens, nq, hd = q.shape
-    if q.stride(2) != 1 or q.stride(1) != hd:
+    token_stride, head_stride, last = q.stride()
+    if last != 1 or (head_stride != hd and nq > 1):
         _bad("q: heads of a token must be contiguous")
-    _dense("k_cache", k_cache, torch.bfloat16, 4, dev)
-    _dense("v_cache", v_cache, torch.bfloat16, 4, dev)
-    if k_cache.shape != v_cache.shape or k_cache.shape[3] != hd:
+    _dense("k_cache", k_cache, _BF16, 4, dev)
+    _dense("v_cache", v_cache, _BF16, 4, dev)
+    rows, nkv, max_seq, cache_hd = k_cache.shape
+    if v_cache.shape != k_cache.shape or cache_hd != hd:
         _bad("k_cache and v_cache must have the same shape and q's head_dim")
-    _dense("offsets", offsets, torch.int32, 1, dev)
-    _dense("ctx_len", ctx_len, torch.int32, 1, dev)
-    _dense("mask", mask, torch.int32, 2, dev)
+    _dense("offsets", offsets, _I32, 1, dev)
+    _dense("ctx_len", ctx_len, _I32, 1, dev)
+    _dense("mask", mask, _I32, 2, dev)
     n_seqs = ctx_len.shape[0]
-    if offsets.shape[0] != n_seqs + 1 or mask.shape[0] < n_tokens:
+    mask_rows, words = mask.shape
+    if offsets.shape[0] != n_seqs + 1 or mask_rows < n_tokens:
         _bad("offsets needs one more entry than ctx_len, mask a row per token")
+    depth_at = sinks_at = rows_at = None
     if depth is not None:
-        _dense("depth", depth, torch.int32, 1, dev)
+        _dense("depth", depth, _I32, 1, dev)
         if depth.shape[0] < n_tokens:
             _bad("depth needs an entry per token")
+        depth_at = depth.data_ptr()
     if sinks is not None:
-        _dense("sinks", sinks, torch.float32, 1, dev)
+        _dense("sinks", sinks, _F32, 1, dev)
         if sinks.shape[0] != nq:
             _bad("sinks needs an entry per query head")
+        sinks_at = sinks.data_ptr()
     if cache_rows is not None:
-        _dense("cache_rows", cache_rows, torch.int32, 1, dev)
+        _dense("cache_rows", cache_rows, _I32, 1, dev)
         if cache_rows.shape[0] != n_seqs:
             _bad("cache_rows needs an entry per sequence")
+        rows_at = cache_rows.data_ptr()
     if out is not None:
-        _need("out", out, torch.bfloat16, 3, dev)
-        if out.shape != q.shape or out.stride(2) != 1 or out.stride(1) != hd:
+        _view("out", out, _BF16, 3, dev)
+        if out.shape != q.shape or out.stride(2) != 1 or (out.stride(1) != hd and nq > 1):
             _bad("out must have q's shape and contiguous heads")
-    rows, nkv, max_seq, _ = k_cache.shape
-    stride = lambda t: t.stride(0) if n_tokens > 1 else nq * hd  # noqa: E731
+    if n_tokens <= 1:
+        token_stride = nq * hd
     args = capi.TreeAttentionArgs(
-        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, offsets.data_ptr(), ctx_len.data_ptr(),
-        None if cache_rows is None else cache_rows.data_ptr(), mask.data_ptr(), None if depth is None else depth.data_ptr(),
-        None if sinks is None else sinks.data_ptr(), None, 0, stride(q), 0, n_tokens, n_seqs, max_nodes, max_ctx,
-        mask.shape[1], rows, max_seq, nq, nkv, hd, window, hd ** -0.5 if scale is None else scale)
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), None, offsets.data_ptr(), ctx_len.data_ptr(), rows_at,
+        mask.data_ptr(), depth_at, sinks_at, None, 0, token_stride, 0, n_tokens, n_seqs, max_nodes, max_ctx, words, rows, max_seq,
+        nq, nkv, hd, window, hd ** -0.5 if scale is None else scale)
+    return _launch(dev, stream, _tree_attention, args, q, out)
 
-    def call(s):
-        nonlocal out
-        if out is None:
-            out = torch.empty((n_tokens, nq, hd), dtype=torch.bfloat16, device=dev)
-        args.out, args.out_stride = out.data_ptr(), stride(out)
-        lib = capi.load()
-        need = lib.gptoss_tree_attention_workspace(C.byref(args))
-        if need:
-            work = torch.empty(need, dtype=torch.uint8, device=dev)
-            args.workspace, args.workspace_bytes = work.data_ptr(), need
-        _check(lib.gptoss_tree_attention(C.byref(args), s))
 
-    _launch(dev, stream, call)
+def _tree_attention(s, args, q, out):
+    lib = capi.load()
+    if out is None:
+        out = q.new_empty(q.shape)
+    args.out = out.data_ptr()
+    args.out_stride = out.stride(0) if args.n_tokens > 1 else args.n_q_heads * args.head_dim
+    need = lib.gptoss_tree_attention_workspace(C.byref(args))
+    if need:
+        work = q.new_empty(need, dtype=torch.uint8)
+        args.workspace, args.workspace_bytes = work.data_ptr(), need
+    _check(lib.gptoss_tree_attention(C.byref(args), s))
     return out
 
 
@@ -151,29 +165,33 @@ def cache_commit(k_cache, v_cache, ctx_len, offsets, path, *, max_path, cache_ro
     """Moves the accepted path of each tree into place, in the caches [layers, rows, n_kv_heads, max_seq, head_dim] (or
     without the layers), bf16.  path int32: the accepted drafted tokens of all sequences, ascending within one; sequence b
     has path[offsets[b]:offsets[b+1]], at most max_path.  ``gptoss_cache_commit`` in the C header."""
-    if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 and isinstance(v_cache, torch.Tensor):
-        k_cache, v_cache = k_cache[None], v_cache[None]
-    _need("k_cache", k_cache, torch.bfloat16, 5)
-    dev = k_cache.device
-    _dense("k_cache", k_cache, torch.bfloat16, 5, dev)
-    _dense("v_cache", v_cache, torch.bfloat16, 5, dev)
-    if k_cache.shape != v_cache.shape:
+    ndim = 4 if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 5
+    dev = _view("k_cache", k_cache, _BF16, ndim)
+    _dense("k_cache", k_cache, _BF16, ndim, dev)
+    _dense("v_cache", v_cache, _BF16, ndim, dev)
+    shape = k_cache.shape
+    if v_cache.shape != shape:
         _bad("k_cache and v_cache must have the same shape")
-    _dense("ctx_len", ctx_len, torch.int32, 1, dev)
-    _dense("offsets", offsets, torch.int32, 1, dev)
-    _dense("path", path, torch.int32, 1, dev)
+    _dense("ctx_len", ctx_len, _I32, 1, dev)
+    _dense("offsets", offsets, _I32, 1, dev)
+    _dense("path", path, _I32, 1, dev)
     n_seqs = ctx_len.shape[0]
     if offsets.shape[0] != n_seqs + 1:
         _bad("offsets needs one more entry than ctx_len")
+    rows_at = None
     if cache_rows is not None:
-        _dense("cache_rows", cache_rows, torch.int32, 1, dev)
+        _dense("cache_rows", cache_rows, _I32, 1, dev)
         if cache_rows.shape[0] != n_seqs:
             _bad("cache_rows needs an entry per sequence")
-    layers, rows, nkv, max_seq, hd = k_cache.shape
-    _launch(dev, stream, lambda s: _check(capi.load().gptoss_cache_commit(
-        k_cache.data_ptr(), v_cache.data_ptr(), layers, rows, nkv, max_seq, hd, n_seqs,
-        None if cache_rows is None else cache_rows.data_ptr(), ctx_len.data_ptr(), offsets.data_ptr(), path.data_ptr(),
-        max_path if path.shape[0] else 0, s)))
+        rows_at = cache_rows.data_ptr()
+    layers = 1 if ndim == 4 else shape[0]
+    rows, nkv, max_seq, hd = shape[-4:]
+    _launch(dev, stream, _cache_commit, k_cache.data_ptr(), v_cache.data_ptr(), layers, rows, nkv, max_seq, hd, n_seqs, rows_at,
+            ctx_len.data_ptr(), offsets.data_ptr(), path.data_ptr(), path.shape[0] and max_path)
+
+
+def _cache_commit(s, *args):
+    _check(capi.load().gptoss_cache_commit(*args, s))
 
 
 def lora_apply(x, a, b, ids, y, *, scale=None, out=None, stream=None):
@@ -181,69 +199,75 @@ def lora_apply(x, a, b, ids, y, *, scale=None, out=None, stream=None):
 
     x [T, K] bf16, a [n_adapters, rank, K] bf16, b [n_adapters, n_out, rank] bf16, ids int32 [T], y fp32 [T, n_out], scale
     fp32 [n_adapters].  out: y itself by default (in place).  ``gptoss_lora_apply`` in the C header."""
-    _need("x", x, torch.bfloat16, 2)
-    dev = x.device
+    dev = _view("x", x, _BF16, 2)
     T, K = x.shape
-    _dense("a", a, torch.bfloat16, 3, dev)
-    _dense("b", b, torch.bfloat16, 3, dev)
-    n, rank, _ = a.shape
-    n_out = b.shape[1]
-    if a.shape[2] != K or b.shape[0] != n or b.shape[2] != rank:
+    _dense("a", a, _BF16, 3, dev)
+    _dense("b", b, _BF16, 3, dev)
+    n, rank, a_k = a.shape
+    b_n, n_out, b_rank = b.shape
+    if a_k != K or b_n != n or b_rank != rank:
         _bad("a must be [n_adapters, rank, K] and b [n_adapters, n_out, rank]")
-    _dense("ids", ids, torch.int32, 1, dev)
-    out = y if out is None else out
-    for name, t in (("y", y), ("out", out)):
-        _need(name, t, torch.float32, 2, dev)
-        if t.shape != (T, n_out) or (n_out > 1 and t.stride(1) != 1):
-            _bad(f"{name} must be [T, n_out] with contiguous rows")
-    if ids.shape[0] != T or (K > 1 and x.stride(1) != 1):
+    _dense("ids", ids, _I32, 1, dev)
+    _view("y", y, _F32, 2, dev)
+    if out is None:
+        out = y
+    else:
+        _view("out", out, _F32, 2, dev)
+    x_stride, y_stride, out_stride = x.stride(), y.stride(), out.stride()
+    if y.shape != (T, n_out) or out.shape != y.shape or y_stride[1] != 1 or out_stride[1] != 1:
+        _bad("y and out must be [T, n_out] with contiguous rows")
+    if ids.shape[0] != T or x_stride[1] != 1:
         _bad("ids needs an entry per token, x contiguous rows")
+    scale_at = None
     if scale is not None:
-        _dense("scale", scale, torch.float32, 1, dev)
+        _dense("scale", scale, _F32, 1, dev)
         if scale.shape[0] != n:
             _bad("scale needs an entry per adapter")
+        scale_at = scale.data_ptr()
     one = T <= 1
-    args = capi.LoraArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), None if scale is None else scale.data_ptr(), ids.data_ptr(),
-                         y.data_ptr(), out.data_ptr(), None, 0, K if one else x.stride(0), n_out if one else y.stride(0),
-                         n_out if one else out.stride(0), T, K, n_out, rank, n)
-
-    def call(s):
-        lib = capi.load()
-        need = lib.gptoss_lora_workspace(C.byref(args))
-        if need:
-            work = torch.empty(need, dtype=torch.uint8, device=dev)
-            args.workspace, args.workspace_bytes = work.data_ptr(), need
-        _check(lib.gptoss_lora_apply(C.byref(args), s))
-
-    _launch(dev, stream, call)
+    args = capi.LoraArgs(x.data_ptr(), a.data_ptr(), b.data_ptr(), scale_at, ids.data_ptr(), y.data_ptr(), out.data_ptr(), None, 0,
+                         K if one else x_stride[0], n_out if one else y_stride[0], n_out if one else out_stride[0], T, K, n_out,
+                         rank, n)
+    _launch(dev, stream, _lora_apply, args, x)
     return out
+
+
+def _lora_apply(s, args, x):
+    lib = capi.load()
+    need = lib.gptoss_lora_workspace(C.byref(args))
+    if need:
+        work = x.new_empty(need, dtype=torch.uint8)
+        args.workspace, args.workspace_bytes = work.data_ptr(), need
+    _check(lib.gptoss_lora_apply(C.byref(args), s))
 
 
 def route_experts(logits, top_k, *, scoring="softmax", bias=None, n_groups=1, topk_groups=1, group_top=1, renormalize=True,
                   weight_scale=1.0, stream=None):
     """Experts of each token from router logits [T, E] fp32: (weights fp32 [T, top_k], ids int32 [T, top_k]) in descending
     order of the choice.  ``gptoss_expert_choice`` in the C header says how they are chosen."""
-    _need("logits", logits, torch.float32, 2)
-    dev = logits.device
+    dev = _view("logits", logits, _F32, 2)
     T, E = logits.shape
-    if E > 1 and logits.stride(1) != 1:
+    stride, last = logits.stride()
+    if last != 1 and E > 1:
         _bad("logits must have contiguous rows")
+    bias_at = None
     if bias is not None:
-        _dense("bias", bias, torch.float32, 1, dev)
+        _dense("bias", bias, _F32, 1, dev)
         if bias.shape[0] != E:
             _bad("bias needs an entry per expert")
+        bias_at = bias.data_ptr()
     if scoring not in _SCORING:
         _bad("scoring must be 'softmax' or 'sigmoid'")
     if not 1 <= top_k <= 8:
         _bad("top_k must be 1..8")
+    args = capi.ExpertChoiceArgs(logits.data_ptr(), bias_at, None, None, stride if T > 1 else E, T, E, top_k, _SCORING[scoring],
+                                 n_groups, topk_groups, group_top, 1 if renormalize else 0, weight_scale)
+    return _launch(dev, stream, _route_experts, args, logits)
 
-    def call(s):
-        w = torch.empty((T, top_k), dtype=torch.float32, device=dev)
-        ids = torch.empty((T, top_k), dtype=torch.int32, device=dev)
-        args = capi.ExpertChoiceArgs(logits.data_ptr(), None if bias is None else bias.data_ptr(), w.data_ptr(), ids.data_ptr(),
-                                     logits.stride(0) if T > 1 else E, T, E, top_k, _SCORING[scoring], n_groups, topk_groups,
-                                     group_top, int(renormalize), weight_scale)
-        _check(capi.load().gptoss_expert_choice(C.byref(args), s))
-        return w, ids
 
-    return _launch(dev, stream, call)
+def _route_experts(s, args, logits):
+    w = logits.new_empty((args.T, args.k))
+    ids = logits.new_empty((args.T, args.k), dtype=_I32)
+    args.topk_w, args.topk_i = w.data_ptr(), ids.data_ptr()
+    _check(capi.load().gptoss_expert_choice(C.byref(args), s))
+    return w, ids
