@@ -12,6 +12,7 @@
 //   lora_kernel       a cluster of 8 CTAs per tile: each computes u = A x over an eighth of K, the partial sums meet in
 //                     distributed shared memory, and each CTA adds s B u to an eighth of the outputs.  One launch, no
 //                     intermediate in memory.
+//   lora_shrink_kernel, lora_expand_kernel  from 2048 tokens on: the two products as two kernels
 // u is not rounded: its fp32 value enters the second product as three bf16 terms (24 bits).
 #include "serving.cuh"
 
@@ -23,14 +24,18 @@ constexpr int kTileTokens = 64;       // tokens of a tile: 4 tiles of 16 rows
 constexpr int kDirectTokens = 32;     // up to here a warp vote replaces the sort
 constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
+constexpr int kWideSplits = 2;        // parts of K with many tiles
+constexpr int kWideTokens = 2048;     // from here on a batch counts as many tiles
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
-constexpr int kSmallU = 512;          // values of u that every CTA of a cluster sums up by itself
+constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all
 
 struct LoraPlan {
   int4 *tiles;   // {adapter or -1, first position in perm, tokens, 0}
   int *perm;     // tokens ordered by adapter
   int *n_tiles;
+  float *u;       // many tiles: [kWideSplits][T][rank up to 16, 32, 64 or 128]
   int max_tiles;
+  bool wide;      // many tiles
   int skip_idle;  // out is y: tokens without an adapter need no work
 };
 
@@ -49,9 +54,11 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  for (int t = tid; t < T; t += 1024) {
-    const int id = ids[t];
-    atomicAdd(&bin_s[id >= 0 && id < n ? id : n], 1);
+  // neighbours often share an adapter: one atomic per adapter and warp
+  for (int t0 = 0; t0 < T; t0 += 1024) {
+    const int t = t0 + tid, id = t < T ? ids[t] : 0, bin = t < T ? (id >= 0 && id < n ? id : n) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, bin);
+    if (bin >= 0 && lane == __ffs(same) - 1) atomicAdd(&bin_s[bin], __popc(same));
   }
   __syncthreads();
   // exclusive prefix of the counts (positions) and of the tile counts; a thread owns `per` consecutive bins
@@ -82,9 +89,14 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   }
   __syncthreads();
   // where a token stands among those of its adapter varies from run to run; its result does not depend on it
-  for (int t = tid; t < T; t += 1024) {
-    const int id = ids[t];
-    p.perm[atomicAdd(&bin_s[id >= 0 && id < n ? id : n], 1)] = t;
+  for (int t0 = 0; t0 < T; t0 += 1024) {
+    const int t = t0 + tid, id = t < T ? ids[t] : 0, bin = t < T ? (id >= 0 && id < n ? id : n) : -1;
+    const uint32_t same = __match_any_sync(0xffffffffu, bin);
+    const int leader = __ffs(same) - 1;
+    int at = 0;
+    if (bin >= 0 && lane == leader) at = atomicAdd(&bin_s[bin], __popc(same));
+    at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
+    if (bin >= 0) p.perm[at] = t;
   }
 }
 
@@ -127,167 +139,173 @@ __device__ __forceinline__ void three_terms(float x, float y, uint32_t (&t)[3]) 
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
-__device__ __forceinline__ float ld_cluster(uint32_t addr, uint32_t rank) {
+__device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
   uint32_t there;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(there) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(there) : "memory");
   return v;
 }
 
-// RN: tiles of 8 ranks, at least rank / 8.
-// u: the warps are `wm` across the tile's 16-row blocks and 8 / wm along K; a CTA's partial sums are added in shared memory
-// in the order of the warps, the cluster's in the order of the CTAs.
-// out: again `wm` across the rows and 8 / wm along the outputs; a warp takes 16 outputs at a time, of which thread c of a
-// row owns [4c, 4c + 4) (column 2c + e of the j-th 8-wide product stands for output 4c + 2j + e), so that y and out move
-// 16 bytes per thread, 64 per row.  y is requested kAhead steps before its use.
+__device__ __forceinline__ void copy_async16(void *dst_shared, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst_shared)), "l"(src) : "memory");
+}
+
+constexpr int kYStages = 4;
+constexpr int kYStageFloats = 3072;  // 16 wm rows of 16 wn + 16 floats (the padding keeps 16-byte reads of 2 rows apart)
+
+// A CTA's view of its tile.  Its 8 warps stand `wm` across the tile's 16-row blocks and wn = 8 / wm along the other index.
+struct Work {
+  Tile t;
+  int wm, wn, m0, k;     // first row and place along the other index of this warp
+  int row, c;            // thread c of row `row` (and row + 8) of the 16
+  bool in0, in1;
+  size_t t0, t1;         // the tokens of those rows
+  __device__ __forceinline__ explicit Work(const Tile &tile) : t(tile) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    wm = t.count <= 16 ? 1 : (t.count <= 32 ? 2 : 4), wn = kLoraWarps / wm;
+    m0 = 16 * (warp % wm), k = warp / wm, row = lane >> 2, c = lane & 3;
+    in0 = m0 + row < t.count, in1 = m0 + row + 8 < t.count;
+    t0 = in0 ? t.token(m0 + row) : 0, t1 = in1 ? t.token(m0 + row + 8) : 0;
+  }
+};
+
+// acc_s[m][r] = sum over this CTA's part of K (steps `part` of `parts`) of A[r, :] x[m, :], rows of 8 RN values (ranks beyond
+// the adapter's: zero); the warps' sums are added in their order.
 template <int RN>
-__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1)
-    lora_kernel(gptoss_lora_args g, LoraPlan p, bool direct) {
-  constexpr int KS = RN / 2;                        // steps of 16 ranks
-  constexpr int kAhead = RN <= 4 ? 4 : 3;
-  extern __shared__ __align__(16) float smem_f[];
-  float *acc_s = smem_f;                            // [8 warps][16][8 RN]
-  float *part_s = acc_s + kLoraWarps * 16 * 8 * RN; // [tokens][rank] of this CTA's part of K
-  float *u_s = part_s + kTileTokens * 8 * RN;       // [tokens][rank]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c = lane & 3;
-  const int tile = blockIdx.x / kClusterCtas, cta = blockIdx.x % kClusterCtas;
-  pdl_wait();
-  const Tile t = find_tile(g, p, direct, tile);
-  if (t.count == 0) {  // the whole cluster
-    pdl_launch_dependents();
-    return;
-  }
-  const int wm = t.count <= 16 ? 1 : (t.count <= 32 ? 2 : 4), wk = kLoraWarps / wm;
-  const int m0 = 16 * (warp % wm), kw = warp / wm;
-  const bool in0 = m0 + row < t.count, in1 = m0 + row + 8 < t.count;
-  const size_t t0 = in0 ? t.token(m0 + row) : 0, t1 = in1 ? t.token(m0 + row + 8) : 0;
-  const int n_per = ((g.n_out + 16 * kClusterCtas - 1) / (16 * kClusterCtas)) * 16;
-  const int n_end = min((cta + 1) * n_per, g.n_out), n_step = 16 * wk;
-  const float *y0 = g.y + t0 * g.y_stride + 4 * c, *y1 = g.y + t1 * g.y_stride + 4 * c;
-  float *o0 = g.out + t0 * g.out_stride + 4 * c, *o1 = g.out + t1 * g.out_stride + 4 * c;
-  const float4 none = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (t.adapter < 0) {  // tokens without an adapter
-    pdl_launch_dependents();
-    for (int n = cta * n_per + 16 * kw; n < n_end; n += n_step)
-      if (n + 4 * c < n_end) {
-        if (in0) *reinterpret_cast<float4 *>(o0 + n) = *reinterpret_cast<const float4 *>(y0 + n);
-        if (in1) *reinterpret_cast<float4 *>(o1 + n) = *reinterpret_cast<const float4 *>(y1 + n);
-      }
-    return;
-  }
-  {
-    const uint16_t *x = static_cast<const uint16_t *>(g.x), *a = static_cast<const uint16_t *>(g.a) + (size_t)t.adapter * g.rank * g.K;
-    const uint16_t *x0 = x + t0 * g.x_stride, *x1 = x + t1 * g.x_stride;
-    float acc[RN][4];
+__device__ __forceinline__ void partial_u(const gptoss_lora_args &g, const Work &k, int part, int parts, float *acc_s) {
+  const int warp = threadIdx.x >> 5, row = k.row, c = k.c;
+  const uint16_t *x = static_cast<const uint16_t *>(g.x), *a = static_cast<const uint16_t *>(g.a) + (size_t)k.t.adapter * g.rank * g.K;
+  const uint16_t *x0 = x + k.t0 * g.x_stride, *x1 = x + k.t1 * g.x_stride;
+  float acc[RN][4];
 #pragma unroll
-    for (int j = 0; j < RN; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-    const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-    for (int k = (cta * wk + kw) * kShrinkStep; k < g.K; k += kClusterCtas * wk * kShrinkStep) {
-      uint4 xa[2], xb[2];
+  for (int j = 0; j < RN; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  uint4 xa[2], xb[2];
+  auto load_x = [&](int at0) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {  // thread c of a row takes elements [8c, 8c + 8) of each 32
-        const int at = k + 32 * h + 8 * c;
-        xa[h] = at < g.K && in0 ? *reinterpret_cast<const uint4 *>(x0 + at) : zero;
-        xb[h] = at < g.K && in1 ? *reinterpret_cast<const uint4 *>(x1 + at) : zero;
-      }
-#pragma unroll
-      for (int j0 = 0; j0 < RN; j0 += 4) {
-        uint4 w[4][2];
-#pragma unroll
-        for (int j = j0; j < j0 + 4 && j < RN; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = k + 32 * h + 8 * c;
-            w[j - j0][h] = at < g.K && 8 * j + row < g.rank ? __ldg(reinterpret_cast<const uint4 *>(a + (size_t)(8 * j + row) * g.K + at)) : zero;
-          }
-#pragma unroll
-        for (int j = j0; j < j0 + 4 && j < RN; ++j)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            mma_16816(acc[j], xa[h].x, xb[h].x, xa[h].y, xb[h].y, w[j - j0][h].x, w[j - j0][h].y);
-            mma_16816(acc[j], xa[h].z, xb[h].z, xa[h].w, xb[h].w, w[j - j0][h].z, w[j - j0][h].w);
-          }
-      }
+    for (int h = 0; h < 2; ++h) {  // thread c of a row takes elements [8c, 8c + 8) of each 32
+      const int at = at0 + 32 * h + 8 * c;
+      xa[h] = at < g.K && k.in0 ? *reinterpret_cast<const uint4 *>(x0 + at) : zero;
+      xb[h] = at < g.K && k.in1 ? *reinterpret_cast<const uint4 *>(x1 + at) : zero;
     }
-    // accumulator of tile j: rows row, row + 8, ranks 8j + 2c, + 1
-    float *mine = acc_s + (size_t)warp * 16 * (8 * RN);
+  };
+  const int stride = parts * k.wn * kShrinkStep;
+  int at0 = (part * k.wn + k.k) * kShrinkStep;
+  load_x(at0);
+  for (; at0 < g.K; at0 += stride) {
+    const uint4 ca[2] = {xa[0], xa[1]}, cb[2] = {xb[0], xb[1]};
+    load_x(at0 + stride);
 #pragma unroll
-    for (int j = 0; j < RN; ++j) {
-      *reinterpret_cast<float2 *>(mine + row * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][0], acc[j][1]);
-      *reinterpret_cast<float2 *>(mine + (row + 8) * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][2], acc[j][3]);
+    for (int j0 = 0; j0 < RN; j0 += 4) {
+      uint4 w[4][2];
+#pragma unroll
+      for (int j = j0; j < j0 + 4 && j < RN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int at = at0 + 32 * h + 8 * c;
+          w[j - j0][h] = at < g.K && 8 * j + row < g.rank ? __ldg(reinterpret_cast<const uint4 *>(a + (size_t)(8 * j + row) * g.K + at)) : zero;
+        }
+#pragma unroll
+      for (int j = j0; j < j0 + 4 && j < RN; ++j)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_16816(acc[j], ca[h].x, cb[h].x, ca[h].y, cb[h].y, w[j - j0][h].x, w[j - j0][h].y);
+          mma_16816(acc[j], ca[h].z, cb[h].z, ca[h].w, cb[h].w, w[j - j0][h].z, w[j - j0][h].w);
+        }
     }
+  }
+  // accumulator of tile j: rows row, row + 8, ranks 8j + 2c, + 1
+  float *mine = acc_s + (size_t)warp * 16 * (8 * RN);
+#pragma unroll
+  for (int j = 0; j < RN; ++j) {
+    *reinterpret_cast<float2 *>(mine + row * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][0], acc[j][1]);
+    *reinterpret_cast<float2 *>(mine + (row + 8) * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][2], acc[j][3]);
   }
   __syncthreads();
-  const int n_u = t.count * g.rank;
-  for (int i = threadIdx.x; i < n_u; i += blockDim.x) {
-    const int m = i / g.rank, r = i - m * g.rank;
-    const float *part = acc_s + ((size_t)(m >> 4) * 16 + (m & 15)) * (8 * RN) + r;
-    float sum = 0.f;
-    for (int w = 0; w < wk; ++w) sum += part[(size_t)w * wm * 16 * (8 * RN)];
-    part_s[i] = sum;
+  float4 *sum4 = reinterpret_cast<float4 *>(acc_s);  // the sums take the place of the first warps' ones
+  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) {
+    float4 sum = sum4[i];
+    for (int w = 1; w < k.wn; ++w) {
+      const float4 v = sum4[i + w * k.wm * 32 * RN];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    sum4[i] = sum;
   }
-  cluster_arrive();
-  // what the second product reads besides u, requested while the partial sums meet
-  const float s = g.scale ? g.scale[t.adapter] : 1.f;
-  const uint16_t *bw = static_cast<const uint16_t *>(g.b) + (size_t)t.adapter * g.n_out * g.rank + 4 * c;
-  const int b_row = 4 * (row >> 1) + (row & 1);  // row of B for column `row` of the first product of 16 outputs
-  const int n_begin = cta * n_per + 16 * kw;
-  float4 ya[kAhead], yb[kAhead];
-  uint2 w[2][KS];
-  auto load_y = [&](int n, float4 &a, float4 &b) {
-    const bool in = n + 4 * c < n_end;
-    a = in && in0 ? *reinterpret_cast<const float4 *>(y0 + n) : none;
-    b = in && in1 ? *reinterpret_cast<const float4 *>(y1 + n) : none;
-  };
-  auto load_w = [&](int n, uint2 (&v)[2][KS]) {
+}
+
+// out = y + s B u for outputs [n_first, n_end) of a tile.  A warp takes 16 outputs a step: thread c of a row owns
+// [4c, 4c + 4) of them (column 2c + e of the j-th 8-wide product stands for output 4c + 2j + e), so that out moves 16 bytes
+// per thread, 64 per row.  y comes through a ring of 4 steps in shared memory (16 wn outputs of a row side by side), which
+// starts to fill before u is there.
+template <int RN>
+struct Expand {
+  static constexpr int KS = (RN + 3) / 4;  // steps of 32 ranks
+  const gptoss_lora_args &g;
+  const Work &k;
+  float *y_s;
+  int n_first, n_end, n_step;
+  const float *ysrc[2];  // this thread's two 16-byte pieces of every step of y
+  int ydst[2], ycol[2];
+  uint4 w[2][KS];        // thread c of a row takes ranks [8c, 8c + 8) of each 32
+  const uint16_t *bw;
+
+  __device__ __forceinline__ Expand(const gptoss_lora_args &args, const Work &work, float *ring, int first, int end)
+      : g(args), k(work), y_s(ring), n_first(first), n_end(end), n_step(16 * work.wn) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int q = threadIdx.x + 256 * i, per_row = n_step / 4, r = q / per_row;
+      ycol[i] = 4 * (q % per_row);
+      ydst[i] = r * (n_step + 16) + ycol[i];
+      ysrc[i] = r < k.t.count ? g.y + (size_t)k.t.token(r) * g.y_stride + ycol[i] : nullptr;
+    }
+    bw = static_cast<const uint16_t *>(g.b) + (size_t)k.t.adapter * g.n_out * g.rank + 8 * k.c;
+  }
+  __device__ __forceinline__ void fetch_y(int step) {
+    const int n = n_first + step * n_step;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if (ysrc[i] && n + ycol[i] < n_end) copy_async16(y_s + (step % kYStages) * kYStageFloats + ydst[i], ysrc[i] + n);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  __device__ __forceinline__ void fetch_w(int n) {
+    const int b_row = n + 4 * (k.row >> 1) + (k.row & 1);  // row of B for column `row` of the first product of 16 outputs
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int k = 0; k < KS; ++k)
-        v[j][k] = n + b_row + 2 * j < n_end && 16 * k + 4 * c < g.rank
-                      ? __ldg(reinterpret_cast<const uint2 *>(bw + (size_t)(n + b_row + 2 * j) * g.rank + 16 * k))
-                      : make_uint2(0u, 0u);
-  };
-#pragma unroll
-  for (int i = 0; i < kAhead; ++i) load_y(n_begin + i * n_step, ya[i], yb[i]);
-  load_w(n_begin, w);
-  cluster_wait();
-  // few values: every CTA adds up all of them; else each adds up an eighth and fetches the others'
-  const bool small = n_u <= kSmallU;
-  const int e_per = (n_u + kClusterCtas - 1) / kClusterCtas;
-  const uint32_t part_at = (uint32_t)__cvta_generic_to_shared(part_s), u_at = (uint32_t)__cvta_generic_to_shared(u_s);
-  for (int i = (small ? 0 : cta * e_per) + threadIdx.x; i < (small ? n_u : min(n_u, (cta + 1) * e_per)); i += blockDim.x) {
-    float sum = 0.f;
-#pragma unroll
-    for (int r = 0; r < kClusterCtas; ++r) sum += ld_cluster(part_at + 4 * i, r);
-    u_s[i] = sum;
+      for (int i = 0; i < KS; ++i)
+        w[j][i] = b_row + 2 * j < n_end && 32 * i + 8 * k.c < g.rank
+                      ? __ldg(reinterpret_cast<const uint4 *>(bw + (size_t)(b_row + 2 * j) * g.rank + 32 * i))
+                      : make_uint4(0u, 0u, 0u, 0u);
   }
-  if (!small) {
-    cluster_arrive();
-    cluster_wait();
-    for (int i = threadIdx.x; i < n_u; i += blockDim.x)
-      if (i / e_per != cta) u_s[i] = ld_cluster(u_at + 4 * i, i / e_per);
-  }
-  cluster_arrive();  // done with the others' memory
-  __syncthreads();
-  pdl_launch_dependents();
-  uint32_t u0[KS][2][3], u1[KS][2][3];  // rows row, row + 8: ranks 16k + 4c + {0,1}, {2,3}
+  __device__ __forceinline__ void start_y() {
 #pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    float4 a = none, b = none;
-    if (16 * k + 4 * c < g.rank) {
-      if (in0) a = *reinterpret_cast<const float4 *>(u_s + (m0 + row) * g.rank + 16 * k + 4 * c);
-      if (in1) b = *reinterpret_cast<const float4 *>(u_s + (m0 + row + 8) * g.rank + 16 * k + 4 * c);
-    }
-    three_terms(a.x, a.y, u0[k][0]), three_terms(a.z, a.w, u0[k][1]);
-    three_terms(b.x, b.y, u1[k][0]), three_terms(b.z, b.w, u1[k][1]);
+    for (int i = 0; i < kYStages - 1; ++i) fetch_y(i);
   }
-  for (int nb = n_begin; nb < n_end; nb += kAhead * n_step) {
+  // u_s: [tokens][8 RN], visible to the whole CTA; the first of B has been fetched
+  __device__ __forceinline__ void run(const float *u_s) {
+    uint32_t u0[KS][4][3], u1[KS][4][3];  // rows row, row + 8: rank pairs 32i + 8c + {0,1}, {2,3}, {4,5}, {6,7}
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      const int n = nb + i * n_step;
-      if (n >= n_end) break;
+    for (int i = 0; i < KS; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+        const float *u = u_s + (k.m0 + k.row) * (8 * RN) + 32 * i + 8 * k.c + 4 * h;
+        if (32 * i + 8 * k.c < g.rank) {
+          if (k.in0) a = *reinterpret_cast<const float4 *>(u);
+          if (k.in1) b = *reinterpret_cast<const float4 *>(u + 8 * (8 * RN));
+        }
+        three_terms(a.x, a.y, u0[i][2 * h]), three_terms(a.z, a.w, u0[i][2 * h + 1]);
+        three_terms(b.x, b.y, u1[i][2 * h]), three_terms(b.z, b.w, u1[i][2 * h + 1]);
+      }
+    const float s = g.scale ? g.scale[k.t.adapter] : 1.f;
+    float *o0 = g.out + k.t0 * g.out_stride + 4 * k.c, *o1 = g.out + k.t1 * g.out_stride + 4 * k.c;
+    int step = 0;
+    for (int nb = n_first; nb < n_end; nb += n_step, ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kYStages - 2) : "memory");
+      __syncthreads();  // this step's y is there, and everybody has left the step whose place the next copy takes
+      fetch_y(step + kYStages - 1);
+      const int n = nb + 16 * k.k;
       float acc[2][4];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
@@ -295,24 +313,144 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 #pragma unroll
         for (int term = 2; term >= 0; --term)  // the smallest terms first
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-            mma_16816(acc[j], u0[k][0][term], u1[k][0][term], u0[k][1][term], u1[k][1][term], w[j][k].x, w[j][k].y);
+          for (int i = 0; i < KS; ++i) {
+            mma_16816(acc[j], u0[i][0][term], u1[i][0][term], u0[i][1][term], u1[i][1][term], w[j][i].x, w[j][i].y);
+            mma_16816(acc[j], u0[i][2][term], u1[i][2][term], u0[i][3][term], u1[i][3][term], w[j][i].z, w[j][i].w);
+          }
       }
-      load_w(n + n_step, w);
-      const float4 a = ya[i], b = yb[i];
-      load_y(n + kAhead * n_step, ya[i], yb[i]);
-      if (n + 4 * c < n_end) {
-        if (in0)
+      fetch_w(n + n_step);
+      if (n + 4 * k.c < n_end) {
+        const float *y = y_s + (step % kYStages) * kYStageFloats + (k.m0 + k.row) * (n_step + 16) + 16 * k.k + 4 * k.c;
+        if (k.in0) {
+          const float4 a = *reinterpret_cast<const float4 *>(y);
           *reinterpret_cast<float4 *>(o0 + n) =
               make_float4(fmaf(s, acc[0][0], a.x), fmaf(s, acc[0][1], a.y), fmaf(s, acc[1][0], a.z), fmaf(s, acc[1][1], a.w));
-        if (in1)
+        }
+        if (k.in1) {
+          const float4 b = *reinterpret_cast<const float4 *>(y + 8 * (n_step + 16));
           *reinterpret_cast<float4 *>(o1 + n) =
               make_float4(fmaf(s, acc[0][2], b.x), fmaf(s, acc[0][3], b.y), fmaf(s, acc[1][2], b.z), fmaf(s, acc[1][3], b.w));
+        }
       }
     }
   }
+};
+
+// Outputs of part `part` of `parts` of a tile.
+__device__ __forceinline__ void output_range(int n_out, int part, int parts, int &first, int &end) {
+  const int per = (n_out + 16 * parts - 1) / (16 * parts) * 16;
+  first = part * per, end = min(first + per, n_out);
+}
+// Tokens without an adapter: out = y.
+__device__ __forceinline__ void copy_rows(const gptoss_lora_args &g, const Work &k, int first, int end) {
+  for (int n = first + 16 * k.k + 4 * k.c; n < end; n += 16 * k.wn) {
+    if (k.in0) *reinterpret_cast<float4 *>(g.out + k.t0 * g.out_stride + n) = *reinterpret_cast<const float4 *>(g.y + k.t0 * g.y_stride + n);
+    if (k.in1) *reinterpret_cast<float4 *>(g.out + k.t1 * g.out_stride + n) = *reinterpret_cast<const float4 *>(g.y + k.t1 * g.y_stride + n);
+  }
+}
+
+// Few tiles: a cluster of 8 CTAs per tile does it all.  Each computes u over an eighth of K, the cluster's sums are added
+// in the order of the CTAs, each CTA then takes an eighth of the outputs.  RN: tiles of 8 ranks, at least rank / 8.
+template <int RN>
+__global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1)
+    lora_kernel(gptoss_lora_args g, LoraPlan p, bool direct) {
+  extern __shared__ __align__(16) float smem_f[];
+  float *acc_s = smem_f;                          // [8 warps][16][8 RN], of which the first [tokens][8 RN] become the sums
+  float *u_s = acc_s + kTileTokens * 8 * RN;      // u, where the last warps' sums were
+  float *y_s = acc_s + kLoraWarps * 16 * 8 * RN;  // ring
+  const int cta = blockIdx.x % kClusterCtas;
+  pdl_wait();
+  const Work k(find_tile(g, p, direct, blockIdx.x / kClusterCtas));
+  int n_first, n_end;
+  output_range(g.n_out, cta, kClusterCtas, n_first, n_end);
+  if (k.t.count == 0 || k.t.adapter < 0) {  // the whole cluster
+    pdl_launch_dependents();
+    copy_rows(g, k, n_first, n_end);
+    return;
+  }
+  Expand<RN> expand(g, k, y_s, n_first, n_end);
+  expand.start_y();
+  partial_u<RN>(g, k, cta, kClusterCtas, acc_s);
+  cluster_arrive();
+  expand.fetch_w(n_first + 16 * k.k);  // while the partial sums meet
+  cluster_wait();
+  // few values: every CTA adds up all of them; else each adds up an eighth and fetches the others'
+  const int n_u = k.t.count * 2 * RN, e_per = (n_u + kClusterCtas - 1) / kClusterCtas;  // in pieces of 4 values
+  const bool small = n_u <= kSmallU;
+  float4 *u4 = reinterpret_cast<float4 *>(u_s);
+  const uint32_t part_at = (uint32_t)__cvta_generic_to_shared(acc_s), u_at = (uint32_t)__cvta_generic_to_shared(u_s);
+  for (int i = (small ? 0 : cta * e_per) + threadIdx.x; i < (small ? n_u : min(n_u, (cta + 1) * e_per)); i += blockDim.x) {
+    float4 v[kClusterCtas];
+#pragma unroll
+    for (int r = 0; r < kClusterCtas; ++r) v[r] = ld_cluster(part_at + 16 * i, r);
+    float4 sum = v[0];
+#pragma unroll
+    for (int r = 1; r < kClusterCtas; ++r) sum.x += v[r].x, sum.y += v[r].y, sum.z += v[r].z, sum.w += v[r].w;
+    u4[i] = sum;
+  }
+  if (!small) {
+    cluster_arrive();
+    cluster_wait();
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n_u; i += blockDim.x) {
+      const int owner = i / e_per;
+      if (owner != cta) u4[i] = ld_cluster(u_at + 16 * i, owner);
+    }
+  }
+  cluster_arrive();  // done with the others' memory
+  __syncthreads();
+  pdl_launch_dependents();
+  expand.run(u_s);
   cluster_wait();  // nobody reads this CTA's memory any more
 }
+
+// Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
+// do not need: they fill the GPU without splitting a tile's K by more than kWideSplits.
+template <int RN>
+__global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_kernel(gptoss_lora_args g, LoraPlan p) {
+  extern __shared__ __align__(16) float smem_f[];
+  pdl_wait();
+  pdl_launch_dependents();
+  const Work k(find_tile(g, p, false, blockIdx.x / kWideSplits));
+  if (k.t.count == 0 || k.t.adapter < 0) return;
+  const int part = blockIdx.x % kWideSplits;
+  partial_u<RN>(g, k, part, kWideSplits, smem_f);
+  __syncthreads();
+  // u by position in the sorted order: a tile's rows side by side
+  float4 *u = reinterpret_cast<float4 *>(p.u) + ((size_t)part * g.T + (k.t.perm - p.perm)) * (2 * RN);
+  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) u[i] = reinterpret_cast<const float4 *>(smem_f)[i];
+}
+template <int RN>
+__global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_expand_kernel(gptoss_lora_args g, LoraPlan p, int parts) {
+  extern __shared__ __align__(16) float smem_f[];
+  float *u_s = smem_f, *y_s = u_s + kTileTokens * 8 * RN;
+  pdl_wait();
+  pdl_launch_dependents();
+  const Work k(find_tile(g, p, false, blockIdx.x / parts));
+  int n_first, n_end;
+  output_range(g.n_out, blockIdx.x % parts, parts, n_first, n_end);
+  if (k.t.count == 0 || k.t.adapter < 0) {
+    copy_rows(g, k, n_first, n_end);
+    return;
+  }
+  Expand<RN> expand(g, k, y_s, n_first, n_end);
+  expand.start_y();
+  expand.fetch_w(n_first + 16 * k.k);
+  const float4 *u = reinterpret_cast<const float4 *>(p.u) + (size_t)(k.t.perm - p.perm) * (2 * RN);
+  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) {
+    float4 sum = u[i];
+#pragma unroll
+    for (int part = 1; part < kWideSplits; ++part) {
+      const float4 v = u[(size_t)part * g.T * (2 * RN) + i];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    reinterpret_cast<float4 *>(u_s)[i] = sum;
+  }
+  __syncthreads();
+  expand.run(u_s);
+}
+
+int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
 
 // Parts of a call's workspace.
 LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
@@ -334,17 +472,32 @@ LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
   p.tiles = reinterpret_cast<int4 *>(take((uint64_t)p.max_tiles * sizeof(int4)));
   p.perm = reinterpret_cast<int *>(take((uint64_t)g.T * sizeof(int)));
   p.n_tiles = reinterpret_cast<int *>(take(sizeof(int)));
+  p.wide = g.T >= kWideTokens;
+  if (p.wide) p.u = reinterpret_cast<float *>(take((uint64_t)kWideSplits * g.T * padded_rank(g.rank) * sizeof(float)));
   return p;
 }
 
+template <typename K>
+cudaError_t allow_smem(K kernel, int bytes) {
+  return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
+}
 template <int RN>
 cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, bool direct, cudaStream_t s) {
-  constexpr int smem = (kLoraWarps * 16 + 2 * kTileTokens) * 8 * RN * (int)sizeof(float);
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(lora_kernel<RN>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
+  constexpr int acc = kLoraWarps * 16 * 8 * RN * (int)sizeof(float), ring = kYStages * kYStageFloats * (int)sizeof(float);
+  const dim3 block(32 * kLoraWarps);
+  cudaError_t e;
+  if (!p.wide) {
+    if ((e = allow_smem(lora_kernel<RN>, acc + ring)) != cudaSuccess) return e;
+    return launch_chain(lora_kernel<RN>, dim3(p.max_tiles * kClusterCtas), block, acc + ring, s, g, p, direct);
   }
-  return launch_chain(lora_kernel<RN>, dim3(p.max_tiles * kClusterCtas), dim3(32 * kLoraWarps), smem, s, g, p, direct);
+  constexpr int expand = kTileTokens * 8 * RN * (int)sizeof(float) + ring;
+  if ((e = allow_smem(lora_shrink_kernel<RN>, acc)) != cudaSuccess || (e = allow_smem(lora_expand_kernel<RN>, expand)) != cudaSuccess) return e;
+  if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * kWideSplits), block, acc, s, g, p)) != cudaSuccess) return e;
+  // parts of the outputs: some 4 CTAs per slot of the GPU, but at least 256 outputs each
+  const int tiles = g.T / kTileTokens;
+  int parts = (4 * 2 * kSmCountFallback + tiles - 1) / tiles;
+  parts = parts > (g.n_out + 255) / 256 ? (g.n_out + 255) / 256 : parts;
+  return launch_chain(lora_expand_kernel<RN>, dim3(p.max_tiles * parts), block, expand, s, g, p, parts);
 }
 
 }  // namespace
