@@ -45,6 +45,13 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// bin of token t: its adapter, n for a token without one, -1 behind the last token
+__device__ __forceinline__ int bin_of(const int *__restrict__ ids, int t, int T, int n) {
+  if (t >= T) return -1;
+  const int id = ids[t];
+  return id >= 0 && id < n ? id : n;
+}
+
 // One block.  Bins 0..n-1 are the adapters, bin n the tokens without one.
 __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__ ids, int T, int n, LoraPlan p) {
   extern __shared__ int bin_s[];  // [n + 1] counts, then cursors
@@ -54,11 +61,17 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
-  // neighbours often share an adapter: one atomic per adapter and warp
-  for (int t0 = 0; t0 < T; t0 += 1024) {
-    const int t = t0 + tid, id = t < T ? ids[t] : 0, bin = t < T ? (id >= 0 && id < n ? id : n) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, bin);
-    if (bin >= 0 && lane == __ffs(same) - 1) atomicAdd(&bin_s[bin], __popc(same));
+  // neighbours often share an adapter: one atomic per adapter and warp.  Eight loads are under way at a time.
+  for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
+    int bin[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bin[i] = bin_of(ids, t0 + 1024 * i + tid, T, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (t0 + 1024 * i >= T) break;
+      const uint32_t same = __match_any_sync(0xffffffffu, bin[i]);
+      if (bin[i] >= 0 && lane == __ffs(same) - 1) atomicAdd(&bin_s[bin[i]], __popc(same));
+    }
   }
   __syncthreads();
   // exclusive prefix of the counts (positions) and of the tile counts; a thread owns `per` consecutive bins
@@ -89,14 +102,20 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   }
   __syncthreads();
   // where a token stands among those of its adapter varies from run to run; its result does not depend on it
-  for (int t0 = 0; t0 < T; t0 += 1024) {
-    const int t = t0 + tid, id = t < T ? ids[t] : 0, bin = t < T ? (id >= 0 && id < n ? id : n) : -1;
-    const uint32_t same = __match_any_sync(0xffffffffu, bin);
-    const int leader = __ffs(same) - 1;
-    int at = 0;
-    if (bin >= 0 && lane == leader) at = atomicAdd(&bin_s[bin], __popc(same));
-    at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
-    if (bin >= 0) p.perm[at] = t;
+  for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
+    int bin[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) bin[i] = bin_of(ids, t0 + 1024 * i + tid, T, n);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (t0 + 1024 * i >= T) break;
+      const uint32_t same = __match_any_sync(0xffffffffu, bin[i]);
+      const int leader = __ffs(same) - 1;
+      int at = 0;
+      if (bin[i] >= 0 && lane == leader) at = atomicAdd(&bin_s[bin[i]], __popc(same));
+      at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
+      if (bin[i] >= 0) p.perm[at] = t0 + 1024 * i + tid;
+    }
   }
 }
 
@@ -147,12 +166,9 @@ __device__ __forceinline__ float4 ld_cluster(uint32_t addr, uint32_t rank) {
   return v;
 }
 
-__device__ __forceinline__ void copy_async16(void *dst_shared, const void *src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst_shared)), "l"(src) : "memory");
+__device__ __forceinline__ void copy_async16(uint32_t dst_shared, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst_shared), "l"(src) : "memory");
 }
-
-constexpr int kYStages = 4;
-constexpr int kYStageFloats = 3072;  // 16 wm rows of 16 wn + 16 floats (the padding keeps 16-byte reads of 2 rows apart)
 
 // A CTA's view of its tile.  Its 8 warps stand `wm` across the tile's 16-row blocks and wn = 8 / wm along the other index.
 struct Work {
@@ -238,34 +254,69 @@ __device__ __forceinline__ void partial_u(const gptoss_lora_args &g, const Work 
 // [4c, 4c + 4) of them (column 2c + e of the j-th 8-wide product stands for output 4c + 2j + e), so that out moves 16 bytes
 // per thread, 64 per row.  y comes through a ring of 4 steps in shared memory (16 wn outputs of a row side by side), which
 // starts to fill before u is there.
-template <int RN>
+// With BRING (the wide kernel, tiles of more than 32 tokens) the rows of B come through shared memory too: four warps
+// read the same ones, and one step's notice is too short for their way from L2.
+template <int RN, bool BRING>
 struct Expand {
   static constexpr int KS = (RN + 3) / 4;  // steps of 32 ranks
+  static constexpr int kBStride = RN <= 4 ? 64 : 16 * RN + 64;  // bytes from row to row: 16-byte reads of two rows stay apart
+  // a warp's blocks of 16 outputs per step: with two, the wide kernel asks for 256 bytes of each row of y at a time
+  static constexpr int BL = BRING ? 2 : 1;
+  static constexpr int kYStages = BRING ? 3 : 4;
+  // 16 wm rows of 16 wn BL + 16 floats (the padding keeps 16-byte reads of 2 rows apart); the wide kernel has wm = 4
+  static constexpr int kYStageFloats = BRING ? 64 * 80 : 3072;
+  static constexpr int kBStageBytes = 32 * BL * kBStride;
+  static constexpr int kRingBytes = kYStages * (4 * kYStageFloats + (BRING ? kBStageBytes : 0));
+  static constexpr int YP = 2 * BL;  // 16-byte pieces of a step's y per thread
+  static constexpr int kBPieces = (32 * BL * RN + 32 * kLoraWarps - 1) / (32 * kLoraWarps);  // of a step's B, per thread
   const gptoss_lora_args &g;
   const Work &k;
   float *y_s;
   int n_first, n_end, n_step;
-  const float *ysrc[2];  // this thread's two 16-byte pieces of every step of y
-  int ydst[2], ycol[2];
+  // this thread's pieces of the next step to be copied: where from, where to, and how many outputs are left (0: none)
+  const float *ysrc[YP];
+  uint32_t ydst[YP], bdst[kBPieces];
+  int yleft[YP], bleft[kBPieces];
+  const uint16_t *bsrc[kBPieces];
   uint4 w[2][KS];        // thread c of a row takes ranks [8c, 8c + 8) of each 32
   const uint16_t *bw;
 
   __device__ __forceinline__ Expand(const gptoss_lora_args &args, const Work &work, float *ring, int first, int end)
-      : g(args), k(work), y_s(ring), n_first(first), n_end(end), n_step(16 * work.wn) {
+      : g(args), k(work), y_s(ring), n_first(first), n_end(end), n_step(16 * BL * work.wn) {
+    const uint32_t y_at = (uint32_t)__cvta_generic_to_shared(y_s);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = threadIdx.x + 256 * i, per_row = n_step / 4, r = q / per_row;
-      ycol[i] = 4 * (q % per_row);
-      ydst[i] = r * (n_step + 16) + ycol[i];
-      ysrc[i] = r < k.t.count ? g.y + (size_t)k.t.token(r) * g.y_stride + ycol[i] : nullptr;
+    for (int i = 0; i < YP; ++i) {
+      const int q = threadIdx.x + 256 * i, per_row = n_step / 4, r = q / per_row, col = 4 * (q - r * per_row);
+      ydst[i] = y_at + 4 * (r * (n_step + 16) + col);
+      yleft[i] = r < k.t.count ? n_end - n_first - col : 0;
+      ysrc[i] = g.y + (r < k.t.count ? (size_t)k.t.token(r) * g.y_stride : 0) + n_first + col;
     }
-    bw = static_cast<const uint16_t *>(g.b) + (size_t)k.t.adapter * g.n_out * g.rank + 8 * k.c;
-  }
-  __device__ __forceinline__ void fetch_y(int step) {
-    const int n = n_first + step * n_step;
+    const uint16_t *b = static_cast<const uint16_t *>(g.b) + (size_t)k.t.adapter * g.n_out * g.rank;
+    bw = b + 8 * k.c;
+    if (BRING) {  // 32 BL rows of rank / 8 pieces a step
+      const int per_row = g.rank / 8;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (ysrc[i] && n + ycol[i] < n_end) copy_async16(y_s + (step % kYStages) * kYStageFloats + ydst[i], ysrc[i] + n);
+      for (int i = 0; i < kBPieces; ++i) {
+        const int q = threadIdx.x + 32 * kLoraWarps * i, r = q / per_row, piece = q - r * per_row;
+        bdst[i] = y_at + 4 * kYStages * kYStageFloats + r * kBStride + 16 * piece;
+        bleft[i] = r < 32 * BL ? n_end - n_first - r : 0;
+        bsrc[i] = b + (size_t)(n_first + min(r, 32 * BL - 1)) * g.rank + 8 * piece;
+      }
+    }
+  }
+  __device__ __forceinline__ void fetch(int stage) {
+#pragma unroll
+    for (int i = 0; i < YP; ++i) {
+      if (yleft[i] > 0) copy_async16(ydst[i] + stage * 4 * kYStageFloats, ysrc[i]);
+      ysrc[i] += n_step, yleft[i] -= n_step;
+    }
+    if (BRING) {
+#pragma unroll
+      for (int i = 0; i < kBPieces; ++i) {
+        if (bleft[i] > 0) copy_async16(bdst[i] + stage * kBStageBytes, bsrc[i]);
+        bsrc[i] += 32 * BL * g.rank, bleft[i] -= 32 * BL;
+      }
+    }
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   __device__ __forceinline__ void fetch_w(int n) {
@@ -278,9 +329,9 @@ struct Expand {
                       ? __ldg(reinterpret_cast<const uint4 *>(bw + (size_t)(b_row + 2 * j) * g.rank + 32 * i))
                       : make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ void start_y() {
+  __device__ __forceinline__ void start() {
 #pragma unroll
-    for (int i = 0; i < kYStages - 1; ++i) fetch_y(i);
+    for (int i = 0; i < kYStages - 1; ++i) fetch(i);
   }
   // u_s: [tokens][8 RN], visible to the whole CTA; the first of B has been fetched
   __device__ __forceinline__ void run(const float *u_s) {
@@ -299,38 +350,67 @@ struct Expand {
         three_terms(b.x, b.y, u1[i][2 * h]), three_terms(b.z, b.w, u1[i][2 * h + 1]);
       }
     const float s = g.scale ? g.scale[k.t.adapter] : 1.f;
-    float *o0 = g.out + k.t0 * g.out_stride + 4 * k.c, *o1 = g.out + k.t1 * g.out_stride + 4 * k.c;
-    int step = 0;
-    for (int nb = n_first; nb < n_end; nb += n_step, ++step) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(kYStages - 2) : "memory");
-      __syncthreads();  // this step's y is there, and everybody has left the step whose place the next copy takes
-      fetch_y(step + kYStages - 1);
-      const int n = nb + 16 * k.k;
-      float acc[2][4];
+    int n = n_first + 16 * BL * k.k, left = n_end - n - 4 * k.c;  // this thread's outputs of the step; outputs left from there on
+    float *o0 = g.out + k.t0 * g.out_stride + n + 4 * k.c, *o1 = g.out + k.t1 * g.out_stride + n + 4 * k.c;
+    const float *y = y_s + (k.m0 + k.row) * (n_step + 16) + 16 * BL * k.k + 4 * k.c;
+    const uint8_t *b_s = reinterpret_cast<const uint8_t *>(y_s + kYStages * kYStageFloats) +
+                         (16 * BL * k.k + 4 * (k.row >> 1) + (k.row & 1)) * kBStride + 16 * k.c;
+    const int steps = (n_end - n_first + n_step - 1) / n_step;
+    for (int step0 = 0; step0 < steps; step0 += kYStages) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+      for (int stage = 0; stage < kYStages; ++stage) {
+        if (step0 + stage >= steps) break;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kYStages - 2) : "memory");
+        __syncthreads();  // this step's y is there, and everybody has left the step whose place the next copy takes
+        fetch((stage + kYStages - 1) % kYStages);
+        n += n_step;
 #pragma unroll
-        for (int term = 2; term >= 0; --term)  // the smallest terms first
+        for (int bl = 0; bl < BL; ++bl) {
+          if (BRING) {
 #pragma unroll
-          for (int i = 0; i < KS; ++i) {
-            mma_16816(acc[j], u0[i][0][term], u1[i][0][term], u0[i][1][term], u1[i][1][term], w[j][i].x, w[j][i].y);
-            mma_16816(acc[j], u0[i][2][term], u1[i][2][term], u0[i][3][term], u1[i][3][term], w[j][i].z, w[j][i].w);
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int i = 0; i < KS; ++i)
+                w[j][i] = 32 * i + 8 * k.c < g.rank
+                              ? *reinterpret_cast<const uint4 *>(b_s + stage * kBStageBytes + (16 * bl + 2 * j) * kBStride + 64 * i)
+                              : make_uint4(0u, 0u, 0u, 0u);
           }
-      }
-      fetch_w(n + n_step);
-      if (n + 4 * k.c < n_end) {
-        const float *y = y_s + (step % kYStages) * kYStageFloats + (k.m0 + k.row) * (n_step + 16) + 16 * k.k + 4 * k.c;
-        if (k.in0) {
-          const float4 a = *reinterpret_cast<const float4 *>(y);
-          *reinterpret_cast<float4 *>(o0 + n) =
-              make_float4(fmaf(s, acc[0][0], a.x), fmaf(s, acc[0][1], a.y), fmaf(s, acc[1][0], a.z), fmaf(s, acc[1][1], a.w));
+          // a sum per term of u: the products of one sum wait for each other
+          float part[3][2][4], acc[2][4];
+#pragma unroll
+          for (int term = 0; term < 3; ++term)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) part[term][j][0] = part[term][j][1] = part[term][j][2] = part[term][j][3] = 0.f;
+#pragma unroll
+          for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int term = 0; term < 3; ++term)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  mma_16816(part[term][j], u0[i][2 * h][term], u1[i][2 * h][term], u0[i][2 * h + 1][term], u1[i][2 * h + 1][term],
+                            h ? w[j][i].z : w[j][i].x, h ? w[j][i].w : w[j][i].y);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[j][e] = (part[2][j][e] + part[1][j][e]) + part[0][j][e];
+          if (!BRING) fetch_w(n);
+          if (left > 16 * bl) {
+            const float *yb = y + stage * kYStageFloats + 16 * bl;
+            if (k.in0) {
+              const float4 a = *reinterpret_cast<const float4 *>(yb);
+              *reinterpret_cast<float4 *>(o0 + 16 * bl) =
+                  make_float4(fmaf(s, acc[0][0], a.x), fmaf(s, acc[0][1], a.y), fmaf(s, acc[1][0], a.z), fmaf(s, acc[1][1], a.w));
+            }
+            if (k.in1) {
+              const float4 b = *reinterpret_cast<const float4 *>(yb + 8 * (n_step + 16));
+              *reinterpret_cast<float4 *>(o1 + 16 * bl) =
+                  make_float4(fmaf(s, acc[0][2], b.x), fmaf(s, acc[0][3], b.y), fmaf(s, acc[1][2], b.z), fmaf(s, acc[1][3], b.w));
+            }
+          }
         }
-        if (k.in1) {
-          const float4 b = *reinterpret_cast<const float4 *>(y + 8 * (n_step + 16));
-          *reinterpret_cast<float4 *>(o1 + n) =
-              make_float4(fmaf(s, acc[0][2], b.x), fmaf(s, acc[0][3], b.y), fmaf(s, acc[1][2], b.z), fmaf(s, acc[1][3], b.w));
-        }
+        o0 += n_step, o1 += n_step, left -= n_step;
       }
     }
   }
@@ -368,8 +448,8 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
     copy_rows(g, k, n_first, n_end);
     return;
   }
-  Expand<RN> expand(g, k, y_s, n_first, n_end);
-  expand.start_y();
+  Expand<RN, false> expand(g, k, y_s, n_first, n_end);
+  expand.start();
   partial_u<RN>(g, k, cta, kClusterCtas, acc_s);
   cluster_arrive();
   expand.fetch_w(n_first + 16 * k.k);  // while the partial sums meet
@@ -406,19 +486,102 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 
 // Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
 // do not need: they fill the GPU without splitting a tile's K by more than kWideSplits.
+// Shrink: a CTA takes 64 tokens and a part of K, x and A come through a ring of 64-element steps in shared memory; the warps are 4
+// across the rows and 2 across the ranks, so no sums have to be joined.
+template <int RN>
+struct ShrinkRing {
+  static constexpr int kStages = RN <= 8 ? 4 : 3;
+  static constexpr int kStride = 192;  // bytes from row to row: 128 and padding that keeps 16-byte reads of two rows apart
+  static constexpr int kStageBytes = (kTileTokens + 8 * RN) * kStride;
+};
+__device__ __forceinline__ void copy_async16_or_zero(void *dst_shared, const void *src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst_shared)), "l"(src), "r"(in ? 16 : 0)
+               : "memory");
+}
 template <int RN>
 __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_kernel(gptoss_lora_args g, LoraPlan p) {
-  extern __shared__ __align__(16) float smem_f[];
+  using Ring = ShrinkRing<RN>;
+  constexpr int NJ = RN / 2;  // rank tiles of a warp
+  extern __shared__ __align__(16) uint8_t smem_b[];
   pdl_wait();
   pdl_launch_dependents();
-  const Work k(find_tile(g, p, false, blockIdx.x / kWideSplits));
-  if (k.t.count == 0 || k.t.adapter < 0) return;
+  const Tile t = find_tile(g, p, false, blockIdx.x / kWideSplits);
+  if (t.count == 0 || t.adapter < 0) return;
   const int part = blockIdx.x % kWideSplits;
-  partial_u<RN>(g, k, part, kWideSplits, smem_f);
+  const int steps_all = (g.K + kShrinkStep - 1) / kShrinkStep, per = (steps_all + kWideSplits - 1) / kWideSplits;
+  const int first = part * per, steps = min(per, steps_all - first);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c = lane & 3;
+  const int piece = threadIdx.x & 7, r0 = threadIdx.x >> 3;  // this thread's 16-byte piece of rows r0, r0 + 32, ...
+  const uint16_t *xsrc[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    xsrc[i] = r0 + 32 * i < t.count ? static_cast<const uint16_t *>(g.x) + (size_t)t.token(r0 + 32 * i) * g.x_stride + 8 * piece : nullptr;
+  const uint16_t *asrc = static_cast<const uint16_t *>(g.a) + ((size_t)t.adapter * g.rank + r0) * g.K + 8 * piece;
+  auto fetch = [&](int step) {
+    if (step < steps) {
+      uint8_t *ring = smem_b + (step % Ring::kStages) * Ring::kStageBytes + 16 * piece;
+      const int k = (first + step) * kShrinkStep;
+      const bool in = k + 8 * piece < g.K;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (xsrc[i]) copy_async16_or_zero(ring + (r0 + 32 * i) * Ring::kStride, in ? xsrc[i] + k : xsrc[i], in);
+#pragma unroll
+      for (int i = 0; i < (8 * RN + 31) / 32; ++i)
+        if (r0 + 32 * i < g.rank)
+          copy_async16_or_zero(ring + (kTileTokens + r0 + 32 * i) * Ring::kStride, in ? asrc + (size_t)32 * i * g.K + k : asrc, in);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < Ring::kStages - 1; ++i) fetch(i);
+  const int m0 = 16 * (warp & 3), j0 = NJ * (warp >> 2);
+  float acc[NJ][4];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  for (int step = 0; step < steps; ++step) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(Ring::kStages - 2) : "memory");
+    __syncthreads();
+    fetch(step + Ring::kStages - 1);
+    const uint8_t *ring = smem_b + (step % Ring::kStages) * Ring::kStageBytes + 16 * c;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint4 xa = *reinterpret_cast<const uint4 *>(ring + (m0 + row) * Ring::kStride + 64 * h);
+      const uint4 xb = *reinterpret_cast<const uint4 *>(ring + (m0 + row + 8) * Ring::kStride + 64 * h);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint4 w = *reinterpret_cast<const uint4 *>(ring + (kTileTokens + 8 * (j0 + j) + row) * Ring::kStride + 64 * h);
+        mma_16816(acc[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+        mma_16816(acc[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+      }
+    }
+  }
+  // u by position in the sorted order; what stands beyond the tile's tokens and the adapter's ranks is not read
+  float *u = p.u + ((size_t)part * g.T + (t.perm - p.perm) + m0 + row) * (8 * RN) + 8 * j0 + 2 * c;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    if (m0 + row < t.count) *reinterpret_cast<float2 *>(u + 8 * j) = make_float2(acc[j][0], acc[j][1]);
+    if (m0 + row + 8 < t.count) *reinterpret_cast<float2 *>(u + 8 * (8 * RN) + 8 * j) = make_float2(acc[j][2], acc[j][3]);
+  }
+}
+template <int RN, bool BRING>
+__device__ __forceinline__ void wide_expand(const gptoss_lora_args &g, const LoraPlan &p, const Work &k, float *u_s, float *y_s, int n_first,
+                                            int n_end) {
+  Expand<RN, BRING> expand(g, k, y_s, n_first, n_end);
+  expand.start();
+  if (!BRING) expand.fetch_w(n_first + 16 * k.k);
+  const float4 *u = reinterpret_cast<const float4 *>(p.u) + (size_t)(k.t.perm - p.perm) * (2 * RN);
+#pragma unroll 2
+  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += 32 * kLoraWarps) {
+    float4 sum = u[i];
+#pragma unroll
+    for (int part = 1; part < kWideSplits; ++part) {
+      const float4 v = u[(size_t)part * g.T * (2 * RN) + i];
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    reinterpret_cast<float4 *>(u_s)[i] = sum;
+  }
   __syncthreads();
-  // u by position in the sorted order: a tile's rows side by side
-  float4 *u = reinterpret_cast<float4 *>(p.u) + ((size_t)part * g.T + (k.t.perm - p.perm)) * (2 * RN);
-  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) u[i] = reinterpret_cast<const float4 *>(smem_f)[i];
+  expand.run(u_s);
 }
 template <int RN>
 __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_expand_kernel(gptoss_lora_args g, LoraPlan p, int parts) {
@@ -431,23 +594,11 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_expand_
   output_range(g.n_out, blockIdx.x % parts, parts, n_first, n_end);
   if (k.t.count == 0 || k.t.adapter < 0) {
     copy_rows(g, k, n_first, n_end);
-    return;
+  } else if (k.wm == 4) {
+    wide_expand<RN, true>(g, p, k, u_s, y_s, n_first, n_end);
+  } else {
+    wide_expand<RN, false>(g, p, k, u_s, y_s, n_first, n_end);
   }
-  Expand<RN> expand(g, k, y_s, n_first, n_end);
-  expand.start_y();
-  expand.fetch_w(n_first + 16 * k.k);
-  const float4 *u = reinterpret_cast<const float4 *>(p.u) + (size_t)(k.t.perm - p.perm) * (2 * RN);
-  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) {
-    float4 sum = u[i];
-#pragma unroll
-    for (int part = 1; part < kWideSplits; ++part) {
-      const float4 v = u[(size_t)part * g.T * (2 * RN) + i];
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
-    reinterpret_cast<float4 *>(u_s)[i] = sum;
-  }
-  __syncthreads();
-  expand.run(u_s);
 }
 
 int padded_rank(int rank) { return rank <= 16 ? 16 : (rank <= 32 ? 32 : (rank <= 64 ? 64 : 128)); }
@@ -483,19 +634,23 @@ cudaError_t allow_smem(K kernel, int bytes) {
 }
 template <int RN>
 cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, bool direct, cudaStream_t s) {
-  constexpr int acc = kLoraWarps * 16 * 8 * RN * (int)sizeof(float), ring = kYStages * kYStageFloats * (int)sizeof(float);
+  constexpr int acc = kLoraWarps * 16 * 8 * RN * (int)sizeof(float), ring = Expand<RN, false>::kRingBytes;
   const dim3 block(32 * kLoraWarps);
   cudaError_t e;
   if (!p.wide) {
     if ((e = allow_smem(lora_kernel<RN>, acc + ring)) != cudaSuccess) return e;
     return launch_chain(lora_kernel<RN>, dim3(p.max_tiles * kClusterCtas), block, acc + ring, s, g, p, direct);
   }
-  constexpr int expand = kTileTokens * 8 * RN * (int)sizeof(float) + ring;
-  if ((e = allow_smem(lora_shrink_kernel<RN>, acc)) != cudaSuccess || (e = allow_smem(lora_expand_kernel<RN>, expand)) != cudaSuccess) return e;
-  if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * kWideSplits), block, acc, s, g, p)) != cudaSuccess) return e;
-  // parts of the outputs: some 4 CTAs per slot of the GPU, but at least 256 outputs each
+  constexpr int wide_ring = Expand<RN, true>::kRingBytes > ring ? Expand<RN, true>::kRingBytes : ring;
+  constexpr int expand = kTileTokens * 8 * RN * (int)sizeof(float) + wide_ring;
+  constexpr int shrink = ShrinkRing<RN>::kStages * ShrinkRing<RN>::kStageBytes;
+  if ((e = allow_smem(lora_shrink_kernel<RN>, shrink)) != cudaSuccess || (e = allow_smem(lora_expand_kernel<RN>, expand)) != cudaSuccess) return e;
+  if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * kWideSplits), block, shrink, s, g, p)) != cudaSuccess) return e;
+  // parts of the outputs: some four rounds of two CTAs per SM, of at least 256 outputs each.  More start-ups (tile, tokens, u
+  // in three terms: 5 us) cost time, fewer parts scatter the rows under way: 8192 tokens x 5120 outputs of rank 64 take
+  // 157 / 135 / 121 / 120 / 124 / 128 us with 2 / 4 / 8 / 10 / 16 / 20 parts.
   const int tiles = g.T / kTileTokens;
-  int parts = (4 * 2 * kSmCountFallback + tiles - 1) / tiles;
+  int parts = (8 * kSmCountFallback + tiles - 1) / tiles;
   parts = parts > (g.n_out + 255) / 256 ? (g.n_out + 255) / 256 : parts;
   return launch_chain(lora_expand_kernel<RN>, dim3(p.max_tiles * parts), block, expand, s, g, p, parts);
 }
