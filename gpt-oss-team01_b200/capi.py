@@ -48,6 +48,7 @@ EXPORTS = [
     "gptoss_moe_forward_host_submit", "gptoss_moe_forward_host_sliced_submit", "gptoss_moe_forward_host_wait",
     "gptoss_model_layer_moe_dispatch", "gptoss_serving_last_error", "gptoss_serving_status", "gptoss_tree_attention_workspace", "gptoss_tree_attention",
     "gptoss_cache_commit", "gptoss_lora_workspace", "gptoss_lora_apply", "gptoss_expert_choice", "gptoss_moe_forward_routed",
+    "gptoss_model_step_tree", "gptoss_model_accept", "gptoss_model_lora_create", "gptoss_model_lora_load", "gptoss_model_lora_bind",
 ]
 
 
@@ -198,6 +199,11 @@ def load() -> C.CDLL:
         "gptoss_lora_apply": ([C.POINTER(LoraArgs), vp], i32),
         "gptoss_expert_choice": ([C.POINTER(ExpertChoiceArgs), vp], i32),
         "gptoss_moe_forward_routed": ([ctxp, i32, i32, vp, vp, vp, vp, vp], i32),
+        "gptoss_model_step_tree": ([vp, i32, vp, vp, vp, vp, vp, vp], i32),
+        "gptoss_model_accept": ([vp, i32, vp, vp, vp, vp], i32),
+        "gptoss_model_lora_create": ([vp, i32, i32], i32),
+        "gptoss_model_lora_load": ([vp, i32, i32, vp, vp, vp, vp, f32], i32),
+        "gptoss_model_lora_bind": ([vp, i32, i32], i32),
     }
     for name, (args, res) in sig.items():
         fn = getattr(lib, name)

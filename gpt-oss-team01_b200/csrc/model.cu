@@ -25,7 +25,7 @@
 #include <string>
 #include <vector>
 
-#include "kernels.cuh"
+#include "serving.cuh"
 
 using namespace gptoss;
 
@@ -63,6 +63,23 @@ struct gptoss_model {
   std::vector<char> row_taken;          // host scratch: cache rows named by the step's sequences (they must be distinct)
   std::vector<int> place;               // after such a step: where the caller's sequence i stands in that order
   bool last_step_ordered = false;       // the last step was one (gptoss_model_read_logits translates its row)
+  // a step over drafted tokens (gptoss_model_step_tree): its lists, on the host and on the device, and the attention's scratch
+  bool step_tree = false;
+  std::vector<int> tree_host;
+  int *tree_dev = nullptr;              // [max_batch * kTreeIntsPerToken + 1], made by the first such step
+  void *tree_work = nullptr;
+  size_t tree_work_bytes = 0;
+  gptoss_tree_attention_args tree_args{};
+  const int *tree_slots = nullptr, *tree_rope = nullptr, *tree_rows = nullptr;
+  // adapters beside the QKV and the output projection (gptoss_model_lora_create)
+  int lora_n = 0, lora_rank = 0, lora_bound = 0;  // adapters, their common rank, cache rows bound to one
+  __nv_bfloat16 *lora_a_qkv = nullptr, *lora_b_qkv = nullptr, *lora_a_o = nullptr, *lora_b_o = nullptr;  // [layer][adapter][..][..]
+  float *lora_scale = nullptr;
+  std::vector<int> lora_of_row, lora_ids_host;
+  int *lora_ids = nullptr;              // adapter of each row of the step
+  void *lora_work = nullptr;
+  size_t lora_work_bytes = 0;
+  bool step_lora = false;               // some row of the step has an adapter
   int cur_B = -1;
   cudaStream_t stream = nullptr;
   bool weights_ready = false;
@@ -88,6 +105,7 @@ struct gptoss_model {
 namespace {
 
 constexpr size_t kStagingElems = 16u << 20;  // 64 MiB of fp32
+constexpr int kTreeIntsPerToken = 4 + 3 + GPTOSS_TREE_MAX_NODES / 32;  // per token: row, slot, position, depth, mask; per sequence 3
 
 template <typename T>
 cudaError_t dalloc(T **p, size_t n) {
@@ -185,6 +203,28 @@ int pick_token_blocks(int B, int n_out, int sm_count) {
     if (best_cost < 0 || cost < best_cost) best_cost = cost, best = nb;
   }
   return best;
+}
+
+// The adapters of the step's rows: row i of the step lives in cache row rows_host[i] (null: i).
+int set_lora_ids(gptoss_model *m, const int *rows_host, int n) {
+  m->step_lora = false;
+  if (m->lora_bound == 0) return GPTOSS_OK;
+  m->lora_ids_host.resize(n);
+  for (int i = 0; i < n; ++i) {
+    m->lora_ids_host[i] = m->lora_of_row[rows_host ? rows_host[i] : i];
+    m->step_lora = m->step_lora || m->lora_ids_host[i] >= 0;
+  }
+  if (m->step_lora) MK(cudaMemcpyAsync(m->lora_ids, m->lora_ids_host.data(), n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+  return GPTOSS_OK;
+}
+
+// y[B, n_out] += s B_a (A_a x) for the rows that have an adapter; a, b: this layer's adapters
+int add_lora(gptoss_model *m, const __nv_bfloat16 *x, int K, int n_out, const __nv_bfloat16 *a, const __nv_bfloat16 *b, float *y, int B) {
+  if (!m->step_lora) return GPTOSS_OK;
+  gptoss_lora_args g{x, a, b, m->lora_scale, m->lora_ids, y, y, nullptr, 0, K, n_out, n_out, B, K, n_out, m->lora_rank, m->lora_n};
+  g.workspace = m->lora_work, g.workspace_bytes = m->lora_work_bytes;
+  const int rc = gptoss_lora_apply(&g, m->stream);
+  return rc ? m->fail(rc, gptoss_serving_last_error()) : GPTOSS_OK;
 }
 
 int set_batch(gptoss_model *m, int B) {
@@ -321,6 +361,7 @@ int gptoss_model_destroy(gptoss_model *m) {
   if (m->moe) gptoss_ctx_destroy(m->moe);
   void *ptrs[] = {m->emb, m->unemb, m->attn_norm, m->mlp_norm, m->final_norm, m->w_qkv, m->b_qkv, m->w_o, m->b_o, m->sinks,
                   m->cos_t, m->sin_t, m->k_cache, m->v_cache, m->x, m->t, m->qkv, m->q, m->att, m->proj, m->logits,
+                  m->tree_dev, m->tree_work, m->lora_a_qkv, m->lora_b_qkv, m->lora_a_o, m->lora_b_o, m->lora_scale, m->lora_ids, m->lora_work,
                   m->tokens_dev, m->next_dev, m->iota, m->rows_dev, m->pos_dev, m->amax_val, m->amax_at, m->amax_sched, m->ones, m->dense_off, m->dense_tbp, m->status, m->staging};
   for (void *p : ptrs) cudaFree(p);
   if (m->stream) cudaStreamDestroy(m->stream);
@@ -456,9 +497,12 @@ int gptoss_model_step_begin(gptoss_model *m, const int *tokens_host, int pos, in
   m->step_rows = nullptr;
   m->step_pos_rows = nullptr;
   m->last_step_ordered = false;
+  m->step_tree = false;
+  m->step_lora = false;
   if (n == 0) return GPTOSS_OK;
   int rc = set_batch(m, n);
   if (rc) return rc;
+  if ((rc = set_lora_ids(m, nullptr, n))) return rc;
   MK(cudaMemcpyAsync(m->tokens_dev, tokens_host, n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
   MK(launch_embed(m->tokens_dev, m->emb, n, m->c.hidden_dim, m->c.vocab_size, m->x, m->stream));
   return GPTOSS_OK;
@@ -477,37 +521,56 @@ int gptoss_model_layer_attention(gptoss_model *m, int layer) {
   if (B > 0) {
     MK(launch_residual_rmsnorm(m->x, nullptr, m->attn_norm + l * H, B, (int)H, m->t, s));
     if ((rc = dense(m, kDenseQkv, m->map_qkv[l], m->map_t, (int)H, (int)qkvd, m->b_qkv + l * qkvd, m->qkv))) return rc;
+    if (m->step_lora) {
+      const size_t n = (size_t)m->lora_n * m->lora_rank * l;
+      if ((rc = add_lora(m, m->t, (int)H, (int)qkvd, m->lora_a_qkv + n * H, m->lora_b_qkv + n * qkvd, m->qkv, B))) return rc;
+    }
     __nv_bfloat16 *kc = m->k_cache + l * (size_t)m->max_local * S * kvd, *vc = m->v_cache + l * (size_t)m->max_local * S * kvd;
-    MK(launch_qkv_rope_store(m->qkv, m->cos_t, m->sin_t, pos, B, nq, nkv, hd, (int)S, m->q, kc, vc, m->step_rows,
-                             m->step_pos_rows, s));
-    const bool windowed = c.sliding_window > 0 && (l % 2 == 0);  // run.cpp:582
-    const int window = windowed ? c.sliding_window : 0;
-    if (!m->step_pos_rows) {
-      const int t_lo = windowed && pos - window + 1 > 0 ? pos - window + 1 : 0;
-      MK(launch_attention(m->q, kc, vc, m->sinks + l * nq, pos, t_lo, B, nq, nkv, hd, (int)S, m->att, m->step_rows, nullptr, 0, s));
+    if (m->step_tree) {
+      __nv_bfloat16 *q16 = reinterpret_cast<__nv_bfloat16 *>(m->q);
+      MK(launch_qkv_rope_store_tree(m->qkv, m->cos_t, m->sin_t, B, nq, nkv, hd, (int)S, q16, kc, vc, m->tree_rows, m->tree_slots,
+                                    m->tree_rope, s));
+      gptoss_tree_attention_args a = m->tree_args;
+      a.q = q16, a.k_cache = kc, a.v_cache = vc, a.out = m->att, a.sinks = m->sinks + l * nq;
+      a.window = c.sliding_window > 0 && l % 2 == 0 ? c.sliding_window : 0;  // run.cpp:582
+      a.workspace = m->tree_work, a.workspace_bytes = m->tree_work_bytes;
+      if ((rc = gptoss_tree_attention(&a, s))) return m->fail(rc, gptoss_serving_last_error());
     } else {
-      // sequences at their own positions, ordered by position: one launch per run of sequences whose contexts (the
-      // window applied) ask for the same number of warps per problem, so every sequence is summed in the order a
-      // lock-step batch at its position would use
-      int b0 = 0;
-      while (b0 < B) {
-        int cls = 0;
-        while (m->class_end[cls] <= b0) ++cls;
-        const auto span_of = [&](int p) { return windowed && p > window - 1 ? window - 1 : p; };
-        const int warps = attention_warps_per_problem(span_of(m->class_pos[cls]));
-        int b1 = m->class_end[cls], span = span_of(m->class_pos[cls]);
-        for (int nx = cls + 1; nx < 3; ++nx) {  // following classes that the window folds into the same split
-          if (m->class_end[nx] == b1) continue;
-          if (attention_warps_per_problem(span_of(m->class_pos[nx])) != warps) break;
-          b1 = m->class_end[nx];
-          span = span_of(m->class_pos[nx]);
+      MK(launch_qkv_rope_store(m->qkv, m->cos_t, m->sin_t, pos, B, nq, nkv, hd, (int)S, m->q, kc, vc, m->step_rows,
+                               m->step_pos_rows, s));
+      const bool windowed = c.sliding_window > 0 && (l % 2 == 0);  // run.cpp:582
+      const int window = windowed ? c.sliding_window : 0;
+      if (!m->step_pos_rows) {
+        const int t_lo = windowed && pos - window + 1 > 0 ? pos - window + 1 : 0;
+        MK(launch_attention(m->q, kc, vc, m->sinks + l * nq, pos, t_lo, B, nq, nkv, hd, (int)S, m->att, m->step_rows, nullptr, 0, s));
+      } else {
+        // sequences at their own positions, ordered by position: one launch per run of sequences whose contexts (the
+        // window applied) ask for the same number of warps per problem, so every sequence is summed in the order a
+        // lock-step batch at its position would use
+        int b0 = 0;
+        while (b0 < B) {
+          int cls = 0;
+          while (m->class_end[cls] <= b0) ++cls;
+          const auto span_of = [&](int p) { return windowed && p > window - 1 ? window - 1 : p; };
+          const int warps = attention_warps_per_problem(span_of(m->class_pos[cls]));
+          int b1 = m->class_end[cls], span = span_of(m->class_pos[cls]);
+          for (int nx = cls + 1; nx < 3; ++nx) {  // following classes that the window folds into the same split
+            if (m->class_end[nx] == b1) continue;
+            if (attention_warps_per_problem(span_of(m->class_pos[nx])) != warps) break;
+            b1 = m->class_end[nx];
+            span = span_of(m->class_pos[nx]);
+          }
+          MK(launch_attention(m->q + (size_t)b0 * qd, kc, vc, m->sinks + l * nq, span, 0, b1 - b0, nq, nkv, hd, (int)S,
+                              m->att + (size_t)b0 * qd, m->step_rows + b0, m->step_pos_rows + b0, window, s));
+          b0 = b1;
         }
-        MK(launch_attention(m->q + (size_t)b0 * qd, kc, vc, m->sinks + l * nq, span, 0, b1 - b0, nq, nkv, hd, (int)S,
-                            m->att + (size_t)b0 * qd, m->step_rows + b0, m->step_pos_rows + b0, window, s));
-        b0 = b1;
       }
     }
     if ((rc = dense(m, kDenseOut, m->map_o[l], m->map_att, (int)qd, (int)H, m->b_o + l * H, m->proj))) return rc;
+    if (m->step_lora) {
+      const size_t n = (size_t)m->lora_n * m->lora_rank * l;
+      if ((rc = add_lora(m, m->att, (int)qd, (int)H, m->lora_a_o + n * qd, m->lora_b_o + n * H, m->proj, B))) return rc;
+    }
   }
   if (m->world == 1) {
     MK(launch_residual_rmsnorm(m->x, m->proj, m->mlp_norm + l * H, B, (int)H, m->t, s));
@@ -621,6 +684,7 @@ int gptoss_model_step_rows(gptoss_model *m, const int *tokens_host, const int *r
   }
   int rc = gptoss_model_step_begin(m, tokens_host, pos, n);
   if (rc) return rc;
+  if ((rc = set_lora_ids(m, rows_host, n))) return rc;
   MK(cudaMemcpyAsync(m->rows_dev, rows_host, n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
   m->step_rows = m->rows_dev;
   for (int l = 0; !rc && l < m->c.n_layers; ++l) {
@@ -673,6 +737,7 @@ int gptoss_model_step_seqs(gptoss_model *m, const int *tokens_host, const int *r
   }
   int rc = gptoss_model_step_begin(m, tok_s, max_pos, n);
   if (rc) return rc;
+  if ((rc = set_lora_ids(m, row_s, n))) return rc;
   MK(cudaMemcpyAsync(m->rows_dev, row_s, n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
   MK(cudaMemcpyAsync(m->pos_dev, pos_s, n * sizeof(int), cudaMemcpyHostToDevice, m->stream));
   m->step_rows = m->rows_dev;
@@ -691,6 +756,195 @@ int gptoss_model_step_seqs(gptoss_model *m, const int *tokens_host, const int *r
   m->place.assign(B, -1);
   for (int j = 0; j < n; ++j) m->place[m->perm[j]] = j;
   m->last_step_ordered = true;
+  return GPTOSS_OK;
+}
+
+// ---- drafted tokens -----------------------------------------------------------------------------------------------
+// One step over the drafted tokens of n_seqs sequences: every token is a row of the step (embedding, projections, MoE block,
+// classifier), K and V go to the slots behind the cached ones, attention goes along the tree.
+int gptoss_model_step_tree(gptoss_model *m, int n_seqs, const int *rows_host, const int *ctx_host, const int *offsets_host,
+                           const int *tokens_host, const int *parents_host, int *next_tokens_host) {
+  if (!m) return GPTOSS_ERR_BAD_ARG;
+  if (m->world != 1) return m->fail(GPTOSS_ERR_UNSUPPORTED, "drafted tokens are for a single-GPU model");
+  if (!rows_host || !ctx_host || !offsets_host || !tokens_host || !parents_host)
+    return m->fail(GPTOSS_ERR_BAD_ARG, "null row, context, offset, token or parent pointer");
+  if (n_seqs <= 0 || n_seqs > m->max_batch || offsets_host[0] != 0) return m->fail(GPTOSS_ERR_BAD_ARG, "number of sequences out of range, or offsets that do not start at 0");
+  m->row_taken.assign(m->max_batch, 0);
+  int max_nodes = 0, max_ctx = 0;
+  for (int b = 0; b < n_seqs; ++b) {
+    const int n = offsets_host[b + 1] - offsets_host[b];
+    if (n < 1 || n > GPTOSS_TREE_MAX_NODES || offsets_host[b + 1] > m->max_batch)
+      return m->fail(GPTOSS_ERR_BAD_ARG, "a sequence needs 1 to 256 drafted tokens, all sequences together at most max_batch");
+    if (rows_host[b] < 0 || rows_host[b] >= m->max_batch) return m->fail(GPTOSS_ERR_BAD_ARG, "cache row out of range");
+    if (m->row_taken[rows_host[b]]++) return m->fail(GPTOSS_ERR_BAD_ARG, "two sequences name the same cache row");
+    if (ctx_host[b] < 0 || ctx_host[b] > m->S - n) return m->fail(GPTOSS_ERR_BAD_ARG, "cached and drafted tokens do not fit in the cache");
+    for (int i = 0; i < n; ++i) {
+      const int p = parents_host[offsets_host[b] + i];
+      if (p < -1 || p >= i) return m->fail(GPTOSS_ERR_BAD_ARG, "a parent must be -1 or an earlier token of the same tree");
+    }
+    max_nodes = n > max_nodes ? n : max_nodes;
+    max_ctx = ctx_host[b] > max_ctx ? ctx_host[b] : max_ctx;
+  }
+  const int T = offsets_host[n_seqs], words = (max_nodes + 31) / 32;
+  int rc = gptoss_model_step_begin(m, tokens_host, 0, T);
+  if (rc) return rc;
+  // [per token: row, slot, position, depth][per sequence: row, context][offsets][masks]
+  m->tree_host.assign((size_t)T * (4 + words) + 3 * n_seqs + 1, 0);
+  int *row = m->tree_host.data(), *slot = row + T, *pos = slot + T, *depth = pos + T, *seq_row = depth + T, *ctx = seq_row + n_seqs,
+      *off = ctx + n_seqs, *mask = off + n_seqs + 1;
+  for (int b = 0; b < n_seqs; ++b) {
+    seq_row[b] = rows_host[b], ctx[b] = ctx_host[b], off[b + 1] = offsets_host[b + 1];
+    for (int t = offsets_host[b]; t < offsets_host[b + 1]; ++t) {
+      const int i = t - offsets_host[b], p = parents_host[t];
+      if (p >= 0) {
+        const int up = offsets_host[b] + p;
+        depth[t] = depth[up] + 1;
+        for (int w = 0; w < words; ++w) mask[(size_t)t * words + w] = mask[(size_t)up * words + w];
+      }
+      mask[(size_t)t * words + (i >> 5)] |= (int)(1u << (i & 31));
+      row[t] = rows_host[b], slot[t] = ctx_host[b] + i, pos[t] = ctx_host[b] + depth[t];
+    }
+  }
+  const auto ready = [&]() -> int {
+    if (!m->tree_dev) MK(dalloc(&m->tree_dev, (size_t)m->max_batch * kTreeIntsPerToken + 1));
+    MK(cudaMemcpyAsync(m->tree_dev, m->tree_host.data(), m->tree_host.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+    const auto there = [&](const int *p) { return m->tree_dev + (p - m->tree_host.data()); };
+    m->tree_rows = there(row), m->tree_slots = there(slot), m->tree_rope = there(pos);
+    gptoss_tree_attention_args a{};
+    a.offsets = there(off), a.ctx_len = there(ctx), a.rows = there(seq_row), a.mask = there(mask), a.depth = there(depth);
+    a.q_stride = a.out_stride = (int64_t)m->c.n_attn_heads * m->c.head_dim;
+    a.n_tokens = T, a.n_seqs = n_seqs, a.max_nodes = max_nodes, a.max_ctx = max_ctx, a.mask_words = words;
+    a.cache_rows = m->max_local, a.max_seq = m->S, a.n_q_heads = m->c.n_attn_heads, a.n_kv_heads = m->c.n_kv_heads;
+    a.head_dim = m->c.head_dim, a.scale = 1.0f / sqrtf((float)m->c.head_dim);
+    m->tree_args = a;
+    uint64_t need = gptoss_tree_attention_workspace(&a);
+    a.window = m->c.sliding_window;  // a shorter context may be cut into more, smaller shares
+    const uint64_t need_windowed = gptoss_tree_attention_workspace(&a);
+    if (need_windowed > need) need = need_windowed;
+    if (need > m->tree_work_bytes) {
+      MK(cudaStreamSynchronize(m->stream));
+      cudaFree(m->tree_work);
+      m->tree_work = nullptr, m->tree_work_bytes = 0;
+      MK(cudaMalloc(&m->tree_work, need));
+      m->tree_work_bytes = need;
+    }
+    m->step_tree = true;
+    return set_lora_ids(m, row, T);
+  };
+  rc = ready();
+  for (int l = 0; !rc && l < m->c.n_layers; ++l) {
+    if ((rc = gptoss_model_layer_attention(m, l))) break;
+    rc = gptoss_model_layer_moe_push(m, l);
+  }
+  int waits[kStatusWords] = {};
+  if (!rc) {
+    const cudaError_t e = serving_status_async(waits, m->stream);
+    if (e != cudaSuccess) rc = m->fail(GPTOSS_ERR_CUDA, "status of the attention", e);
+  }
+  if (!rc) rc = gptoss_model_step_end(m, next_tokens_host);  // synchronises the stream
+  m->step_B = 0;
+  m->step_tree = false;
+  if (!rc && waits[0] != 0) {
+    gptoss_serving_status();  // takes the report back
+    rc = m->fail(GPTOSS_ERR_TIMEOUT, "device-side bounded wait gave up in the tree attention");
+  }
+  return rc;
+}
+
+int gptoss_model_accept(gptoss_model *m, int n_seqs, const int *rows_host, const int *ctx_host, const int *offsets_host,
+                        const int *path_host) {
+  if (!m) return GPTOSS_ERR_BAD_ARG;
+  if (m->world != 1) return m->fail(GPTOSS_ERR_UNSUPPORTED, "drafted tokens are for a single-GPU model");
+  if (!rows_host || !ctx_host || !offsets_host || !path_host) return m->fail(GPTOSS_ERR_BAD_ARG, "null row, context, offset or path pointer");
+  if (n_seqs <= 0 || n_seqs > m->max_batch || offsets_host[0] != 0) return m->fail(GPTOSS_ERR_BAD_ARG, "number of sequences out of range, or offsets that do not start at 0");
+  m->row_taken.assign(m->max_batch, 0);
+  int longest = 0;
+  for (int b = 0; b < n_seqs; ++b) {
+    const int n = offsets_host[b + 1] - offsets_host[b];
+    if (n < 0 || n > GPTOSS_TREE_MAX_NODES || offsets_host[b + 1] > m->max_batch) return m->fail(GPTOSS_ERR_BAD_ARG, "path length out of range");
+    if (rows_host[b] < 0 || rows_host[b] >= m->max_batch) return m->fail(GPTOSS_ERR_BAD_ARG, "cache row out of range");
+    if (m->row_taken[rows_host[b]]++) return m->fail(GPTOSS_ERR_BAD_ARG, "two sequences name the same cache row");
+    for (int j = 0; j < n; ++j) {
+      const int at = path_host[offsets_host[b] + j], before = j ? path_host[offsets_host[b] + j - 1] : -1;
+      if (at <= before || at >= GPTOSS_TREE_MAX_NODES || ctx_host[b] < 0 || ctx_host[b] > m->S - 1 - at)
+        return m->fail(GPTOSS_ERR_BAD_ARG, "a path must ascend and lie in the cache");
+    }
+    longest = n > longest ? n : longest;
+  }
+  if (longest == 0) return GPTOSS_OK;
+  MK(cudaSetDevice(m->device));
+  if (!m->tree_dev) return m->fail(GPTOSS_ERR_STATE, "no step over drafted tokens before");
+  m->tree_host.assign(rows_host, rows_host + n_seqs);
+  m->tree_host.insert(m->tree_host.end(), ctx_host, ctx_host + n_seqs);
+  m->tree_host.insert(m->tree_host.end(), offsets_host, offsets_host + n_seqs + 1);
+  m->tree_host.insert(m->tree_host.end(), path_host, path_host + offsets_host[n_seqs]);
+  MK(cudaMemcpyAsync(m->tree_dev, m->tree_host.data(), m->tree_host.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream));
+  const int rc = gptoss_cache_commit(m->k_cache, m->v_cache, m->c.n_layers, m->max_local, m->c.n_kv_heads, m->S, m->c.head_dim, n_seqs,
+                                     m->tree_dev, m->tree_dev + n_seqs, m->tree_dev + 2 * n_seqs, m->tree_dev + 3 * n_seqs + 1, longest,
+                                     m->stream);
+  return rc ? m->fail(rc, gptoss_serving_last_error()) : GPTOSS_OK;
+}
+
+// ---- adapters -----------------------------------------------------------------------------------------------------
+int gptoss_model_lora_create(gptoss_model *m, int n_adapters, int rank) {
+  if (!m) return GPTOSS_ERR_BAD_ARG;
+  if (m->world != 1) return m->fail(GPTOSS_ERR_UNSUPPORTED, "adapters are for a single-GPU model");
+  if (m->lora_n) return m->fail(GPTOSS_ERR_STATE, "the model has its adapters already");
+  if (n_adapters < 1 || n_adapters > 8192 || rank < 8 || rank > GPTOSS_LORA_MAX_RANK || rank % 8)
+    return m->fail(GPTOSS_ERR_BAD_ARG, "1 to 8192 adapters of a rank that is a multiple of 8 up to 128");
+  MK(cudaSetDevice(m->device));
+  const gptoss_model_config &c = m->c;
+  const size_t qd = (size_t)c.head_dim * c.n_attn_heads, qkvd = m->qkv_dim(), H = c.hidden_dim, n = (size_t)c.n_layers * n_adapters * rank;
+  // it grows with the rows of a step and does not depend on the projection's size
+  gptoss_lora_args g{};
+  g.T = m->max_batch, g.K = (int)H, g.n_out = (int)qkvd, g.rank = rank, g.n_adapters = n_adapters;
+  m->lora_work_bytes = gptoss_lora_workspace(&g);
+  struct { void **p; size_t bytes; } parts[] = {
+      {(void **)&m->lora_a_qkv, n * H * 2}, {(void **)&m->lora_b_qkv, n * qkvd * 2}, {(void **)&m->lora_a_o, n * qd * 2},
+      {(void **)&m->lora_b_o, n * H * 2}, {(void **)&m->lora_scale, n_adapters * sizeof(float)},
+      {(void **)&m->lora_ids, m->max_batch * sizeof(int)}, {&m->lora_work, m->lora_work_bytes ? m->lora_work_bytes : 16}};
+  cudaError_t e = cudaSuccess;
+  for (auto &x : parts) {
+    if (e == cudaSuccess) e = cudaMalloc(x.p, x.bytes);
+    if (e == cudaSuccess) e = cudaMemset(*x.p, 0, x.bytes);
+  }
+  if (e != cudaSuccess) {
+    for (auto &x : parts) {
+      cudaFree(*x.p);
+      *x.p = nullptr;
+    }
+    m->lora_work_bytes = 0;
+    return m->fail(GPTOSS_ERR_CUDA, "memory for the adapters", e);
+  }
+  m->lora_of_row.assign(m->max_batch, -1);
+  m->lora_n = n_adapters, m->lora_rank = rank;
+  return GPTOSS_OK;
+}
+
+int gptoss_model_lora_load(gptoss_model *m, int adapter, int layer, const float *a_qkv, const float *b_qkv, const float *a_o,
+                           const float *b_o, float scale) {
+  if (!m) return GPTOSS_ERR_BAD_ARG;
+  if (adapter < 0 || adapter >= m->lora_n || layer < 0 || layer >= m->c.n_layers) return m->fail(GPTOSS_ERR_BAD_ARG, "adapter or layer out of range");
+  MK(cudaSetDevice(m->device));
+  MK(cudaStreamSynchronize(m->stream));  // no step in flight reads what changes
+  const size_t qd = (size_t)m->c.head_dim * m->c.n_attn_heads, qkvd = m->qkv_dim(), H = m->c.hidden_dim, r = m->lora_rank;
+  const size_t at = ((size_t)layer * m->lora_n + adapter) * r;
+  int rc = GPTOSS_OK;
+  if (!rc && a_qkv) rc = upload_bf16(m, m->lora_a_qkv + at * H, a_qkv, r * H);
+  if (!rc && b_qkv) rc = upload_bf16(m, m->lora_b_qkv + at * qkvd, b_qkv, r * qkvd);
+  if (!rc && a_o) rc = upload_bf16(m, m->lora_a_o + at * qd, a_o, r * qd);
+  if (!rc && b_o) rc = upload_bf16(m, m->lora_b_o + at * H, b_o, r * H);
+  if (!rc) MK(cudaMemcpy(m->lora_scale + adapter, &scale, sizeof scale, cudaMemcpyHostToDevice));
+  if (!rc) MK(cudaDeviceSynchronize());
+  return rc;
+}
+
+int gptoss_model_lora_bind(gptoss_model *m, int row, int adapter) {
+  if (!m) return GPTOSS_ERR_BAD_ARG;
+  if (m->lora_n == 0) return m->fail(GPTOSS_ERR_STATE, "the model has no adapters");
+  if (row < 0 || row >= m->max_batch || adapter < -1 || adapter >= m->lora_n) return m->fail(GPTOSS_ERR_BAD_ARG, "cache row or adapter out of range");
+  m->lora_bound += (adapter >= 0) - (m->lora_of_row[row] >= 0);
+  m->lora_of_row[row] = adapter;
   return GPTOSS_OK;
 }
 

@@ -55,13 +55,17 @@ __global__ void __launch_bounds__(256) residual_rmsnorm_kernel(float *__restrict
 // qkv[b, :] = (q heads | k heads | v heads), bias already added (run.cpp:534-557).  Rotates q and k with the
 // cos/sin of position `pos` (half-split pairs: element i pairs with i + hd/2), writes q as fp32 and k, v as
 // bf16 into the caches at [b, kv_head, pos, i]: the rows that one (sequence, kv head) attends to are contiguous.
+// TREE: row b is a drafted token, cached in slot pos_rows[b] of row cache_rows[b] but rotated for position rope_rows[b]
+// (siblings share a position), and q goes out as bf16, the type of the tree attention's products.
+template <bool TREE>
 __global__ void __launch_bounds__(256) qkv_rope_store_kernel(const float *__restrict__ qkv, const float *__restrict__ cos_t,
                                                              const float *__restrict__ sin_t, int pos, int nq, int nkv,
                                                              int hd, int S, float *__restrict__ q_out,
                                                              __nv_bfloat16 *__restrict__ k_cache,
                                                              __nv_bfloat16 *__restrict__ v_cache,
                                                              const int *__restrict__ cache_rows,
-                                                             const int *__restrict__ pos_rows) {
+                                                             const int *__restrict__ pos_rows,
+                                                             const int *__restrict__ rope_rows) {
   pdl_wait();
   const int b = blockIdx.x;
   const int cb = cache_rows ? cache_rows[b] : b;  // cache row of sequence b (a compacted batch keeps its rows)
@@ -69,8 +73,9 @@ __global__ void __launch_bounds__(256) qkv_rope_store_kernel(const float *__rest
   const int half = hd >> 1, hp = half >> 1;  // hp: pairs of adjacent rotation indices per head (hd is 32 or 64)
   const int qdim = nq * hd, kvdim = nkv * hd;
   const float *row = qkv + (size_t)b * (qdim + 2 * kvdim);
-  const float2 *cs = reinterpret_cast<const float2 *>(cos_t + (size_t)pos * half);
-  const float2 *sn = reinterpret_cast<const float2 *>(sin_t + (size_t)pos * half);
+  const int rope_pos = TREE ? rope_rows[b] : pos;
+  const float2 *cs = reinterpret_cast<const float2 *>(cos_t + (size_t)rope_pos * half);
+  const float2 *sn = reinterpret_cast<const float2 *>(sin_t + (size_t)rope_pos * half);
   for (int i = threadIdx.x; i < (nq + nkv) * hp; i += blockDim.x) {
     const int h = i / hp, j = 2 * (i - h * hp);  // heads 0..nq-1 are q, nq.. are k; elements j, j+1 and their partners
     const float *src = row + (size_t)h * hd;
@@ -78,7 +83,11 @@ __global__ void __launch_bounds__(256) qkv_rope_store_kernel(const float *__rest
     const float2 c = cs[j >> 1], s = sn[j >> 1];
     const float2 o1 = make_float2(x1.x * c.x - x2.x * s.x, x1.y * c.y - x2.y * s.y);
     const float2 o2 = make_float2(x2.x * c.x + x1.x * s.x, x2.y * c.y + x1.y * s.y);
-    if (h < nq) {
+    if (TREE && h < nq) {
+      __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(q_out) + (size_t)b * qdim + h * hd + j;
+      *reinterpret_cast<__nv_bfloat162 *>(dst) = __floats2bfloat162_rn(o1.x, o1.y);
+      *reinterpret_cast<__nv_bfloat162 *>(dst + half) = __floats2bfloat162_rn(o2.x, o2.y);
+    } else if (h < nq) {
       float *dst = q_out + (size_t)b * qdim + h * hd + j;
       *reinterpret_cast<float2 *>(dst) = o1;
       *reinterpret_cast<float2 *>(dst + half) = o2;
@@ -451,8 +460,14 @@ cudaError_t launch_residual_rmsnorm(float *x, const float *add, const float *w, 
 cudaError_t launch_qkv_rope_store(const float *qkv, const float *cos_t, const float *sin_t, int pos, int B, int nq, int nkv,
                                   int hd, int S, float *q_out, __nv_bfloat16 *k_cache, __nv_bfloat16 *v_cache,
                                   const int *cache_rows, const int *pos_rows, cudaStream_t s) {
-  return launch_chain(qkv_rope_store_kernel, dim3(B), dim3(256), 0, s, qkv, cos_t, sin_t, pos, nq, nkv, hd, S, q_out, k_cache,
-                      v_cache, cache_rows, pos_rows);
+  return launch_chain(qkv_rope_store_kernel<false>, dim3(B), dim3(256), 0, s, qkv, cos_t, sin_t, pos, nq, nkv, hd, S, q_out, k_cache,
+                      v_cache, cache_rows, pos_rows, nullptr);
+}
+cudaError_t launch_qkv_rope_store_tree(const float *qkv, const float *cos_t, const float *sin_t, int B, int nq, int nkv, int hd, int S,
+                                       __nv_bfloat16 *q_out, __nv_bfloat16 *k_cache, __nv_bfloat16 *v_cache, const int *cache_rows,
+                                       const int *slots, const int *rope_rows, cudaStream_t s) {
+  return launch_chain(qkv_rope_store_kernel<true>, dim3(B), dim3(256), 0, s, qkv, cos_t, sin_t, 0, nq, nkv, hd, S,
+                      reinterpret_cast<float *>(q_out), k_cache, v_cache, cache_rows, slots, rope_rows);
 }
 cudaError_t launch_attention(const float *q, const __nv_bfloat16 *k_cache, const __nv_bfloat16 *v_cache, const float *sinks,
                              int pos, int t_lo, int B, int nq, int nkv, int hd, int S, __nv_bfloat16 *out, const int *cache_rows,

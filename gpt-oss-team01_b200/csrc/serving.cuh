@@ -1,5 +1,5 @@
 // What the serving operators (tree_attention.cu, lora.cu, expert_choice.cu) share: the message of the last failing call
-// of a host thread, and the launchers that the model step calls.
+// of a host thread, and the report of bounded waits that gave up.
 #pragma once
 
 #include "kernels.cuh"
@@ -8,6 +8,9 @@ namespace gptoss {
 
 // Remembers `msg` for gptoss_serving_last_error() of this host thread and returns `code`.
 int serving_fail(int code, const char *msg, cudaError_t e = cudaSuccess);
+
+// Copies the status words of the operators' bounded waits ([0] != 0: one gave up) to the host behind what `s` holds.
+cudaError_t serving_status_async(int *host, cudaStream_t s);
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

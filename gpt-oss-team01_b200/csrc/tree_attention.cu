@@ -600,6 +600,10 @@ __global__ void __launch_bounds__(128) cache_commit_kernel(uint4 *__restrict__ k
 
 }  // namespace
 
+cudaError_t serving_status_async(int *host, cudaStream_t s) {
+  return cudaMemcpyFromSymbolAsync(host, g_serving_status, kStatusWords * sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+}
+
 int serving_fail(int code, const char *msg, cudaError_t e) {
   if (e != cudaSuccess)
     snprintf(g_serving_error, sizeof g_serving_error, "%s: %s (%s)", msg, cudaGetErrorName(e), cudaGetErrorString(e));

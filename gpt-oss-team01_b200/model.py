@@ -123,6 +123,107 @@ class Model:
                                                     nxt.ctypes.data_as(C.c_void_p) if need_next else None))
         return nxt
 
+    # ---- drafted tokens ---------------------------------------------------------------------------------------
+    def step_tree(self, tokens, parents, rows, ctx, need_next=True):
+        """A step over drafted tokens: sequence b (cache row ``rows[b]``, ``ctx[b]`` cached tokens) runs ``tokens[b]``, a tree
+        in which token i follows token ``parents[b][i]`` (-1: the last cached one).  Returns the greedy tokens that follow
+        each of them, a list of int32 arrays (None with need_next=False)."""
+        offsets = np.zeros(len(tokens) + 1, np.int32)
+        offsets[1:] = np.cumsum([len(t) for t in tokens])
+        flat = np.concatenate([np.asarray(t, np.int32) for t in tokens]) if len(tokens) else np.zeros(0, np.int32)
+        up = np.concatenate([np.asarray(p, np.int32) for p in parents]) if len(tokens) else np.zeros(0, np.int32)
+        rows, ctx = np.ascontiguousarray(rows, dtype=np.int32), np.ascontiguousarray(ctx, dtype=np.int32)
+        assert flat.shape == up.shape and rows.shape == ctx.shape == (len(tokens),)
+        nxt = np.empty_like(flat) if need_next else None
+        p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+        self._check(self.lib.gptoss_model_step_tree(self._m, len(tokens), p(rows), p(ctx), p(offsets), p(flat), p(up),
+                                                    p(nxt) if need_next else None))
+        return [nxt[offsets[b]:offsets[b + 1]] for b in range(len(tokens))] if need_next else None
+
+    def accept(self, rows, ctx, paths):
+        """Keeps the drafted tokens ``paths[b]`` (ascending, from the root down) of the last step_tree as the next cached
+        tokens of the sequence in cache row ``rows[b]``; ``ctx``: the contexts of that step.  Returns the new ones."""
+        offsets = np.zeros(len(paths) + 1, np.int32)
+        offsets[1:] = np.cumsum([len(t) for t in paths])
+        flat = np.concatenate([np.asarray(t, np.int32) for t in paths] + [np.zeros(1, np.int32)])
+        rows, ctx = np.ascontiguousarray(rows, dtype=np.int32), np.ascontiguousarray(ctx, dtype=np.int32)
+        assert rows.shape == ctx.shape == (len(paths),)
+        p = lambda a: a.ctypes.data_as(C.c_void_p)  # noqa: E731
+        self._check(self.lib.gptoss_model_accept(self._m, len(paths), p(rows), p(ctx), p(offsets), p(flat)))
+        return ctx + np.diff(offsets)
+
+    @staticmethod
+    def greedy_path(tokens, parents, nxt):
+        """The path of a tree rooted in token 0 that greedy decoding takes: from the root on, the child that equals the
+        greedy token after its parent.  ``nxt``: what step_tree returned for the tree."""
+        path = [0]
+        while True:
+            children = [i for i in range(path[-1] + 1, len(tokens)) if parents[i] == path[-1] and tokens[i] == nxt[path[-1]]]
+            if not children:
+                return path
+            path.append(children[0])
+
+    def generate_drafted(self, prompts, n_generate, draft):
+        """Greedy continuations of ``prompts`` (lists of ids, any lengths) in steps over drafted tokens.  ``draft(history)``
+        proposes what may follow the ids seen so far: (tokens, parents), parents counting within the proposal, -1 for a
+        token that follows the history directly.  Returns int32 [B, n_generate]; the number of steps does not change the
+        result (up to bf16 rounding of near-ties), only the time."""
+        B = len(prompts)
+        hist, ctx = [list(map(int, p)) for p in prompts], np.zeros(B, np.int32)
+        room = max(1, min(256, self.max_batch // B))
+        goal = [len(h) + n_generate for h in hist]
+        while any(len(h) < g for h, g in zip(hist, goal)):
+            live = [b for b in range(B) if len(hist[b]) < goal[b]]
+            toks, pars, new = [], [], {}
+            for b in live:
+                todo = hist[b][ctx[b]:]           # ids that are not cached yet: a piece of the prompt, or the last token
+                piece = todo[:room]
+                t, p = list(piece), list(range(-1, len(piece) - 1))
+                if len(piece) == len(todo):       # the history is complete: drafted tokens behind it
+                    dt, dp = draft(hist[b])
+                    keep = min(len(dt), room - len(piece), self.max_seq - int(ctx[b]) - len(piece))
+                    for i in range(max(0, keep)):
+                        t.append(int(dt[i]))
+                        p.append(len(piece) - 1 if dp[i] < 0 else len(piece) + dp[i])
+                toks.append(t), pars.append(p), new.setdefault(b, (len(piece), len(piece) == len(todo)))
+            nxt = self.step_tree(toks, pars, live, ctx[live])
+            paths = []
+            for j, b in enumerate(live):
+                n, complete = new[b]
+                path = list(range(n))
+                if complete:
+                    t, p = toks[j][n - 1:], [q - (n - 1) for q in pars[j][n - 1:]]
+                    tail = self.greedy_path(t, p, nxt[j][n - 1:])
+                    out = [int(nxt[j][n - 1 + i]) for i in tail][:goal[b] - len(hist[b])]
+                    path += [n - 1 + i for i in tail[1:len(out)]]
+                    hist[b] += out
+                paths.append(path)
+            ctx[live] = self.accept(live, ctx[live], paths)
+        return np.array([h[-n_generate:] for h in hist], np.int32).reshape(B, n_generate)
+
+    # ---- adapters ---------------------------------------------------------------------------------------------
+    def lora_create(self, n_adapters, rank):
+        """Room for low-rank adapters beside the QKV and the attention output projection of every layer (all zero)."""
+        self._check(self.lib.gptoss_model_lora_create(self._m, int(n_adapters), int(rank)))
+        self._lora_rank = int(rank)
+
+    def lora_load(self, adapter, layer, a_qkv=None, b_qkv=None, a_o=None, b_o=None, scale=1.0):
+        """One layer of an adapter: a_qkv [rank, hidden], b_qkv [qkv, rank], a_o [rank, heads * head_dim], b_o [hidden, rank]
+        (fp32 arrays; None leaves a part as it is).  ``scale`` holds for every layer of the adapter."""
+        c, r = self.cfg, getattr(self, "_lora_rank", 0)
+        qd = c.head_dim * c.n_attn_heads
+        qkv = c.head_dim * (c.n_attn_heads + 2 * c.n_kv_heads)
+        arrs = []
+        for a, shape in ((a_qkv, (r, c.hidden_dim)), (b_qkv, (qkv, r)), (a_o, (r, qd)), (b_o, (c.hidden_dim, r))):
+            arrs.append(None if a is None else np.ascontiguousarray(a, dtype=np.float32))
+            assert a is None or arrs[-1].shape == shape, (arrs[-1].shape, shape)
+        self._check(self.lib.gptoss_model_lora_load(self._m, int(adapter), int(layer),
+                                                    *[None if a is None else a.ctypes.data_as(C.c_void_p) for a in arrs], float(scale)))
+
+    def lora_bind(self, row, adapter):
+        """The sequence in cache row ``row`` (sequence ``row`` of a lock-step batch) uses this adapter; -1: none."""
+        self._check(self.lib.gptoss_model_lora_bind(self._m, int(row), int(adapter)))
+
     @staticmethod
     def step_group(models, tokens, pos, need_next=True):
         """One step of a whole group driven from this thread: ``tokens`` int32 [B] for the whole batch; every phase

@@ -462,6 +462,31 @@ int gptoss_model_step_rows(gptoss_model *m, const int *tokens_host, const int *r
  * whoever shares the batch.  Single-GPU models only. */
 int gptoss_model_step_seqs(gptoss_model *m, const int *tokens_host, const int *rows_host, const int *pos_host, int n,
                            int *next_tokens_host);
+/* One step over drafted tokens: sequence b holds cache row rows_host[b] (distinct) with ctx_host[b] cached tokens, and
+ * drafted tokens tokens_host[offsets_host[b] .. offsets_host[b+1]) (1 to 256 of them, max_batch over all sequences) form a
+ * tree: parents_host[t] is the index within the tree of the token that t follows (an earlier one), or -1 if it follows the
+ * last cached token.  Every drafted token is run at position ctx + depth, seeing the cached tokens, its ancestors and
+ * itself; next_tokens_host (may be NULL) gets the greedy token that follows each of them.  Their K and V stay in the slots
+ * behind the cached ones until gptoss_model_accept keeps some.  With a chain per sequence this is also a prompt in pieces.
+ * The attention rounds queries and weights to bf16 (the one-token step keeps them in two terms), so logits agree with those
+ * of one-token steps to bf16 rounding, not bit for bit.  Single-GPU models only. */
+int gptoss_model_step_tree(gptoss_model *m, int n_seqs, const int *rows_host, const int *ctx_host, const int *offsets_host,
+                           const int *tokens_host, const int *parents_host, int *next_tokens_host);
+/* Keeps the drafted tokens path_host[offsets_host[b] .. offsets_host[b+1]) (ascending indices of the tree of the last
+ * gptoss_model_step_tree of that row, a path from its root) as the next cached tokens of sequence b, in every layer; the
+ * caller counts its context up by their number.  ctx_host: the context of that step.  Asynchronous on the model's stream. */
+int gptoss_model_accept(gptoss_model *m, int n_seqs, const int *rows_host, const int *ctx_host, const int *offsets_host,
+                        const int *path_host);
+/* Low-rank adapters beside the QKV and the attention output projection of every layer: room for n_adapters (up to 8192) of
+ * one rank (a multiple of 8 up to GPTOSS_LORA_MAX_RANK), all zero.  Once per model; single-GPU models only. */
+int gptoss_model_lora_create(gptoss_model *m, int n_adapters, int rank);
+/* One layer of one adapter (host fp32, rounded to bf16; a NULL part stays as it is): a_qkv [rank][hidden],
+ * b_qkv [qkv][rank], a_o [rank][n_q_heads * head_dim], b_o [hidden][rank].  scale multiplies B A in every layer.  Waits for
+ * the model's stream. */
+int gptoss_model_lora_load(gptoss_model *m, int adapter, int layer, const float *a_qkv, const float *b_qkv, const float *a_o,
+                           const float *b_o, float scale);
+/* The sequence in cache row `row` uses this adapter from its next step on (-1: none, the state of every row at first). */
+int gptoss_model_lora_bind(gptoss_model *m, int row, int adapter);
 /* The phases of gptoss_model_step, which runs begin, then per layer attention / moe_dispatch / moe_push / moe_combine,
  * then end.  In a group, B is the batch of the group and tokens_host / next_tokens_host hold this rank's sequences only.
  * Separate entry points so that one host thread can drive the ranks of a group in turn (each phase for every rank
