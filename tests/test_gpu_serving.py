@@ -417,6 +417,33 @@ def test_route_experts_infinities_and_nan(serving, scoring):
     check_route(serving, logits, 5, scoring=scoring, n_groups=4, topk_groups=2, group_top=1)
 
 
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_experts_scores_that_all_but_vanish(serving, scoring):
+    logits = torch.randn(20, 64, generator=gen(12), device="cuda") - (150 if scoring == "sigmoid" else 0)
+    logits[:, 40:] -= 150
+    bias = torch.zeros(64, device="cuda")
+    bias[40:] = torch.linspace(3, 2, 24, device="cuda")
+    for renorm in (True, False):
+        check_route(serving, logits, 6, scoring=scoring, bias=bias, renormalize=renorm)
+        check_route(serving, logits, 3, scoring=scoring, bias=bias, renormalize=renorm, n_groups=8, topk_groups=2, group_top=2)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_experts_many_random_rows(serving, scoring):
+    """Against the plain operator in 64 bits on the GPU: 20000 rows, so that near ties of every kind occur."""
+    logits = torch.randn(20000, 256, generator=gen(13), device="cuda") * 1.5
+    bias = torch.randn(256, generator=gen(14), device="cuda") * 0.1
+    x = logits.double()
+    score = torch.softmax(x, 1) if scoring == "softmax" else torch.sigmoid(x)
+    for b in (None, bias):
+        choice = score if b is None else score + b.double()
+        want = torch.sort(choice, dim=1, descending=True, stable=True).indices[:, :8]
+        w, i = serving.route_experts(logits, 8, scoring=scoring, bias=b)
+        assert torch.equal(i.long(), want)
+        ww = torch.gather(score, 1, want)
+        torch.testing.assert_close(w.double(), ww / ww.sum(1, keepdim=True), rtol=W_TOL, atol=0)
+
+
 def test_route_experts_strided_rows_stream_and_graph(serving):
     wide = torch.randn(70, 100, generator=gen(8), device="cuda")
     check_route(serving, wide[:, 3:67], 4, scoring="sigmoid")
