@@ -2,6 +2,7 @@
 // place.  Both replace nothing in the reference, which decodes one token per sequence and step
 // (getp-csrc/src/model.cpp:6-151); the attention is that of run.cpp:565-607 (learned sink in the denominator, sliding
 // window) for many queries per sequence under a mask.
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -39,6 +40,9 @@ constexpr int kAttStages = 4;
 constexpr int kAttThreads = 2 * kAttRows + 64;    // two groups of 4 softmax warps, the products' warp, the copies' warp
 constexpr int kAttCtasPerSm = 2;
 constexpr int kMaxPoison = 1536;                  // slots of masked tiles that can hold a non-finite V element, noted by each group
+constexpr int kMaxClusterSplits = 8;              // shares of the context that join as a cluster
+template <int HD>
+constexpr int kJoinStride = HD + 4;               // floats from row to row there: O, m, l; 16-byte accesses of 8 rows stay apart
 constexpr uint32_t kTmemS = 0, kTmemO = 64, kTmemGroup = 128, kAttTmemCols = 256;  // per group: S (P in its first columns), O
 
 struct AttCtrl {
@@ -53,6 +57,7 @@ struct AttParams {
   CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 64, 1}
   gptoss_tree_attention_args a;
   int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
+  bool in_cluster;           // the shares of the context are a cluster and join in shared memory
   float c;                   // scale * log2(e)
 };
 
@@ -212,10 +217,10 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const gptoss_tree_attention_args &a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   int x = blockIdx.x;
-  const int pair = x % p.q_pairs;
-  x /= p.q_pairs;
   const int split = x % p.n_splits;
   x /= p.n_splits;
+  const int pair = x % p.q_pairs;
+  x /= p.q_pairs;
   const int kvh = x % a.n_kv_heads, b = x / a.n_kv_heads;
   pdl_wait();
   const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
@@ -481,6 +486,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
       join[(HD + 1) * kAttRows] = l;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
+    bool keep = false;
     if (valid && (by_rows || g == 0)) {
       if (!by_rows) {
         const float m1 = join[HD * kAttRows], top1 = fmaxf(m, m1), base1 = top1 == -INFINITY ? 0.f : top1;
@@ -499,7 +505,9 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         for (int j = 0; j < HD; ++j)
           if ((v[j] & 0x7f80u) == 0x7f80u) o[j] += __uint_as_float((uint32_t)v[j] << 16);
       }
-      if (p.n_splits == 1) {
+      if (p.in_cluster) {
+        keep = true;
+      } else if (p.n_splits == 1) {
         const float sink = a.sinks ? a.sinks[head] * 1.44269504f : -INFINITY;
         const float top = fmaxf(m, sink), base = top == -INFINITY ? 0.f : top;
         const float w = ex2(m - base), total = fmaf(l, w, ex2(sink - base));
@@ -518,6 +526,15 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         ml[at] = make_float2(m, l);
       }
     }
+    if (p.in_cluster) {
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // the memory that the rows are left in has been read
+      if (keep) {
+        float *mine = reinterpret_cast<float *>(smem) + (g * kAttRows + r) * kJoinStride<HD>;
+#pragma unroll
+        for (int j = 0; j < HD; j += 4) *reinterpret_cast<float4 *>(mine + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        *reinterpret_cast<float2 *>(mine + HD) = make_float2(m, l);
+      }
+    }
   }
   pdl_launch_dependents();
   tc_fence_before();
@@ -526,6 +543,47 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     tc_fence_after();
     tmem_dealloc(tmem, kAttTmemCols);
   }
+  if (!p.in_cluster) return;
+  // The shares meet: each CTA of the cluster joins every n_splits-th row, HD / 4 threads a row, the shares in their order.
+  static_assert(2 * kAttRows * kJoinStride<HD> * 4 <= 2 * kAttQBytes + 2 * kAttStages * kAttTileBytes, "the rows fit where Q and the ring were");
+  cluster_sync_all();
+  constexpr int TPR = HD / 4;
+  const int rows_here = by_rows ? 2 * kAttRows : kAttRows, per_tile = p.nodes_per_tile * p.group, d4 = threadIdx.x % TPR;
+  for (int i = split + p.n_splits * (threadIdx.x / TPR); i < rows_here; i += p.n_splits * (kAttThreads / TPR)) {
+    const int in_tile = i % kAttRows, nd = (i / kAttRows) * p.nodes_per_tile + in_tile / p.group;
+    if (in_tile >= per_tile || nd >= nodes) continue;
+    const int hq = kvh * p.group + in_tile % p.group;
+    const uint32_t at = q_s + 4 * i * kJoinStride<HD>;
+    const float sink = a.sinks ? a.sinks[hq] * 1.44269504f : -INFINITY;
+    float2 ml[kMaxClusterSplits];
+    float4 v[kMaxClusterSplits];
+    float top = sink;
+#pragma unroll
+    for (int s = 0; s < kMaxClusterSplits; ++s)
+      if (s < p.n_splits) {
+        const uint32_t there = map_to_cta(at, s);
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[s].x), "=f"(ml[s].y) : "r"(there + 4 * HD) : "memory");
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
+                     : "r"(there + 16 * d4)
+                     : "memory");
+        top = fmaxf(top, ml[s].x);
+      }
+    const float base = top == -INFINITY ? 0.f : top;
+    float total = ex2(sink - base);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int s = 0; s < kMaxClusterSplits; ++s)
+      if (s < p.n_splits) {
+        const float w = ex2(ml[s].x - base);
+        total = fmaf(ml[s].y, w, total);
+        acc.x = fmaf(v[s].x, w, acc.x), acc.y = fmaf(v[s].y, w, acc.y), acc.z = fmaf(v[s].z, w, acc.z), acc.w = fmaf(v[s].w, w, acc.w);
+      }
+    const float inv = total == 0.f ? 0.f : 1.f / total;
+    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (size_t)(first + n0 + nd) * a.out_stride + (size_t)hq * HD + 4 * d4) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  }
+  cluster_sync_all();  // nobody reads this CTA's memory any more
 }
 
 // Joins the shares of the context: out = sum_s O_s 2^(m_s - M) / (sum_s l_s 2^(m_s - M) + 2^(sink - M)).  HD / 4 threads
@@ -622,6 +680,7 @@ namespace {
 
 // How a call is cut: query tiles, and shares of the context when the (sequence, kv head, query tile) items alone would not
 // fill two CTAs on every SM.
+constexpr int kClusterTiles = 64;
 struct AttPlan {
   int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
 };
@@ -638,6 +697,9 @@ AttPlan plan_of(const gptoss_tree_attention_args &a) {
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
   long long splits = items > 0 ? ((long long)kAttCtasPerSm * sms + items - 1) / items : 1;
   if (splits > tiles) splits = tiles;
+  // More shares than a cluster holds go through memory and a second kernel, which a context has to be worth: up to
+  // kClusterTiles tiles, 8 shares it is.
+  if (splits > kMaxClusterSplits && tiles <= kClusterTiles) splits = kMaxClusterSplits;
   if (splits < 1) splits = 1;
   p.tiles_per_split = (int)((tiles + splits - 1) / splits);
   p.n_splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
@@ -650,16 +712,41 @@ bool countable(const gptoss_tree_attention_args &a) {
 }
 
 uint64_t workspace_of(const gptoss_tree_attention_args &a, int n_splits) {
-  return n_splits <= 1 ? 0 : (uint64_t)n_splits * a.n_tokens * a.n_q_heads * (a.head_dim + 2) * sizeof(float);
+  return n_splits <= kMaxClusterSplits ? 0 : (uint64_t)n_splits * a.n_tokens * a.n_q_heads * (a.head_dim + 2) * sizeof(float);
 }
 
 template <int HD>
 cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
+  static std::atomic<uint64_t> configured{0};  // devices (of the first 64) on which the kernel may have its shared memory
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e == cudaSuccess && (device >= 64 || !(configured.load(std::memory_order_relaxed) >> device & 1))) {
+    e = cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
+    if (e == cudaSuccess && device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
+  }
   if (e != cudaSuccess) return e;
-  const dim3 grid((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_pairs * p.n_splits));
-  e = launch_chain(tree_attention_kernel<HD>, grid, dim3(kAttThreads), kAttSmem, s, p);
-  if (e != cudaSuccess || p.n_splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_pairs * p.n_splits));
+  cfg.blockDim = dim3(kAttThreads);
+  cfg.dynamicSmemBytes = kAttSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (p.in_cluster) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = (unsigned)p.n_splits;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  count_launch();
+  e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<HD>, p);
+  if (e != cudaSuccess || p.n_splits <= kMaxClusterSplits) return e;
   const int heads = 256 / (HD / 4);
   return launch_chain(tree_merge_kernel<HD>, dim3(p.a.n_seqs * p.a.max_nodes, (p.a.n_q_heads + heads - 1) / heads), dim3(256), 0, s,
                       p.a, p.n_splits);
@@ -716,6 +803,7 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
   p.a = a;
   p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.q_pairs = plan.q_pairs;
   p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
+  p.in_cluster = plan.n_splits > 1 && plan.n_splits <= kMaxClusterSplits;
   p.c = a.scale * 1.44269504f;
   const uint64_t slabs = (uint64_t)a.cache_rows * a.n_kv_heads;
   cudaError_t e = encode_map_3d(&p.map_k, a.k_cache, a.head_dim, a.max_seq, slabs, kAttTile);
