@@ -379,13 +379,16 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
                  a.mask + (size_t)tok * a.mask_words, a.depth + first};
     const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * kTmemGroup + kTmemS, to = ts + kTmemO;
     const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
+    const uint32_t s_full = smem_u32(&ctrl->s_full[g]), p_full = smem_u32(&ctrl->p_full[g]);
+    // tiles [plain_first, plain_end) are seen whole by every row
+    const int plain_first = (max(lo_max - slot_first, 0) + kAttTile - 1) / kAttTile, plain_end = max(ctx - slot_first, 0) / kAttTile;
     float m = -INFINITY, l = 0.f;
     int k = 0;
     for (int i = by_rows ? 0 : g; i < n_tiles; i += by_rows ? 1 : 2, ++k) {
-      const int t0 = slot_first + i * kAttTile;
-      const bool masked = t0 < lo_max || t0 + kAttTile > ctx;
+      const bool masked = i < plain_first || i >= plain_end;
       uint32_t bits[2] = {0u, 0u};
       if (masked) {
+        const int t0 = slot_first + i * kAttTile;
         if (valid) bits[0] = view.word(t0), bits[1] = view.word(t0 + 32);
         // half of slot r / 2 of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
         // (two groups on one tile both look at all of it: what the second still finds, the first has written as well)
@@ -410,10 +413,11 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      float s[kAttTile];
-      wait_warp(&ctrl->s_full[g], k & 1, &ctrl->abort, 0x2600);
+      wait_addr(s_full, k & 1, &ctrl->abort, 0x2600);
+      __syncwarp();
       tc_fence_after();
       if (live) {
+        float s[kAttTile];
 #pragma unroll
         for (int j = 0; j < kAttTile; j += 32) tmem_ld32(ts + j, s + j);
         tmem_ld_wait();
@@ -426,20 +430,23 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         for (int j = 12; j + 1 < kAttTile; j += 2) mx[(j >> 1) & 3] = max3_nan(mx[(j >> 1) & 3], s[j], s[j + 1]);
         const float top = max3_nan(max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * p.c;
         const bool move = top > m + 8.f;
-        float corr = 1.f;
-        if (move) {
-          corr = ex2(m - top);
-          m = top;
-        }
-        if (k > 0 && __any_sync(0xffffffffu, move)) {
+        if (__any_sync(0xffffffffu, move)) {
+          float corr = 1.f;
+          if (move) {
+            corr = ex2(m - top);
+            m = top;
+          }
+          l *= corr;
+          if (k > 0) {  // P V of the tile before is complete, as S of this tile is
 #pragma unroll
-          for (int h = 0; h < HD; h += 16) {
-            uint32_t o[16];
-            tmem_ld16(to + h, o);
-            tmem_ld_wait();
+            for (int h = 0; h < HD; h += 16) {
+              uint32_t o[16];
+              tmem_ld16(to + h, o);
+              tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-            tmem_st16(to + h, o);
+              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+              tmem_st16(to + h, o);
+            }
           }
         }
         const float base = m == -INFINITY ? 0.f : m;
@@ -457,12 +464,12 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
           }
           tmem_st16(ts + (h >> 1), pk);
         }
-        l = l * corr + ((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y));
+        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         tmem_st_wait();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&ctrl->p_full[g]));
+      if (lane == 0) mbar_arrive(p_full);
     }
     // ---- result of this share of the context ----
     wait_warp(&ctrl->retired, 0, &ctrl->abort, 0x2900);
@@ -695,7 +702,7 @@ AttPlan plan_of(const gptoss_tree_attention_args &a) {
   // the cached tokens that a tree can reach: with a window, as many as its first token sees
   const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
-  long long splits = items > 0 ? ((long long)kAttCtasPerSm * sms + items - 1) / items : 1;
+  long long splits = items > 0 ? (long long)kAttCtasPerSm * sms / items : 1;  // one round of CTAs
   if (splits > tiles) splits = tiles;
   // More shares than a cluster holds go through memory and a second kernel, which a context has to be worth: up to
   // kClusterTiles tiles, 8 shares it is.
