@@ -39,6 +39,7 @@ constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 
 constexpr int kAttStages = 4;
 constexpr int kAttThreads = 2 * kAttRows + 64;    // two groups of 4 softmax warps, the products' warp, the copies' warp
 constexpr int kAttCtasPerSm = 2;
+constexpr int kMaxDepth = GPTOSS_TREE_MAX_NODES;  // beyond any depth
 constexpr int kMaxPoison = 1536;                  // slots of masked tiles that can hold a non-finite V element, noted by each group
 constexpr int kMaxClusterSplits = 8;              // shares of the context that join as a cluster
 template <int HD>
@@ -48,8 +49,9 @@ constexpr uint32_t kTmemS = 0, kTmemO = 64, kTmemGroup = 128, kAttTmemCols = 256
 struct AttCtrl {
   uint64_t full[kAttStages], empty[kAttStages], s_full[2], p_full[2], retired;
   uint32_t tmem_base;
-  int abort, depth_lo, depth_hi, n_poison;
+  int abort, n_poison;
   int poison[kMaxPoison];
+  int mask[GPTOSS_TREE_MAX_NODES * GPTOSS_TREE_MAX_NODES / 32];  // of this CTA's tokens
 };
 constexpr size_t kAttSmem = 2 * kAttQBytes + kAttTileBytes * 2 * kAttStages + 1024 + sizeof(AttCtrl);
 
@@ -222,55 +224,48 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const int pair = x % p.q_pairs;
   x /= p.q_pairs;
   const int kvh = x % a.n_kv_heads, b = x / a.n_kv_heads;
-  pdl_wait();
-  const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
-  const int n0 = 2 * pair * p.nodes_per_tile, nodes = n - n0;
-  if (first < 0 || nodes <= 0) {
-    pdl_launch_dependents();
-    return;
-  }
-  const bool by_rows = nodes > p.nodes_per_tile;  // a query tile for each group, else the slot tiles are dealt out to them
-  const int row = a.rows ? a.rows[b] : b;
-  int ctx = min(max(a.ctx_len[b], 0), a.max_seq);
-  int len = min(ctx + n, a.max_seq);
-  if (row < 0 || row >= a.cache_rows) ctx = len = 0;
-  const int slab = row * a.n_kv_heads + kvh;
-
+  // what does not depend on the kernels before
   if (threadIdx.x == 0) {
     for (int i = 0; i < kAttStages; ++i) mbar_init(smem_u32(&ctrl->full[i]), 1), mbar_init(smem_u32(&ctrl->empty[i]), 1);
     for (int i = 0; i < 2; ++i) mbar_init(smem_u32(&ctrl->s_full[i]), 1), mbar_init(smem_u32(&ctrl->p_full[i]), 4);
     mbar_init(smem_u32(&ctrl->retired), 1);
-    ctrl->abort = 0, ctrl->n_poison = 0, ctrl->depth_lo = 0x3fffffff, ctrl->depth_hi = 0;
+    ctrl->abort = 0, ctrl->n_poison = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
     tmem_alloc(smem_u32(&ctrl->tmem_base), kAttTmemCols);
     tmem_relinquish();
   }
-  // query rows into shared memory, in the layout a 128-byte-swizzled copy would give them (rows beyond the tree hold
-  // whatever lies there: a row of the products depends on its own row of Q only)
-  const int r = threadIdx.x % kAttRows, g = threadIdx.x / kAttRows;
-  const int tile_node = by_rows ? g * p.nodes_per_tile : 0;  // first node of this group's query tile
-  const int node = tile_node + r / p.group, head = kvh * p.group + r % p.group;
-  const bool valid = g < 2 && r < p.nodes_per_tile * p.group && node < nodes;
-  const int tok = first + n0 + (valid ? node : 0);
-  if (valid && (by_rows || g == 0)) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
-#pragma unroll
-    for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + g * kAttQBytes + r * 128 + ((c ^ (r & 7)) << 4)) = src[c];
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const int depth = a.window > 0 && valid ? min(max(a.depth[tok], 0), kMaxPoison) : 0;
-  if (a.window > 0) {
-    if (valid) atomicMin(&ctrl->depth_lo, depth), atomicMax(&ctrl->depth_hi, depth);
-    __syncthreads();
-  }
   const uint32_t tmem = ctrl->tmem_base;
-  const int lo_min = a.window > 0 ? min(max(ctx + ctrl->depth_lo - a.window + 1, 0), ctx) : 0;
-  const int lo_max = a.window > 0 ? min(max(ctx + ctrl->depth_hi - a.window + 1, 0), ctx) : 0;
+  pdl_wait();
+  const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
+  const int row = a.rows ? a.rows[b] : b;
+  int ctx = min(max(a.ctx_len[b], 0), a.max_seq);
+  const int n0 = 2 * pair * p.nodes_per_tile, nodes = min(n - n0, 2 * p.nodes_per_tile);
+  if (first < 0 || nodes <= 0) {  // with all CTAs of its cluster
+    pdl_launch_dependents();
+    if (warp == 8) tmem_dealloc(tmem, kAttTmemCols);
+    return;
+  }
+  const bool by_rows = nodes > p.nodes_per_tile;  // a query tile for each group, else the slot tiles are dealt out to them
+  int len = min(ctx + n, a.max_seq);
+  if (row < 0 || row >= a.cache_rows) ctx = len = 0;
+  const int slab = row * a.n_kv_heads + kvh;
+  // least and largest depth of this CTA's tokens, found by each warp for itself
+  int depth_lo = 0, depth_hi = 0;
+  if (a.window > 0) {
+    depth_lo = kMaxDepth;
+    for (int i = lane; i < nodes; i += 32) {
+      const int d = min(max(a.depth[first + n0 + i], 0), kMaxDepth);
+      depth_lo = min(depth_lo, d), depth_hi = max(depth_hi, d);
+    }
+    depth_lo = __reduce_min_sync(0xffffffffu, depth_lo), depth_hi = __reduce_max_sync(0xffffffffu, depth_hi);
+  }
+  const int lo_min = a.window > 0 ? min(max(ctx + depth_lo - a.window + 1, 0), ctx) : 0;
+  const int lo_max = a.window > 0 ? min(max(ctx + depth_hi - a.window + 1, 0), ctx) : 0;
   const int tiles = (len - lo_min + kAttTile - 1) / kAttTile;
   const int t_begin = min(tiles, split * p.tiles_per_split);
   const int n_tiles = (split == p.n_splits - 1 ? tiles : min(tiles, t_begin + p.tiles_per_split)) - t_begin;
@@ -303,6 +298,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     // One elected lane does it all (elect.sync tells the compiler that one thread runs; under a plain lane == 0 every issue
     // becomes a loop over lanes).  Its instructions stand between P and the next S: addresses and descriptors are kept as
     // running values.
+    asm volatile("bar.sync 2, 288;" ::: "memory");  // the query rows are there
+    tc_fence_after();
     if (elect_one()) {
       const uint32_t idesc_s = umma_idesc(kAttTile), idesc_o = umma_idesc(HD) | kIdescTransposeB;
       const uint32_t full = smem_u32(ctrl->full), empty = smem_u32(ctrl->empty), s_full = smem_u32(ctrl->s_full),
@@ -375,8 +372,28 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     __syncwarp();
   } else {
     // ===================== softmax, a thread per query row =====================
-    RowView view{ctx, len - ctx, a.window > 0 ? min(max(ctx + depth - a.window + 1, 0), ctx) : 0, a.window, depth, a.mask_words,
-                 a.mask + (size_t)tok * a.mask_words, a.depth + first};
+    // query rows into shared memory, in the layout a 128-byte-swizzled copy would give them (rows beyond the tree hold
+    // whatever lies there: a row of the products depends on its own row of Q only), and the tokens' masks
+    const int r = threadIdx.x % kAttRows, g = threadIdx.x / kAttRows;
+    const int node = (by_rows ? g * p.nodes_per_tile : 0) + r / p.group, head = kvh * p.group + r % p.group;
+    const bool valid = r < p.nodes_per_tile * p.group && node < nodes;
+    const int tok = first + n0 + (valid ? node : 0);
+    if (valid && (by_rows || g == 0)) {
+      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
+      uint4 q[HD / 8];
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) q[c] = src[c];
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4 *>(smem + g * kAttQBytes + r * 128 + ((c ^ (r & 7)) << 4)) = q[c];
+    }
+    const int words = min(a.mask_words, GPTOSS_TREE_MAX_NODES / 32);
+    for (int i = threadIdx.x; i < nodes * words; i += 2 * kAttRows)
+      ctrl->mask[i] = a.mask[(size_t)(first + n0 + i / words) * a.mask_words + i % words];
+    const int depth = a.window > 0 ? min(max(a.depth[tok], 0), kMaxDepth) : 0;
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    asm volatile("bar.sync 2, 288;" ::: "memory");
+    RowView view{ctx, len - ctx, a.window > 0 ? min(max(ctx + depth - a.window + 1, 0), ctx) : 0, a.window, depth, words,
+                 ctrl->mask + (valid ? node : 0) * words, a.depth + first};
     const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * kTmemGroup + kTmemS, to = ts + kTmemO;
     const bool live = __any_sync(0xffffffffu, valid);  // a warp without rows only keeps the barriers going
     const uint32_t s_full = smem_u32(&ctrl->s_full[g]), p_full = smem_u32(&ctrl->p_full[g]);
@@ -554,8 +571,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   // The shares meet: each CTA of the cluster joins every n_splits-th row, HD / 4 threads a row, the shares in their order.
   static_assert(2 * kAttRows * kJoinStride<HD> * 4 <= 2 * kAttQBytes + 2 * kAttStages * kAttTileBytes, "the rows fit where Q and the ring were");
   cluster_sync_all();
-  constexpr int TPR = HD / 4;
-  const int rows_here = by_rows ? 2 * kAttRows : kAttRows, per_tile = p.nodes_per_tile * p.group, d4 = threadIdx.x % TPR;
+  constexpr int TPR = HD / 16;  // threads per row
+  const int rows_here = by_rows ? 2 * kAttRows : kAttRows, per_tile = p.nodes_per_tile * p.group, part = threadIdx.x % TPR;
   for (int i = split + p.n_splits * (threadIdx.x / TPR); i < rows_here; i += p.n_splits * (kAttThreads / TPR)) {
     const int in_tile = i % kAttRows, nd = (i / kAttRows) * p.nodes_per_tile + in_tile / p.group;
     if (in_tile >= per_tile || nd >= nodes) continue;
@@ -563,32 +580,42 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     const uint32_t at = q_s + 4 * i * kJoinStride<HD>;
     const float sink = a.sinks ? a.sinks[hq] * 1.44269504f : -INFINITY;
     float2 ml[kMaxClusterSplits];
-    float4 v[kMaxClusterSplits];
     float top = sink;
 #pragma unroll
-    for (int s = 0; s < kMaxClusterSplits; ++s)
-      if (s < p.n_splits) {
-        const uint32_t there = map_to_cta(at, s);
-        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[s].x), "=f"(ml[s].y) : "r"(there + 4 * HD) : "memory");
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(v[s].x), "=f"(v[s].y), "=f"(v[s].z), "=f"(v[s].w)
-                     : "r"(there + 16 * d4)
-                     : "memory");
-        top = fmaxf(top, ml[s].x);
-      }
+    for (int s = 0; s < kMaxClusterSplits; ++s) {
+      ml[s] = make_float2(-INFINITY, 0.f);
+      if (s < p.n_splits)
+        asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ml[s].x), "=f"(ml[s].y) : "r"(map_to_cta(at, s) + 4 * HD) : "memory");
+    }
+    float acc[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+#pragma unroll
+    for (int s = 0; s < kMaxClusterSplits; ++s) top = fmaxf(top, ml[s].x);
     const float base = top == -INFINITY ? 0.f : top;
     float total = ex2(sink - base);
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int s = 0; s < kMaxClusterSplits; ++s)
       if (s < p.n_splits) {
+        const uint32_t there = map_to_cta(at, s) + 64 * part;
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j += 4)
+          asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                       : "=f"(v[j]), "=f"(v[j + 1]), "=f"(v[j + 2]), "=f"(v[j + 3])
+                       : "r"(there + 4 * j)
+                       : "memory");
         const float w = ex2(ml[s].x - base);
         total = fmaf(ml[s].y, w, total);
-        acc.x = fmaf(v[s].x, w, acc.x), acc.y = fmaf(v[s].y, w, acc.y), acc.z = fmaf(v[s].z, w, acc.z), acc.w = fmaf(v[s].w, w, acc.w);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[j] = fmaf(v[j], w, acc[j]);
       }
     const float inv = total == 0.f ? 0.f : 1.f / total;
-    *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(a.out) + (size_t)(first + n0 + nd) * a.out_stride + (size_t)hq * HD + 4 * d4) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    uint4 *dst = reinterpret_cast<uint4 *>(static_cast<uint16_t *>(a.out) + (size_t)(first + n0 + nd) * a.out_stride + (size_t)hq * HD + 16 * part);
+#pragma unroll
+    for (int j = 0; j < 16; j += 8)
+      dst[j >> 3] = make_uint4(pack_bf16(acc[j] * inv, acc[j + 1] * inv), pack_bf16(acc[j + 2] * inv, acc[j + 3] * inv),
+                               pack_bf16(acc[j + 4] * inv, acc[j + 5] * inv), pack_bf16(acc[j + 6] * inv, acc[j + 7] * inv));
   }
   cluster_sync_all();  // nobody reads this CTA's memory any more
 }
@@ -687,7 +714,7 @@ namespace {
 
 // How a call is cut: query tiles, and shares of the context when the (sequence, kv head, query tile) items alone would not
 // fill two CTAs on every SM.
-constexpr int kClusterTiles = 64;
+constexpr int kJoinTiles = 2, kMergeTiles = 8;
 struct AttPlan {
   int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
 };
@@ -702,12 +729,17 @@ AttPlan plan_of(const gptoss_tree_attention_args &a) {
   // the cached tokens that a tree can reach: with a window, as many as its first token sees
   const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
-  long long splits = items > 0 ? (long long)kAttCtasPerSm * sms / items : 1;  // one round of CTAs
-  if (splits > tiles) splits = tiles;
-  // More shares than a cluster holds go through memory and a second kernel, which a context has to be worth: up to
-  // kClusterTiles tiles, 8 shares it is.
-  if (splits > kMaxClusterSplits && tiles <= kClusterTiles) splits = kMaxClusterSplits;
-  if (splits < 1) splits = 1;
+  // Shares of the context for one round of CTAs, as far as they pay: joining them costs a CTA as much time as some kJoinTiles
+  // tiles (a cluster) or kMergeTiles (through memory and a second kernel).
+  const long long most = items > 0 ? (long long)kAttCtasPerSm * sms / items : 1;
+  const auto per = [&](long long n) { return (tiles + n - 1) / n; };
+  long long splits = 1, cost = tiles;
+  for (long long n = 2; n <= kMaxClusterSplits && n <= most && n <= tiles; ++n)
+    if (per(n) + kJoinTiles < cost) splits = n, cost = per(n) + kJoinTiles;
+  if (most > kMaxClusterSplits && tiles > kMaxClusterSplits) {
+    const long long n = most < tiles ? most : tiles;
+    if (per(n) + kMergeTiles < cost) splits = n;
+  }
   p.tiles_per_split = (int)((tiles + splits - 1) / splits);
   p.n_splits = (int)((tiles + p.tiles_per_split - 1) / p.tiles_per_split);
   return p;
