@@ -159,20 +159,20 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
   asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// 2^x for finite x below 127 (below -126: 2^-126): x = n + f with n the nearest integer, taken from the low bits of
-// x + 1.5 * 2^23, and 2^f by the polynomial of degree 4 with the smallest largest relative error on [-1/2, 1/2]
-// (Remez exchange: 2^-18.5), its exponent then raised by n.
+// 2^x for x below 127, 0 below -125.5 (-infinity among them): x = n + f with n the nearest integer, taken from the low bits
+// of x + 1.5 * 2^23, and 2^f by the polynomial of degree 4 with the smallest largest relative error on [-1/2, 1/2] (Remez
+// exchange: 2^-18.5), its exponent then raised by n.
 __device__ __forceinline__ float2 ex2_poly(float2 x) {
   constexpr float kShift = 12582912.f;
-  x.x = fmaxf(x.x, -126.f), x.y = fmaxf(x.y, -126.f);
-  const float2 t = add2(x, make_float2(kShift, kShift));
-  const float2 f = fma2(add2(t, make_float2(-kShift, -kShift)), make_float2(-1.f, -1.f), x);
+  const float2 z = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  const float2 t = add2(z, make_float2(kShift, kShift));
+  const float2 f = fma2(add2(t, make_float2(-kShift, -kShift)), make_float2(-1.f, -1.f), z);
   float2 y = fma2(f, make_float2(0.009570102f, 0.009570102f), make_float2(0.05591786f, 0.05591786f));
   y = fma2(f, y, make_float2(0.24024744f, 0.24024744f));
   y = fma2(f, y, make_float2(0.6931218f, 0.6931218f));
   y = fma2(f, y, make_float2(0.9999993f, 0.9999993f));
-  return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
-                     __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+  return make_float2(x.x < -125.5f ? 0.f : __uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)),
+                     x.y < -125.5f ? 0.f : __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
 }
 __device__ __forceinline__ bool bf16_nonfinite(uint32_t pair) {
   return (pair & 0x7f80u) == 0x7f80u || (pair & 0x7f800000u) == 0x7f800000u;
@@ -466,16 +466,19 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
             }
           }
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        // an infinite or NaN score makes the row NaN whatever the rest is (ex2_poly could not tell)
+        const float base = fabsf(top) < INFINITY || top == -INFINITY ? (m == -INFINITY ? 0.f : m) : NAN;
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         const float2 c2 = make_float2(p.c, p.c), base2 = make_float2(-base, -base);
+        // Every eighth pair goes through the FMA units instead of the exponential unit, which takes 8 cycles for a warp's 32
+        // (64 x 64 tokens over 4096: 293 us instead of 300).
 #pragma unroll
         for (int h = 0; h < kAttTile; h += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float2 x = fma2(make_float2(s[h + j], s[h + j + 1]), c2, base2);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+            const float2 e = j % 16 == 6 ? ex2_poly(x) : make_float2(ex2(x.x), ex2(x.y));
             sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
             pk[j >> 1] = pack_bf16(e.x, e.y);
           }
@@ -714,7 +717,7 @@ namespace {
 
 // How a call is cut: query tiles, and shares of the context when the (sequence, kv head, query tile) items alone would not
 // fill two CTAs on every SM.
-constexpr int kJoinTiles = 2, kMergeTiles = 8;
+constexpr int kJoinTiles = 4, kMergeTiles = 8;
 struct AttPlan {
   int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
 };
@@ -826,7 +829,7 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
   if (!a.q || !a.k_cache || !a.v_cache || !a.offsets || !a.ctx_len || !a.mask || !a.out)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "null pointer");
   if (a.window < 0 || (a.window > 0 && !a.depth)) return serving_fail(GPTOSS_ERR_BAD_ARG, "a window needs the depths of the drafted tokens");
-  if (!(a.scale >= 0.f) || std::isinf(a.scale)) return serving_fail(GPTOSS_ERR_BAD_ARG, "scale must be finite and not negative");
+  if (!(a.scale > 0.f) || std::isinf(a.scale)) return serving_fail(GPTOSS_ERR_BAD_ARG, "scale must be finite and positive");
   if (!aligned16(a.q) || !aligned16(a.k_cache) || !aligned16(a.v_cache) || !aligned16(a.out) || a.q_stride % 8 || a.out_stride % 8)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "q, caches and out must be 16-byte aligned, token strides multiples of 8 elements");
   if (a.q_stride < (int64_t)a.n_q_heads * a.head_dim || a.out_stride < (int64_t)a.n_q_heads * a.head_dim)

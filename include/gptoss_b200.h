@@ -318,7 +318,7 @@ typedef struct {
   int n_tokens, n_seqs, max_nodes, max_ctx, mask_words;
   int cache_rows, max_seq, n_q_heads, n_kv_heads, head_dim;
   int window;           /* 0: none */
-  float scale;          /* of the scores, 1/sqrt(head_dim) as a rule; finite, not negative */
+  float scale;          /* of the scores, 1/sqrt(head_dim) as a rule; finite and positive */
 } gptoss_tree_attention_args;
 uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *args);
 int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream);

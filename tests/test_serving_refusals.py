@@ -31,7 +31,7 @@ def tree_args(**kw):
     dict(n_seqs=-1), dict(n_tokens=-1), dict(max_nodes=-1), dict(max_ctx=-1), dict(head_dim=48), dict(head_dim=128),
     dict(n_q_heads=9), dict(n_q_heads=18, n_kv_heads=2), dict(n_kv_heads=0), dict(max_nodes=257), dict(max_nodes=33),
     dict(cache_rows=0), dict(max_seq=0), dict(q=None), dict(k_cache=None), dict(v_cache=None), dict(out=None), dict(offsets=None),
-    dict(ctx_len=None), dict(mask=None), dict(window=-1), dict(window=5, depth=None), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(workspace=A + 8, max_ctx=64000), dict(max_ctx=64000), dict(workspace=A, workspace_bytes=1000, max_ctx=64000), dict(q=A + 8), dict(k_cache=A + 2),
+    dict(ctx_len=None), dict(mask=None), dict(window=-1), dict(window=5, depth=None), dict(scale=-1.0), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(workspace=A + 8, max_ctx=64000), dict(max_ctx=64000), dict(workspace=A, workspace_bytes=1000, max_ctx=64000), dict(q=A + 8), dict(k_cache=A + 2),
     dict(v_cache=A + 8), dict(out=A + 4), dict(q_stride=516), dict(out_stride=516), dict(q_stride=504), dict(out_stride=8)])
 def test_tree_attention_refuses(lib, bad):
     assert lib.gptoss_tree_attention(C.byref(tree_args(**bad)), None) == capi.ERR_BAD_ARG
