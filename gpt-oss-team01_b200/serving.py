@@ -11,8 +11,9 @@ Each call runs on the device of its tensors, asynchronously on ``stream`` (defau
 comes from torch's allocator, so calls on different streams and captured graphs have their own.  Errors raise
 ``GptossError``.  Nothing is kept between calls.
 
-The calls are short on the GPU (from 2 us), so their host side counts: checks are plain attribute comparisons, and the
-raw stream handle is asked for directly (a ``torch.cuda.Stream`` object costs 3 us, a device context 1.4 us).
+The calls are short on the GPU (from 2 us), so their host side counts: what a call is given is looked over in one
+expression, and only where that fails are the arguments gone through one by one for the message; the raw stream handle is
+asked for directly (a ``torch.cuda.Stream`` object costs 3 us, a device context 1.4 us).
 """
 from __future__ import annotations
 
@@ -101,36 +102,51 @@ def tree_attention(q, k_cache, v_cache, offsets, ctx_len, mask, depth=None, *, m
     offsets int32 [B+1], ctx_len int32 [B], mask int32 [n_tokens, words], depth int32 [n_tokens] (with a window), sinks fp32
     [n_q_heads], cache_rows int32 [B].  max_nodes / max_ctx: upper bounds of the drafted / cached tokens of a sequence.
     Returns out like q (bf16); rows behind the last sequence are not written."""
-    dev = _view("q", q, _BF16, 3)
+    try:
+        dev = q.get_device()
+        plain = (
+            q.dtype is _BF16 is k_cache.dtype is v_cache.dtype and offsets.dtype is _I32 is ctx_len.dtype is mask.dtype
+            and q.dim() == 3 and k_cache.dim() == 4 and mask.dim() == 2 and offsets.dim() == 1 == ctx_len.dim()
+            and 0 <= dev == k_cache.get_device() == v_cache.get_device() == offsets.get_device() == ctx_len.get_device() == mask.get_device()
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and offsets.is_contiguous() and ctx_len.is_contiguous()
+            and mask.is_contiguous()
+            and (depth is None or depth.dtype is _I32 and depth.dim() == 1 and depth.get_device() == dev and depth.is_contiguous())
+            and (sinks is None or sinks.dtype is _F32 and sinks.dim() == 1 and sinks.get_device() == dev and sinks.is_contiguous())
+            and (cache_rows is None or cache_rows.dtype is _I32 and cache_rows.dim() == 1 and cache_rows.get_device() == dev
+                 and cache_rows.is_contiguous()))
+    except AttributeError:
+        plain = False
+    if not plain:
+        dev = _view("q", q, _BF16, 3)
+        _dense("k_cache", k_cache, _BF16, 4, dev)
+        _dense("v_cache", v_cache, _BF16, 4, dev)
+        _dense("offsets", offsets, _I32, 1, dev)
+        _dense("ctx_len", ctx_len, _I32, 1, dev)
+        _dense("mask", mask, _I32, 2, dev)
+        for name, t, dtype in (("depth", depth, _I32), ("sinks", sinks, _F32), ("cache_rows", cache_rows, _I32)):
+            if t is not None:
+                _dense(name, t, dtype, 1, dev)
     n_tokens, nq, hd = q.shape
     token_stride, head_stride, last = q.stride()
     if last != 1 or (head_stride != hd and nq > 1):
         _bad("q: heads of a token must be contiguous")
-    _dense("k_cache", k_cache, _BF16, 4, dev)
-    _dense("v_cache", v_cache, _BF16, 4, dev)
     rows, nkv, max_seq, cache_hd = k_cache.shape
     if v_cache.shape != k_cache.shape or cache_hd != hd:
         _bad("k_cache and v_cache must have the same shape and q's head_dim")
-    _dense("offsets", offsets, _I32, 1, dev)
-    _dense("ctx_len", ctx_len, _I32, 1, dev)
-    _dense("mask", mask, _I32, 2, dev)
     n_seqs = ctx_len.shape[0]
     mask_rows, words = mask.shape
     if offsets.shape[0] != n_seqs + 1 or mask_rows < n_tokens:
         _bad("offsets needs one more entry than ctx_len, mask a row per token")
     depth_at = sinks_at = rows_at = None
     if depth is not None:
-        _dense("depth", depth, _I32, 1, dev)
         if depth.shape[0] < n_tokens:
             _bad("depth needs an entry per token")
         depth_at = depth.data_ptr()
     if sinks is not None:
-        _dense("sinks", sinks, _F32, 1, dev)
         if sinks.shape[0] != nq:
             _bad("sinks needs an entry per query head")
         sinks_at = sinks.data_ptr()
     if cache_rows is not None:
-        _dense("cache_rows", cache_rows, _I32, 1, dev)
         if cache_rows.shape[0] != n_seqs:
             _bad("cache_rows needs an entry per sequence")
         rows_at = cache_rows.data_ptr()
@@ -150,7 +166,7 @@ def tree_attention(q, k_cache, v_cache, offsets, ctx_len, mask, depth=None, *, m
 def _tree_attention(s, args, q, out):
     lib = capi.load()
     if out is None:
-        out = q.new_empty(q.shape)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     args.out = out.data_ptr()
     args.out_stride = out.stride(0) if args.n_tokens > 1 else args.n_q_heads * args.head_dim
     need = lib.gptoss_tree_attention_workspace(C.byref(args))
@@ -165,22 +181,36 @@ def cache_commit(k_cache, v_cache, ctx_len, offsets, path, *, max_path, cache_ro
     """Moves the accepted path of each tree into place, in the caches [layers, rows, n_kv_heads, max_seq, head_dim] (or
     without the layers), bf16.  path int32: the accepted drafted tokens of all sequences, ascending within one; sequence b
     has path[offsets[b]:offsets[b+1]], at most max_path.  ``gptoss_cache_commit`` in the C header."""
-    ndim = 4 if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 5
-    dev = _view("k_cache", k_cache, _BF16, ndim)
-    _dense("k_cache", k_cache, _BF16, ndim, dev)
-    _dense("v_cache", v_cache, _BF16, ndim, dev)
+    try:
+        dev, ndim = k_cache.get_device(), k_cache.dim()
+        plain = (
+            k_cache.dtype is _BF16 is v_cache.dtype and ctx_len.dtype is _I32 is offsets.dtype is path.dtype and 4 <= ndim <= 5
+            and ctx_len.dim() == 1 == offsets.dim() == path.dim()
+            and 0 <= dev == v_cache.get_device() == ctx_len.get_device() == offsets.get_device() == path.get_device()
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and ctx_len.is_contiguous() and offsets.is_contiguous()
+            and path.is_contiguous()
+            and (cache_rows is None or cache_rows.dtype is _I32 and cache_rows.dim() == 1 and cache_rows.get_device() == dev
+                 and cache_rows.is_contiguous()))
+    except AttributeError:
+        plain = False
+    if not plain:
+        ndim = 4 if isinstance(k_cache, torch.Tensor) and k_cache.dim() == 4 else 5
+        dev = _view("k_cache", k_cache, _BF16, ndim)
+        _dense("k_cache", k_cache, _BF16, ndim, dev)
+        _dense("v_cache", v_cache, _BF16, ndim, dev)
+        _dense("ctx_len", ctx_len, _I32, 1, dev)
+        _dense("offsets", offsets, _I32, 1, dev)
+        _dense("path", path, _I32, 1, dev)
+        if cache_rows is not None:
+            _dense("cache_rows", cache_rows, _I32, 1, dev)
     shape = k_cache.shape
     if v_cache.shape != shape:
         _bad("k_cache and v_cache must have the same shape")
-    _dense("ctx_len", ctx_len, _I32, 1, dev)
-    _dense("offsets", offsets, _I32, 1, dev)
-    _dense("path", path, _I32, 1, dev)
     n_seqs = ctx_len.shape[0]
     if offsets.shape[0] != n_seqs + 1:
         _bad("offsets needs one more entry than ctx_len")
     rows_at = None
     if cache_rows is not None:
-        _dense("cache_rows", cache_rows, _I32, 1, dev)
         if cache_rows.shape[0] != n_seqs:
             _bad("cache_rows needs an entry per sequence")
         rows_at = cache_rows.data_ptr()
@@ -199,20 +229,32 @@ def lora_apply(x, a, b, ids, y, *, scale=None, out=None, stream=None):
 
     x [T, K] bf16, a [n_adapters, rank, K] bf16, b [n_adapters, n_out, rank] bf16, ids int32 [T], y fp32 [T, n_out], scale
     fp32 [n_adapters].  out: y itself by default (in place).  ``gptoss_lora_apply`` in the C header."""
-    dev = _view("x", x, _BF16, 2)
+    if out is None:
+        out = y
+    try:
+        dev = x.get_device()
+        plain = (
+            x.dtype is _BF16 is a.dtype is b.dtype and ids.dtype is _I32 and y.dtype is _F32 is out.dtype
+            and x.dim() == 2 == y.dim() == out.dim() and a.dim() == 3 == b.dim() and ids.dim() == 1
+            and 0 <= dev == a.get_device() == b.get_device() == ids.get_device() == y.get_device() == out.get_device()
+            and a.is_contiguous() and b.is_contiguous() and ids.is_contiguous()
+            and (scale is None or scale.dtype is _F32 and scale.dim() == 1 and scale.get_device() == dev and scale.is_contiguous()))
+    except AttributeError:
+        plain = False
+    if not plain:
+        dev = _view("x", x, _BF16, 2)
+        _dense("a", a, _BF16, 3, dev)
+        _dense("b", b, _BF16, 3, dev)
+        _dense("ids", ids, _I32, 1, dev)
+        _view("y", y, _F32, 2, dev)
+        _view("out", out, _F32, 2, dev)
+        if scale is not None:
+            _dense("scale", scale, _F32, 1, dev)
     T, K = x.shape
-    _dense("a", a, _BF16, 3, dev)
-    _dense("b", b, _BF16, 3, dev)
     n, rank, a_k = a.shape
     b_n, n_out, b_rank = b.shape
     if a_k != K or b_n != n or b_rank != rank:
         _bad("a must be [n_adapters, rank, K] and b [n_adapters, n_out, rank]")
-    _dense("ids", ids, _I32, 1, dev)
-    _view("y", y, _F32, 2, dev)
-    if out is None:
-        out = y
-    else:
-        _view("out", out, _F32, 2, dev)
     x_stride, y_stride, out_stride = x.stride(), y.stride(), out.stride()
     if y.shape != (T, n_out) or out.shape != y.shape or y_stride[1] != 1 or out_stride[1] != 1:
         _bad("y and out must be [T, n_out] with contiguous rows")
@@ -220,7 +262,6 @@ def lora_apply(x, a, b, ids, y, *, scale=None, out=None, stream=None):
         _bad("ids needs an entry per token, x contiguous rows")
     scale_at = None
     if scale is not None:
-        _dense("scale", scale, _F32, 1, dev)
         if scale.shape[0] != n:
             _bad("scale needs an entry per adapter")
         scale_at = scale.data_ptr()

@@ -498,3 +498,39 @@ def test_routed_block_matches_the_block_on_its_own_routing_and_the_oracle(servin
     with pytest.raises(moe.GptossError):
         blk.forward_routed(1, t_dev, rw, ri, x)  # no such layer
     blk.close()
+
+
+def test_arguments_that_the_python_layer_refuses(serving):
+    """Types, shapes, layouts and devices, one at a time; nothing is launched."""
+    from gptoss_b200 import capi, moe
+
+    def refused(call, good, changes):
+        call(**good)
+        for name, value in changes:
+            with pytest.raises(moe.GptossError) as e:
+                call(**{**good, name: value})
+            assert e.value.code == capi.ERR_BAD_ARG, name
+
+    c = tree_case(serving, [3, 4], [5, 6], seed=1)
+    good = {**c, "cache_rows": ints([0, 1]), "max_nodes": 4, "max_ctx": 6, "window": 3}
+    refused(serving.tree_attention, good, [
+        ("q", c["q"].float()), ("q", c["q"][0]), ("q", c["q"].cpu()), ("q", c["q"].transpose(0, 1)), ("q", None), ("k_cache", c["k_cache"].half()),
+        ("v_cache", c["v_cache"][:, :1]), ("v_cache", c["v_cache"].transpose(1, 2)), ("offsets", c["offsets"].long()), ("offsets", c["offsets"][:2]),
+        ("ctx_len", c["ctx_len"].cpu()), ("mask", c["mask"][:3]), ("mask", c["mask"].float()), ("depth", c["depth"][:2]), ("depth", None),
+        ("depth", c["depth"].long()), ("sinks", c["sinks"][:3]), ("sinks", c["sinks"].bfloat16()), ("cache_rows", ints([0])), ("max_nodes", 300),
+        ("max_nodes", 40), ("out", torch.empty(7, 8, 64, device="cuda")), ("out", torch.empty(6, 8, 64, device="cuda").bfloat16()), ("window", -1),
+        ("scale", 0.0), ("scale", math.nan)])
+    k = torch.zeros(2, 3, 2, 16, 32, dtype=torch.bfloat16, device="cuda")
+    good = dict(k_cache=k, v_cache=k.clone(), ctx_len=ints([1, 2]), offsets=ints([0, 1, 2]), path=ints([0, 1]), max_path=2, cache_rows=ints([0, 2]))
+    refused(serving.cache_commit, good, [
+        ("k_cache", k.float()), ("k_cache", k[0, 0]), ("v_cache", k[:1]), ("v_cache", k.transpose(1, 2)), ("ctx_len", ints([1, 2]).long()),
+        ("offsets", ints([0, 1])), ("path", ints([0, 1]).cpu()), ("cache_rows", ints([0])), ("max_path", -1), ("path", None)])
+    c = lora_case(5, 64, 32, 8, 2)
+    refused(serving.lora_apply, c, [
+        ("x", c["x"].float()), ("x", c["x"][:, :60]), ("x", c["x"][:4]), ("a", c["a"][:1]), ("a", c["a"].transpose(1, 2)), ("b", c["b"][:, :, :4]),
+        ("ids", c["ids"].long()), ("ids", c["ids"][:3]), ("y", c["y"].bfloat16()), ("y", c["y"][:, :24]), ("y", c["y"].t()), ("y", c["y"].cpu()),
+        ("scale", c["scale"][:1]), ("scale", c["scale"].double()), ("out", c["y"][:4]), ("ids", None)])
+    good = dict(logits=torch.zeros(3, 16, device="cuda"), top_k=2, bias=torch.zeros(16, device="cuda"))
+    refused(serving.route_experts, good, [
+        ("logits", good["logits"].half()), ("logits", good["logits"].t()), ("logits", good["logits"].cpu()), ("bias", good["bias"][:8]),
+        ("bias", good["bias"].double()), ("top_k", 0), ("top_k", 9), ("scoring", "relu"), ("n_groups", 3), ("topk_groups", 2), ("group_top", 3)])
