@@ -543,6 +543,11 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
     __syncthreads();
     fetch(step + Ring::kStages - 1);
     const uint8_t *ring = smem_b + (step % Ring::kStages) * Ring::kStageBytes + 16 * c;
+    // a step's products have a sum of their own: the tensor core cuts off what falls below the last bit of a sum, always
+    // towards zero, which over thousands of elements would show (errors of 4.8e-7 of the result instead of 5.6e-8 at 2880)
+    float sum[NJ][4];
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint4 xa = *reinterpret_cast<const uint4 *>(ring + (m0 + row) * Ring::kStride + 64 * h);
@@ -550,10 +555,14 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const uint4 w = *reinterpret_cast<const uint4 *>(ring + (kTileTokens + 8 * (j0 + j) + row) * Ring::kStride + 64 * h);
-        mma_16816(acc[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
-        mma_16816(acc[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
+        mma_16816(sum[j], xa.x, xb.x, xa.y, xb.y, w.x, w.y);
+        mma_16816(sum[j], xa.z, xb.z, xa.w, xb.w, w.z, w.w);
       }
     }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[j][e] += sum[j][e];
   }
   // u by position in the sorted order; what stands beyond the tile's tokens and the adapter's ranks is not read
   float *u = p.u + ((size_t)part * g.T + (t.perm - p.perm) + m0 + row) * (8 * RN) + 8 * j0 + 2 * c;
