@@ -194,7 +194,7 @@ def load() -> C.CDLL:
         "gptoss_serving_status": ([], i32),
         "gptoss_tree_attention_workspace": ([C.POINTER(TreeAttentionArgs)], u64),
         "gptoss_tree_attention": ([C.POINTER(TreeAttentionArgs), vp], i32),
-        "gptoss_cache_commit": ([vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, vp], i32),
+        "gptoss_cache_commit": ([vp, vp, i32, i32, i32, i32, i32, i32, vp, vp, vp, vp, i32, i32, vp], i32),
         "gptoss_lora_workspace": ([C.POINTER(LoraArgs)], u64),
         "gptoss_lora_apply": ([C.POINTER(LoraArgs), vp], i32),
         "gptoss_expert_choice": ([C.POINTER(ExpertChoiceArgs), vp], i32),

@@ -682,6 +682,7 @@ extern "C" int gptoss_lora_apply(const gptoss_lora_args *args, void *stream) {
   const gptoss_lora_args &g = *args;
   if (g.T < 0) return serving_fail(GPTOSS_ERR_BAD_ARG, "negative T");
   if (g.K <= 0 || g.K % 8 || g.n_out <= 0 || g.n_out % 8) return serving_fail(GPTOSS_ERR_BAD_ARG, "K and n_out must be positive multiples of 8");
+  if (g.K > 1 << 30 || g.n_out > 1 << 30) return serving_fail(GPTOSS_ERR_BAD_ARG, "K and n_out go up to 2^30");
   if (g.rank <= 0 || g.rank % 8 || g.rank > GPTOSS_LORA_MAX_RANK)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "rank must be a multiple of 8 up to 128 (pad smaller adapters with zero rows)");
   if (g.n_adapters <= 0 || g.n_adapters > kMaxAdapters) return serving_fail(GPTOSS_ERR_BAD_ARG, "n_adapters must be 1..8192");

@@ -880,7 +880,7 @@ int gptoss_model_accept(gptoss_model *m, int n_seqs, const int *rows_host, const
   m->tree_host.insert(m->tree_host.end(), path_host, path_host + offsets_host[n_seqs]);
   MK(cudaMemcpyAsync(m->tree_dev, m->tree_host.data(), m->tree_host.size() * sizeof(int), cudaMemcpyHostToDevice, m->stream));
   const int rc = gptoss_cache_commit(m->k_cache, m->v_cache, m->c.n_layers, m->max_local, m->c.n_kv_heads, m->S, m->c.head_dim, n_seqs,
-                                     m->tree_dev, m->tree_dev + n_seqs, m->tree_dev + 2 * n_seqs, m->tree_dev + 3 * n_seqs + 1, longest,
+                                     m->tree_dev, m->tree_dev + n_seqs, m->tree_dev + 2 * n_seqs, m->tree_dev + 3 * n_seqs + 1, offsets_host[n_seqs], longest,
                                      m->stream);
   return rc ? m->fail(rc, gptoss_serving_last_error()) : GPTOSS_OK;
 }

@@ -17,22 +17,34 @@ namespace {
 thread_local char g_serving_error[256] = "";
 
 // ---- kernel ---------------------------------------------------------------------------------------------------------
-// One CTA per (sequence, kv head, tile of up to 128 query rows, share of the context).  A query row is a (drafted token,
-// head of the group) pair, so a tree of n tokens with g heads per kv head gives n g rows that all read the same K and V.
-// Per tile of 128 slots:   S = Q K^T   (tcgen05, accumulator in TMEM)
-//                          P = 2^(c S - m), c = scale log2(e), in the registers of one thread per row, bf16 to TMEM
-//                          O += P V    (tcgen05, A operand from TMEM; V as it lies in the cache, K-index outermost)
+// One CTA per (sequence, kv head, pair of query tiles, share of the context).  A query row is a (drafted token, head of the
+// group) pair, so a tree of n tokens with g heads per kv head gives n g rows that all read the same K and V; a query tile
+// has 128 of them.  Per tile of 64 slots:
+//   S = Q K^T             tcgen05, accumulator in TMEM
+//   P = 2^(c S - m)       c = scale log2(e); in the registers of one thread per row, as bf16 back to TMEM in place of S
+//   O += P V              tcgen05, A operand from TMEM, V as it lies in the cache (its N index innermost)
 // m is a running reference, not the running maximum: it moves (and O is rescaled in TMEM) only when the maximum has grown
 // by more than 2^8, so that most tiles leave O alone; P and O stay below 2^8 times their usual range.  P is rounded to
 // bf16, the type of V (both operands of the product have the same type); the denominator adds the unrounded values.
-// S is read into registers at once, which frees its TMEM columns for the next tile's QK^T while this tile's exponentials
-// run; with 256 of the 512 TMEM columns and under 114 KiB of shared memory two CTAs share an SM, so the exponentials of
-// one overlap the products of the other.
+//
+// Two groups of four softmax warps work side by side, so that one's exponentials cover the other's products: on a query tile
+// each (K and V tiles are then fetched once for 256 rows: with 128 rows per CTA the L2 reads alone took 247 of 310 us for
+// 64 sequences x 64 tokens over 4096), or, with up to 128 rows, on every other slot tile of the same rows.  One warp issues
+// the products, one the copies (a ring of four stages).  256 of the 512 TMEM columns and 111 KiB of shared memory: two CTAs,
+// hence 16 softmax warps, per SM.
+// What bounds it (64 x 64 over 4096: 293 us, 0.33 of the tensor peak; floors 97 us products, 70 us HBM): the exponential
+// unit's 16 results per cycle and SM make 172 us of it, and each warp's row of dependent steps (S from TMEM, maximum,
+// exponentials, P to TMEM, hand-over) keeps that unit 55 % busy.  No gain: 128-slot tiles with two rows of S (370 us), four
+// CTAs of 128 rows (312 us), two threads per row (319 us), S in two halves with the products one half ahead (311 us), no
+// maximum unless the tile's sum asks for it (spills: 388 us).
 //
 // Tiles that every row sees whole skip all masking.  In the others (the window's edge, the drafted slots, the end) each
-// thread builds a 128-bit mask of its row.  What a row must not see still goes through P V as 0 * V, so in those tiles
-// the non-finite elements of V are replaced by zeros in shared memory; the epilogue adds them back to the rows that do
-// see them.
+// thread builds a mask of its row, 32 slots to a word.  What a row must not see still goes through P V as 0 * V, so in those
+// tiles the non-finite elements of V are replaced by zeros in shared memory; the epilogue adds them back to the rows that
+// do see them.
+//
+// The context is split when the CTAs would not fill the GPU: up to 8 shares are a cluster and join through distributed
+// shared memory, more go through memory and a second kernel.
 constexpr int kAttRows = 128, kAttTile = 64;      // query rows per tile of them, slots per tile
 constexpr int kAttQBytes = kAttRows * 128;
 constexpr int kAttTileBytes = kAttTile * 128;     // a K or V tile: rows of 128 bytes (head_dim 32: the upper half is zero-filled)
@@ -657,14 +669,15 @@ __global__ void __launch_bounds__(256) tree_merge_kernel(gptoss_tree_attention_a
 }
 
 // One warp per (layer, sequence, kv head).  Row path[j] moves to row j of the drafted rows; path ascends, so path[j] >= j
-// and no row is overwritten before it has been read as long as a batch of rows is read before it is written.
-// A pass of the warp moves R rows of K and of V.
+// and no row is overwritten before it has been read as long as a batch of rows is read before it is written.  A pass of the
+// warp moves R rows of K and of V, 16 bytes per lane.  Bound by the two dependent round trips (path, row) of the few rows
+// that a sequence moves, and with many warps by HBM: 64 sequences x 24 layers move 25 MB in 4.9 us (floor 3.8).
 template <int HD>
 __global__ void __launch_bounds__(128) cache_commit_kernel(uint4 *__restrict__ kc, uint4 *__restrict__ vc, int n_layers,
                                                            int cache_rows, int nkv, int S, int n_seqs,
                                                            const int *__restrict__ rows, const int *__restrict__ ctx_len,
                                                            const int *__restrict__ offsets, const int *__restrict__ path,
-                                                           int max_path) {
+                                                           int n_path, int max_path) {
   constexpr int LPR = HD / 8, R = 32 / LPR;  // lanes (16-byte pieces) per row, rows per pass
   const int lane = threadIdx.x & 31;
   const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -672,7 +685,7 @@ __global__ void __launch_bounds__(128) cache_commit_kernel(uint4 *__restrict__ k
   pdl_launch_dependents();
   if (w >= (long long)n_layers * n_seqs * nkv) return;
   const int kvh = (int)(w % nkv), b = (int)(w / nkv % n_seqs), layer = (int)(w / nkv / n_seqs);
-  const int first = offsets[b], n = min(offsets[b + 1] - first, max_path), ctx = ctx_len[b], row = rows ? rows[b] : b;
+  const int first = offsets[b], n = min(min(offsets[b + 1], n_path) - first, max_path), ctx = ctx_len[b], row = rows ? rows[b] : b;
   if (first < 0 || row < 0 || row >= cache_rows || ctx < 0) return;
   const size_t base = (((size_t)layer * cache_rows + row) * nkv + kvh) * S;
   for (int j0 = 0; j0 < n; j0 += R) {
@@ -856,11 +869,11 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
 
 extern "C" int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_rows, int n_kv_heads, int max_seq,
                                    int head_dim, int n_seqs, const int *rows, const int *ctx_len, const int *offsets,
-                                   const int *path, int max_path, void *stream) {
-  if (n_layers < 0 || n_seqs < 0 || max_path < 0) return serving_fail(GPTOSS_ERR_BAD_ARG, "negative count");
+                                   const int *path, int n_path, int max_path, void *stream) {
+  if (n_layers < 0 || n_seqs < 0 || n_path < 0 || max_path < 0) return serving_fail(GPTOSS_ERR_BAD_ARG, "negative count");
   if (head_dim != 32 && head_dim != 64) return serving_fail(GPTOSS_ERR_BAD_ARG, "head_dim must be 32 or 64");
   if (cache_rows <= 0 || n_kv_heads <= 0 || max_seq <= 0) return serving_fail(GPTOSS_ERR_BAD_ARG, "empty cache");
-  if (n_layers == 0 || n_seqs == 0 || max_path == 0) return GPTOSS_OK;
+  if (n_layers == 0 || n_seqs == 0 || n_path == 0 || max_path == 0) return GPTOSS_OK;
   if (!k_cache || !v_cache || !ctx_len || !offsets || !path) return serving_fail(GPTOSS_ERR_BAD_ARG, "null pointer");
   if (!aligned16(k_cache) || !aligned16(v_cache)) return serving_fail(GPTOSS_ERR_BAD_ARG, "caches must be 16-byte aligned");
   const long long warps = (long long)n_layers * n_seqs * n_kv_heads;
@@ -869,8 +882,8 @@ extern "C" int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, i
   auto *k = static_cast<uint4 *>(k_cache), *v = static_cast<uint4 *>(v_cache);
   const cudaError_t e =
       head_dim == 64 ? launch_chain(cache_commit_kernel<64>, grid, dim3(128), 0, static_cast<cudaStream_t>(stream), k, v, n_layers,
-                                    cache_rows, n_kv_heads, max_seq, n_seqs, rows, ctx_len, offsets, path, max_path)
+                                    cache_rows, n_kv_heads, max_seq, n_seqs, rows, ctx_len, offsets, path, n_path, max_path)
                      : launch_chain(cache_commit_kernel<32>, grid, dim3(128), 0, static_cast<cudaStream_t>(stream), k, v, n_layers,
-                                    cache_rows, n_kv_heads, max_seq, n_seqs, rows, ctx_len, offsets, path, max_path);
+                                    cache_rows, n_kv_heads, max_seq, n_seqs, rows, ctx_len, offsets, path, n_path, max_path);
   return e == cudaSuccess ? GPTOSS_OK : serving_fail(GPTOSS_ERR_CUDA, "cache commit launch", e);
 }

@@ -8,8 +8,10 @@
                       (``MoEBlock.forward_routed`` runs the expert GEMMs on the result)
 
 Each call runs on the device of its tensors, asynchronously on ``stream`` (default: that device's current stream); scratch
-comes from torch's allocator, so calls on different streams and captured graphs have their own.  Errors raise
-``GptossError``.  Nothing is kept between calls.
+comes from torch's allocator, so calls on different streams and captured graphs have their own.  As with torch's own
+operators, a tensor that belongs to another stream than the one it is used on is the caller's to keep alive and to order
+(``record_stream``, ``wait_stream``); what a call returns belongs to the stream it ran on.  Errors raise ``GptossError``.
+Nothing is kept between calls.
 
 The calls are short on the GPU (from 2 us), so their host side counts: what a call is given is looked over in one
 expression, and only where that fails are the arguments gone through one by one for the message; the raw stream handle is
@@ -217,7 +219,7 @@ def cache_commit(k_cache, v_cache, ctx_len, offsets, path, *, max_path, cache_ro
     layers = 1 if ndim == 4 else shape[0]
     rows, nkv, max_seq, hd = shape[-4:]
     _launch(dev, stream, _cache_commit, k_cache.data_ptr(), v_cache.data_ptr(), layers, rows, nkv, max_seq, hd, n_seqs, rows_at,
-            ctx_len.data_ptr(), offsets.data_ptr(), path.data_ptr(), path.shape[0] and max_path)
+            ctx_len.data_ptr(), offsets.data_ptr(), path.data_ptr(), path.shape[0], max_path)
 
 
 def _cache_commit(s, *args):

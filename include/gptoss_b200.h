@@ -325,16 +325,16 @@ int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream);
 
 /* Moves the accepted path of each tree into place: path[offsets[b] + j], ascending, is the drafted token that becomes the
  * j-th new token of sequence b; its K and V move from slot ctx_len[b] + path to slot ctx_len[b] + j in every layer of the
- * caches [n_layers][cache_rows][n_kv_heads][max_seq][head_dim] (bf16).  Other slots are left as they were.  No path is
- * longer than max_path.  Sequences must name distinct cache rows. */
+ * caches [n_layers][cache_rows][n_kv_heads][max_seq][head_dim] (bf16).  Other slots are left as they were.  path has n_path
+ * entries in all, no sequence more than max_path.  Sequences must name distinct cache rows. */
 int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_rows, int n_kv_heads, int max_seq, int head_dim,
-                        int n_seqs, const int *rows, const int *ctx_len, const int *offsets, const int *path, int max_path,
+                        int n_seqs, const int *rows, const int *ctx_len, const int *offsets, const int *path, int n_path, int max_path,
                         void *stream);
 
 /* Adapters beside a shared projection: out[t] = y[t] + scale[a] * B_a (A_a x[t]) with a = ids[t]; a token whose id is
  * outside [0, n_adapters) has no adapter (out[t] = y[t]).  x [T][K] bf16, a [n_adapters][rank][K] bf16,
  * b [n_adapters][n_out][rank] bf16, scale [n_adapters] fp32 or NULL for 1, y and out [T][n_out] fp32; out may be y.
- * Products accumulate in fp32 and the intermediate A x is not rounded.  K and n_out multiples of 8, rank a
+ * Products accumulate in fp32 and the intermediate A x is not rounded.  K and n_out multiples of 8 (up to 2^30), rank a
  * multiple of 8 up to GPTOSS_LORA_MAX_RANK (adapters of lower rank: zero rows of A, zero columns of B), at most 8192
  * adapters.  What adapters that no token uses and rows of x without an adapter hold does not matter. */
 #define GPTOSS_LORA_MAX_RANK 128

@@ -253,6 +253,7 @@ def test_cache_commit_one_layer_without_rows_and_bad_indices(serving):
     want[1, 0, 12] = before[1, 0, 14]  # slot 12 + 9 lies behind the cache: not moved
     assert torch.equal(k, want) and torch.equal(v, -want)
     serving.cache_commit(k, v, ints([4, 99]), ints([0, 0, 1]), ints([1]), max_path=4)
+    serving.cache_commit(k, v, ints([4, 4]), ints([1, 1000, 70]), ints([0]), max_path=64)  # offsets behind the path's end
     serving.cache_commit(k, v, ints([4, 4]), ints([0, 1, 2]), ints([1, 1]), cache_rows=ints([-1, 2]), max_path=4)
     assert torch.equal(k, want) and torch.equal(v, -want)
 

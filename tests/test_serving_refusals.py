@@ -50,20 +50,21 @@ def test_null_arguments(lib):
 
 
 @pytest.mark.parametrize("bad", [
-    (None, A, 1, 2, 2, 16, 64, 1, None, A, A, A, 4), (A, None, 1, 2, 2, 16, 64, 1, None, A, A, A, 4),
-    (A, A, -1, 2, 2, 16, 64, 1, None, A, A, A, 4), (A, A, 1, 0, 2, 16, 64, 1, None, A, A, A, 4),
-    (A, A, 1, 2, 0, 16, 64, 1, None, A, A, A, 4), (A, A, 1, 2, 2, 0, 64, 1, None, A, A, A, 4),
-    (A, A, 1, 2, 2, 16, 48, 1, None, A, A, A, 4), (A, A, 1, 2, 2, 16, 64, -1, None, A, A, A, 4),
-    (A, A, 1, 2, 2, 16, 64, 1, None, None, A, A, 4), (A, A, 1, 2, 2, 16, 64, 1, None, A, None, A, 4),
-    (A, A, 1, 2, 2, 16, 64, 1, None, A, A, None, 4), (A, A, 1, 2, 2, 16, 64, 1, None, A, A, A, -4),
-    (A + 2, A, 1, 2, 2, 16, 64, 1, None, A, A, A, 4)])
+    (None, A, 1, 2, 2, 16, 64, 1, None, A, A, A, 8, 4), (A, None, 1, 2, 2, 16, 64, 1, None, A, A, A, 8, 4),
+    (A, A, -1, 2, 2, 16, 64, 1, None, A, A, A, 8, 4), (A, A, 1, 0, 2, 16, 64, 1, None, A, A, A, 8, 4),
+    (A, A, 1, 2, 0, 16, 64, 1, None, A, A, A, 8, 4), (A, A, 1, 2, 2, 0, 64, 1, None, A, A, A, 8, 4),
+    (A, A, 1, 2, 2, 16, 48, 1, None, A, A, A, 8, 4), (A, A, 1, 2, 2, 16, 64, -1, None, A, A, A, 8, 4),
+    (A, A, 1, 2, 2, 16, 64, 1, None, None, A, A, 8, 4), (A, A, 1, 2, 2, 16, 64, 1, None, A, None, A, 8, 4),
+    (A, A, 1, 2, 2, 16, 64, 1, None, A, A, None, 8, 4), (A, A, 1, 2, 2, 16, 64, 1, None, A, A, A, 8, -4),
+    (A + 2, A, 1, 2, 2, 16, 64, 1, None, A, A, A, 8, 4), (A, A, 1, 2, 2, 16, 64, 1, None, A, A, A, -8, 4)])
 def test_cache_commit_refuses(lib, bad):
     assert lib.gptoss_cache_commit(*bad, None) == capi.ERR_BAD_ARG
 
 
-@pytest.mark.parametrize("empty", [(None, None, 0, 2, 2, 16, 64, 1, None, None, None, None, 4),
-                                   (None, None, 1, 2, 2, 16, 64, 0, None, None, None, None, 4),
-                                   (None, None, 1, 2, 2, 16, 64, 1, None, None, None, None, 0)])
+@pytest.mark.parametrize("empty", [(None, None, 0, 2, 2, 16, 64, 1, None, None, None, None, 8, 4),
+                                   (None, None, 1, 2, 2, 16, 64, 0, None, None, None, None, 8, 4),
+                                   (None, None, 1, 2, 2, 16, 64, 1, None, None, None, None, 8, 0),
+                                   (None, None, 1, 2, 2, 16, 64, 1, None, None, None, None, 0, 4)])
 def test_cache_commit_of_nothing_is_a_no_op(lib, empty):
     assert lib.gptoss_cache_commit(*empty, None) == capi.OK
 
@@ -76,7 +77,7 @@ def lora_args(**kw):
 
 
 @pytest.mark.parametrize("bad", [
-    dict(T=-1), dict(K=0), dict(K=60), dict(n_out=0), dict(n_out=30), dict(rank=0), dict(rank=12), dict(rank=136),
+    dict(T=-1), dict(K=0), dict(K=60), dict(n_out=0), dict(n_out=30), dict(K=(1 << 30) + 8), dict(n_out=(1 << 30) + 8), dict(rank=0), dict(rank=12), dict(rank=136),
     dict(n_adapters=0), dict(n_adapters=8193), dict(out_stride=36, out=A, y=A), dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(y=None), dict(out=None), dict(x=A + 2),
     dict(a=A + 8), dict(b=A + 8), dict(y=A + 4), dict(out=A + 8), dict(x_stride=68), dict(x_stride=56), dict(y_stride=33),
     dict(y_stride=28), dict(out_stride=28), dict(T=33, workspace=None), dict(T=33, workspace=A + 4), dict(T=33, workspace_bytes=4)])
