@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(128) expert_choice_kernel(const __grid_constan
 #pragma unroll
   for (int s = 1; s < SLOTS; ++s) mx = fmaxf(mx, x[s]);
   mx = unordered(__reduce_max_sync(0xffffffffu, ordered(mx)));
-  // Without a bias and groups the scores order like the logits, and only logits closer than 2^-40 (or sigmoids near 1) can
-  // look alike in fp64.
+  // Without a bias and groups the scores order like the logits, and only logits closer than 2^-40, sigmoids near 1 and scores
+  // below e^-700, the end of fp64's range, can look alike in fp64.
   const bool by_logits = !a.bias && a.n_groups == 1 && (softmax || mx <= 16.f);
   float total = 1.f, err = 0x1p-40f;  // sum of the softmax terms; bound on the error of a choice
   if (softmax && !(by_logits && a.renormalize)) {
@@ -269,12 +269,13 @@ __global__ void __launch_bounds__(128) expert_choice_kernel(const __grid_constan
     sort_keys(key);
     const float gap = 2.f * err + 0x1p-19f * largest;  // the slot took the place of three bits of each choice
     float before = INFINITY;
+    const float floor = by_logits ? (softmax ? mx : 0.f) - 700.f : -INFINITY;
     for (int j = 0; j <= a.k; ++j) {  // the one after the last tells whether the last is sure
       const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
       if (top == 0u) break;
       const uint32_t who = __ballot_sync(0xffffffffu, key[0] == top);
       const float v = unordered(top & ~7u);
-      if ((who & (who - 1)) || !(before - v > gap)) sure = false;
+      if ((who & (who - 1)) || !(before - v > gap) || (j < a.k && v < floor)) sure = false;
       before = v;
       if (lane == j) my_e = 32 * (int)(top & 7u) + __ffs(who) - 1;
       if (key[0] == top) {

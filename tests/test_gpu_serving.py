@@ -430,6 +430,17 @@ def test_route_experts_scores_that_all_but_vanish(serving, scoring):
 
 
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [True, False])
+def test_route_experts_scores_below_the_range_of_fp64_tie(serving, scoring, renorm):
+    logits = torch.full((3, 40), -2000.0, device="cuda")
+    logits[0, 1], logits[0, 7], logits[0, 9] = 0.0, -900.0, -800.0   # all but the first score 0 in fp64
+    logits[1, 3], logits[1, 5], logits[1, 6] = 0.0, -690.0, -600.0   # these do not
+    logits[2] -= torch.arange(40, device="cuda").flip(0)
+    check_route(serving, logits, 4, scoring=scoring, renormalize=renorm)
+    check_route(serving, logits[:, :2], 1, scoring=scoring, renormalize=renorm)
+
+
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 def test_route_experts_many_random_rows(serving, scoring):
     """Against the plain operator in 64 bits on the GPU: 20000 rows, so that near ties of every kind occur."""
     logits = torch.randn(20000, 256, generator=gen(13), device="cuda") * 1.5
