@@ -5,7 +5,9 @@ There is no CPU fallback: if the library has not been built, ``load()`` raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import subprocess
+import sysconfig
 from pathlib import Path
 
 import os
@@ -19,6 +21,9 @@ SOURCES = ["routing.cu", "router.cu", "grouped_gemm.cu", "grouped_gemm_pair.cu",
 HEADERS = ["common.cuh", "kernels.cuh", "serving.cuh", "tcgen05.cuh", "gemm_tile.cuh", "../../include/gptoss_b200.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "--threads", "4"]
+# the serving operators' binding to torch tensors (serving.py), a Python module
+TORCH_LIB_PATH = CSRC / "_serving_torch.so"
+TORCH_SOURCES = ["serving_torch.cpp"]
 
 OK, ERR_BAD_ARG, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED, ERR_STATE = range(6)
 WIRE_F32, WIRE_BF16 = 0, 1
@@ -86,25 +91,40 @@ class ExpertChoiceArgs(C.Structure):
                [("weight_scale", C.c_float)]
 
 
+def _stale(path, sources) -> bool:
+    return not path.exists() or any((CSRC / f).stat().st_mtime > path.stat().st_mtime for f in sources)
+
+
+def _lib_stale() -> bool:
+    return _stale(LIB_PATH, SOURCES + HEADERS)
+
+
+def _torch_lib_stale() -> bool:
+    return _stale(TORCH_LIB_PATH, TORCH_SOURCES + HEADERS[-1:])
+
+
 def needs_build() -> bool:
-    if not LIB_PATH.exists():
-        return True
-    t = LIB_PATH.stat().st_mtime
-    return any((CSRC / f).stat().st_mtime > t for f in SOURCES + HEADERS)
+    return _lib_stale() or _torch_lib_stale()
+
+
+def _nvcc(args):
+    r = subprocess.run(["nvcc", *args], cwd=CSRC, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"nvcc failed:\n{r.stdout}")
+    return r.stdout
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the library for sm_100a with nvcc (works without a GPU)."""
-    if not force and not needs_build():
-        return LIB_PATH
-    cmd = ["nvcc", *NVCC_FLAGS, "-o", str(LIB_PATH), *SOURCES]
-    if verbose:
-        cmd[1:1] = ["-Xptxas", "-v"]
-    r = subprocess.run(cmd, cwd=CSRC, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed:\n{r.stdout}")
-    if verbose:
-        print(r.stdout)
+    """Compiles the library for sm_100a and the torch binding with nvcc (works without a GPU)."""
+    if force or _lib_stale():
+        out = _nvcc([*(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-o", str(LIB_PATH), *SOURCES])
+        if verbose:
+            print(out)
+    if force or _torch_lib_stale():
+        torch_dir = Path(importlib.util.find_spec("torch").origin).parent
+        _nvcc(["-x", "c++", "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"],
+               "-I", str(torch_dir / "include"), "-o", str(TORCH_LIB_PATH), *TORCH_SOURCES, "-L", str(torch_dir / "lib"),
+               "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda"])
     return LIB_PATH
 
 

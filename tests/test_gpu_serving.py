@@ -546,3 +546,40 @@ def test_arguments_that_the_python_layer_refuses(serving):
     refused(serving.route_experts, good, [
         ("logits", good["logits"].half()), ("logits", good["logits"].t()), ("logits", good["logits"].cpu()), ("bias", good["bias"][:8]),
         ("bias", good["bias"].double()), ("top_k", 0), ("top_k", 9), ("scoring", "relu"), ("n_groups", 3), ("topk_groups", 2), ("group_top", 3)])
+
+
+def test_python_layer_refuses_numbers(serving):
+    """Numbers of the wrong kind or beyond 32 bits."""
+    from gptoss_b200 import moe
+    c = tree_case(serving, [3, 4], [5, 6], seed=2)
+    for bad in (1 << 31, -(1 << 31), 1 << 40):
+        with pytest.raises(moe.GptossError):
+            serving.tree_attention(**c, max_nodes=bad, max_ctx=6)
+    with pytest.raises(OverflowError):
+        serving.tree_attention(**c, max_nodes=4, max_ctx=1 << 70)
+    for name, value in (("max_nodes", 4.5), ("max_nodes", None), ("max_ctx", "6"), ("scale", "1")):
+        with pytest.raises(TypeError):
+            serving.tree_attention(**{**c, "max_nodes": 4, "max_ctx": 6, name: value})
+    logits = torch.zeros(2, 8, device="cuda")
+    with pytest.raises(moe.GptossError):
+        serving.route_experts(logits, 2, scoring="relu")
+    with pytest.raises(TypeError):
+        serving.route_experts(logits, 2, weight_scale=None)
+    got = serving.tree_attention(**c, max_nodes=np.int64(4), max_ctx=np.int32(6), scale=np.float32(0.125))
+    assert torch.equal(got, serving.tree_attention(**c, max_nodes=4, max_ctx=6))
+
+
+def test_what_a_call_returns(serving):
+    """The given output itself, y in place, and on a side stream the same results."""
+    c = tree_case(serving, [3, 4], [5, 6], seed=3)
+    out = torch.empty_like(c["q"])
+    assert serving.tree_attention(**c, max_nodes=4, max_ctx=6, out=out) is out
+    lo = lora_case(40, 64, 32, 8, 2)
+    want = serving.lora_apply(**{**lo, "out": torch.empty_like(lo["y"])})
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    y = lo["y"].clone()
+    side.wait_stream(torch.cuda.current_stream())
+    assert serving.lora_apply(**{**lo, "y": y}, stream=side) is y
+    side.synchronize()
+    assert torch.equal(y, want)
