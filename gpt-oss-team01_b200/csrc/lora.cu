@@ -27,12 +27,13 @@ constexpr int kClusterCtas = 8, kLoraWarps = 8;
 constexpr int kWideSplits = 2;        // parts of K with many tiles
 constexpr int kWideTokens = 2048;     // from here on a batch counts as many tiles
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
+constexpr int kColBlock = 128;        // outputs of a tile that go to one CTA as a whole, with many tiles
 constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all
 
 struct LoraPlan {
-  int4 *tiles;   // {adapter or -1, first position in perm, tokens, 0}
+  int4 *tiles;   // {adapter or -1, first position in perm, tokens, cost of the tiles before}
   int *perm;     // tokens ordered by adapter
-  int *n_tiles;
+  int *n_tiles;  // number of tiles, cost of them all
   float *u;       // many tiles: [kWideSplits][T][rank up to 16, 32, 64 or 128]
   int max_tiles;
   bool wide;      // many tiles
@@ -45,6 +46,9 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// What a tile costs, for cutting the work of many tiles into equal shares: its 16-row blocks and the start.
+__host__ __device__ __forceinline__ int tile_cost(int tokens) { return (tokens + 15) / 16 + 1; }
+
 // bin of token t: its adapter, n for a token without one, -1 behind the last token
 __device__ __forceinline__ int bin_of(const int *__restrict__ ids, int t, int T, int n) {
   if (t >= T) return -1;
@@ -55,7 +59,7 @@ __device__ __forceinline__ int bin_of(const int *__restrict__ ids, int t, int T,
 // One block.  Bins 0..n-1 are the adapters, bin n the tokens without one.
 __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__ ids, int T, int n, LoraPlan p) {
   extern __shared__ int bin_s[];  // [n + 1] counts, then cursors
-  __shared__ int warp_tok[32], warp_tile[32];
+  __shared__ int warp_tok[32], warp_tile[32], warp_cost[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i <= n; i += 1024) bin_s[i] = 0;
   __syncthreads();
@@ -77,27 +81,32 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   // exclusive prefix of the counts (positions) and of the tile counts; a thread owns `per` consecutive bins
   const int bins = p.skip_idle ? n : n + 1;  // bins that need tiles
   const int per = (n + 1 + 1023) / 1024, b0 = tid * per, b1 = min(b0 + per, n + 1);
-  int tok = 0, til = 0;
+  int tok = 0, til = 0, cost = 0;
   for (int b = b0; b < b1; ++b) {
-    tok += bin_s[b];
-    if (b < bins) til += (bin_s[b] + kTileTokens - 1) / kTileTokens;
+    const int c = bin_s[b], rest = c % kTileTokens;
+    tok += c;
+    if (b < bins) til += (c + kTileTokens - 1) / kTileTokens, cost += c / kTileTokens * tile_cost(kTileTokens) + (rest ? tile_cost(rest) : 0);
   }
-  int tok_in = tok, til_in = til;
+  int tok_in = tok, til_in = til, cost_in = cost;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int x = __shfl_up_sync(0xffffffffu, tok_in, o), y = __shfl_up_sync(0xffffffffu, til_in, o);
-    if (lane >= o) tok_in += x, til_in += y;
+    const int z = __shfl_up_sync(0xffffffffu, cost_in, o);
+    if (lane >= o) tok_in += x, til_in += y, cost_in += z;
   }
-  if (lane == 31) warp_tok[warp] = tok_in, warp_tile[warp] = til_in;
+  if (lane == 31) warp_tok[warp] = tok_in, warp_tile[warp] = til_in, warp_cost[warp] = cost_in;
   __syncthreads();
-  int tok_at = tok_in - tok, til_at = til_in - til;
-  for (int w = 0; w < warp; ++w) tok_at += warp_tok[w], til_at += warp_tile[w];
-  if (tid == 1023) *p.n_tiles = til_at + til;
+  int tok_at = tok_in - tok, til_at = til_in - til, cost_at = cost_in - cost;
+  for (int w = 0; w < warp; ++w) tok_at += warp_tok[w], til_at += warp_tile[w], cost_at += warp_cost[w];
+  if (tid == 1023) p.n_tiles[0] = til_at + til, p.n_tiles[1] = cost_at + cost;
   for (int b = b0; b < b1; ++b) {
     const int c = bin_s[b];
     bin_s[b] = tok_at;
     if (b < bins)
-      for (int j = 0; j < c; j += kTileTokens) p.tiles[til_at++] = make_int4(b < n ? b : -1, tok_at + j, min(kTileTokens, c - j), 0);
+      for (int j = 0; j < c; j += kTileTokens) {
+        p.tiles[til_at++] = make_int4(b < n ? b : -1, tok_at + j, min(kTileTokens, c - j), cost_at);
+        cost_at += tile_cost(min(kTileTokens, c - j));
+      }
     tok_at += c;
   }
   __syncthreads();
@@ -421,11 +430,25 @@ __device__ __forceinline__ void output_range(int n_out, int part, int parts, int
   const int per = (n_out + 16 * parts - 1) / (16 * parts) * 16;
   first = part * per, end = min(first + per, n_out);
 }
-// Tokens without an adapter: out = y.
+// Tokens without an adapter: out = y.  Eight 16-byte pieces per thread are under way at a time (one: 1 us per 32 outputs of
+// the tile's rows).
 __device__ __forceinline__ void copy_rows(const gptoss_lora_args &g, const Work &k, int first, int end) {
-  for (int n = first + 16 * k.k + 4 * k.c; n < end; n += 16 * k.wn) {
-    if (k.in0) *reinterpret_cast<float4 *>(g.out + k.t0 * g.out_stride + n) = *reinterpret_cast<const float4 *>(g.y + k.t0 * g.y_stride + n);
-    if (k.in1) *reinterpret_cast<float4 *>(g.out + k.t1 * g.out_stride + n) = *reinterpret_cast<const float4 *>(g.y + k.t1 * g.y_stride + n);
+  const float *y0 = g.y + k.t0 * g.y_stride, *y1 = g.y + k.t1 * g.y_stride;
+  float *o0 = g.out + k.t0 * g.out_stride, *o1 = g.out + k.t1 * g.out_stride;
+  for (int n0 = first + 16 * k.k + 4 * k.c; n0 < end; n0 += 4 * 16 * k.wn) {
+    float4 a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 16 * k.wn * i;
+      if (n < end && k.in0) a[i] = *reinterpret_cast<const float4 *>(y0 + n);
+      if (n < end && k.in1) b[i] = *reinterpret_cast<const float4 *>(y1 + n);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int n = n0 + 16 * k.wn * i;
+      if (n < end && k.in0) *reinterpret_cast<float4 *>(o0 + n) = a[i];
+      if (n < end && k.in1) *reinterpret_cast<float4 *>(o1 + n) = b[i];
+    }
   }
 }
 
@@ -592,21 +615,43 @@ __device__ __forceinline__ void wide_expand(const gptoss_lora_args &g, const Lor
   __syncthreads();
   expand.run(u_s);
 }
+// Each CTA takes an equal share (by cost) of the tiles' blocks of 128 outputs, tile after tile: it starts on at most a few
+// tiles, and the CTAs stand at different columns at any time.
 template <int RN>
-__global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_expand_kernel(gptoss_lora_args g, LoraPlan p, int parts) {
+__global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_expand_kernel(gptoss_lora_args g, LoraPlan p) {
   extern __shared__ __align__(16) float smem_f[];
   float *u_s = smem_f, *y_s = u_s + kTileTokens * 8 * RN;
   pdl_wait();
   pdl_launch_dependents();
-  const Work k(find_tile(g, p, false, blockIdx.x / parts));
-  int n_first, n_end;
-  output_range(g.n_out, blockIdx.x % parts, parts, n_first, n_end);
-  if (k.t.count == 0 || k.t.adapter < 0) {
-    copy_rows(g, k, n_first, n_end);
-  } else if (k.wm == 4) {
-    wide_expand<RN, true>(g, p, k, u_s, y_s, n_first, n_end);
-  } else {
-    wide_expand<RN, false>(g, p, k, u_s, y_s, n_first, n_end);
+  const int n = p.n_tiles[0];
+  const long long blocks = (g.n_out + kColBlock - 1) / kColBlock, all = blocks * p.n_tiles[1];
+  const long long lo = all * blockIdx.x / gridDim.x, hi = all * (blockIdx.x + 1) / gridDim.x;
+  if (lo >= hi) return;
+  // block j of a tile stands at blocks * (cost before it) + j * (its cost); the last tile that starts at lo or before:
+  int tile = 0;
+  for (int len = n; len > 1;) {
+    const int step = (len + 32 * kLoraWarps - 1) / (32 * kLoraWarps), at = threadIdx.x * step;
+    const int ahead = __syncthreads_count(at < len && blocks * p.tiles[tile + at].w <= lo) - 1;
+    tile += ahead * step, len = min(step, len - ahead * step);
+  }
+  for (; tile < n; ++tile) {
+    const int4 d = p.tiles[tile];
+    const long long at = blocks * d.w;
+    if (at >= hi) break;
+    const int cost = tile_cost(d.z);
+    const int first = at >= lo ? 0 : (int)((lo - at + cost - 1) / cost), end = (int)min(blocks, (hi - at + cost - 1) / cost);
+    if (first >= end) continue;
+    const Work k(Tile{d.x, d.z, 0u, p.perm + d.y});
+    const int n_first = first * kColBlock, n_end = min(end * kColBlock, g.n_out);
+    if (d.x < 0) {
+      copy_rows(g, k, n_first, n_end);
+    } else if (k.wm == 4) {
+      wide_expand<RN, true>(g, p, k, u_s, y_s, n_first, n_end);
+    } else {
+      wide_expand<RN, false>(g, p, k, u_s, y_s, n_first, n_end);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();  // u and the ring are free for the next tile
   }
 }
 
@@ -631,7 +676,7 @@ LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
   };
   p.tiles = reinterpret_cast<int4 *>(take((uint64_t)p.max_tiles * sizeof(int4)));
   p.perm = reinterpret_cast<int *>(take((uint64_t)g.T * sizeof(int)));
-  p.n_tiles = reinterpret_cast<int *>(take(sizeof(int)));
+  p.n_tiles = reinterpret_cast<int *>(take(2 * sizeof(int)));
   p.wide = g.T >= kWideTokens;
   if (p.wide) p.u = reinterpret_cast<float *>(take((uint64_t)kWideSplits * g.T * padded_rank(g.rank) * sizeof(float)));
   return p;
@@ -655,13 +700,9 @@ cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, bool direc
   constexpr int shrink = ShrinkRing<RN>::kStages * ShrinkRing<RN>::kStageBytes;
   if ((e = allow_smem(lora_shrink_kernel<RN>, shrink)) != cudaSuccess || (e = allow_smem(lora_expand_kernel<RN>, expand)) != cudaSuccess) return e;
   if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * kWideSplits), block, shrink, s, g, p)) != cudaSuccess) return e;
-  // parts of the outputs: some four rounds of two CTAs per SM, of at least 256 outputs each.  More start-ups (tile, tokens, u
-  // in three terms: 5 us) cost time, fewer parts scatter the rows under way: 8192 tokens x 5120 outputs of rank 64 take
-  // 157 / 135 / 121 / 120 / 124 / 128 us with 2 / 4 / 8 / 10 / 16 / 20 parts.
-  const int tiles = g.T / kTileTokens;
-  int parts = (8 * kSmCountFallback + tiles - 1) / tiles;
-  parts = parts > (g.n_out + 255) / 256 ? (g.n_out + 255) / 256 : parts;
-  return launch_chain(lora_expand_kernel<RN>, dim3(p.max_tiles * parts), block, expand, s, g, p, parts);
+  int device = 0, sms = kSmCountFallback;
+  if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+  return launch_chain(lora_expand_kernel<RN>, dim3((RN <= 8 ? 2 : 1) * sms), block, expand, s, g, p);
 }
 
 }  // namespace
