@@ -7,8 +7,8 @@
 // innermost; which element of a row stands where in that index is free, as long as both operands agree, so every thread
 // loads consecutive elements).  tcgen05's M = 128 tiles would be mostly empty: a decode step has a handful of tokens per
 // adapter.
-//   lora_sort_kernel  more than 32 tokens: counting sort of the tokens by adapter, list of tiles of up to 64 tokens
-//                     (up to 32 tokens the other kernel finds each other's tokens with one warp vote)
+//   lora_sort_kernel  more than 512 tokens (or 1023 adapters): counting sort of the tokens by adapter, list of tiles of up to 64 tokens
+//                     (with fewer each CTA of the next kernel finds its tile's tokens itself)
 //   lora_kernel       a cluster of 8 CTAs per tile: each computes u = A x over an eighth of K, the partial sums meet in
 //                     distributed shared memory, and each CTA adds s B u to an eighth of the outputs.  One launch, no
 //                     intermediate in memory.
@@ -21,7 +21,8 @@ namespace gptoss {
 namespace {
 
 constexpr int kTileTokens = 64;       // tokens of a tile: 4 tiles of 16 rows
-constexpr int kDirectTokens = 32;     // up to here a warp vote replaces the sort
+constexpr int kDirectTokens = 32;     // up to here a warp vote replaces the sort,
+constexpr int kBlockTokens = 512, kBlockBins = 1024;  // and up to here, with fewer adapters, each CTA finds its tile by itself
 constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
 constexpr int kWideSplits = 2;        // parts of K with many tiles
@@ -48,6 +49,10 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 
 // What a tile costs, for cutting the work of many tiles into equal shares: its 16-row blocks and the start.
 __host__ __device__ __forceinline__ int tile_cost(int tokens) { return (tokens + 15) / 16 + 1; }
+
+__host__ __device__ __forceinline__ bool sorts(const gptoss_lora_args &g) {
+  return g.T > kBlockTokens || (g.T > kDirectTokens && g.n_adapters >= kBlockBins);
+}
 
 // bin of token t: its adapter, n for a token without one, -1 behind the last token
 __device__ __forceinline__ int bin_of(const int *__restrict__ ids, int t, int T, int n) {
@@ -128,26 +133,93 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   }
 }
 
-// The tokens of a tile, whichever way they were found.  Called by whole warps.
+// The tokens of a tile, whichever way they were found.  Called by whole CTAs.
 struct Tile {
   int adapter, count;   // count 0: nothing to do
-  uint32_t members;     // direct: the tokens' bits
-  const int *perm;      // sorted: the tokens
+  uint32_t members;     // up to 32 tokens: their bits
+  const int *perm;      // more: the tokens
   __device__ __forceinline__ int token(int i) const { return perm ? perm[i] : (int)__fns(members, 0, i + 1); }
 };
-__device__ __forceinline__ Tile find_tile(const gptoss_lora_args &g, const LoraPlan &p, bool direct, int tile) {
+__device__ __forceinline__ Tile vote_tile(const gptoss_lora_args &g, bool skip_idle, int tile) {
   Tile t{-1, 0, 0u, nullptr};
-  if (direct) {
-    const int lane = threadIdx.x & 31;
-    int id = lane < g.T ? g.ids[lane] : -2;
-    if (lane < g.T && (id < 0 || id >= g.n_adapters)) id = -1;
-    t.members = __shfl_sync(0xffffffffu, __match_any_sync(0xffffffffu, id), tile);
-    t.adapter = __shfl_sync(0xffffffffu, id, tile);
-    if (tile == __ffs(t.members) - 1 && !(t.adapter < 0 && p.skip_idle)) t.count = __popc(t.members);
-  } else if (tile < *p.n_tiles) {
+  const int lane = threadIdx.x & 31;
+  int id = lane < g.T ? g.ids[lane] : -2;
+  if (lane < g.T && (id < 0 || id >= g.n_adapters)) id = -1;
+  t.members = __shfl_sync(0xffffffffu, __match_any_sync(0xffffffffu, id), tile);
+  t.adapter = __shfl_sync(0xffffffffu, id, tile);
+  if (tile == __ffs(t.members) - 1 && !(t.adapter < 0 && skip_idle)) t.count = __popc(t.members);
+  return t;
+}
+__device__ __forceinline__ Tile sorted_tile(const LoraPlan &p, int tile) {
+  Tile t{-1, 0, 0u, nullptr};
+  if (tile < *p.n_tiles) {
     const int4 d = p.tiles[tile];
     t.adapter = d.x, t.count = d.z, t.perm = p.perm + d.y;
   }
+  return t;
+}
+// A tile found by each CTA for itself (400 tokens of 16 adapters, rank 16: 12.5 us, 14.5 with the sorting kernel; 512 of 64:
+// 16.8 and 18.6; with room for 1024 tokens it is the sorting kernel that is faster, 24.9 and 23.8): counts per adapter in shared memory, the adapter whose tiles include the wanted one by
+// a prefix sum, that adapter's tokens in their order by ballots.
+struct BlockGroup {
+  int bin[kBlockBins], perm[kTileTokens], warp_sum[kLoraWarps];
+  uint32_t members[kBlockTokens / 32];
+  int adapter, chunk;
+};
+__device__ __forceinline__ Tile block_tile(const gptoss_lora_args &g, bool skip_idle, int tile, BlockGroup &s) {
+  constexpr int kThreads = 32 * kLoraWarps, kPer = kBlockTokens / kThreads;
+  static_assert(kBlockBins == 4 * kThreads, "a thread has four bins");
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, n = g.n_adapters;
+  int bin[kPer];
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) bin[c] = bin_of(g.ids, tid + kThreads * c, g.T, n);
+  reinterpret_cast<int4 *>(s.bin)[tid] = make_int4(0, 0, 0, 0);
+  if (tid == 0) s.adapter = -1;
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < kPer; ++c)
+    if (bin[c] >= 0) atomicAdd(&s.bin[bin[c]], 1);
+  __syncthreads();
+  const int4 mine = reinterpret_cast<const int4 *>(s.bin)[tid];
+  int tiles[4] = {mine.x, mine.y, mine.z, mine.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) tiles[i] = skip_idle && 4 * tid + i == n ? 0 : (tiles[i] + kTileTokens - 1) / kTileTokens;
+  const int sum = tiles[0] + tiles[1] + tiles[2] + tiles[3];
+  int at = sum;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, at, o);
+    if (lane >= o) at += v;
+  }
+  if (lane == 31) s.warp_sum[warp] = at;
+  __syncthreads();
+  at -= sum;
+  for (int w = 0; w < warp; ++w) at += s.warp_sum[w];
+  if (tile >= at && tile < at + sum) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (tile >= at && tile < at + tiles[i]) s.adapter = 4 * tid + i, s.chunk = tile - at;
+      at += tiles[i];
+    }
+  }
+  __syncthreads();
+  Tile t{-1, 0, 0u, s.perm};
+  const int adapter = s.adapter, first = s.chunk * kTileTokens;
+  if (adapter < 0) return t;  // fewer tiles than that
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) {
+    const uint32_t members = __ballot_sync(0xffffffffu, bin[c] == adapter);
+    if (lane == 0) s.members[kLoraWarps * c + warp] = members;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < kPer; ++c) {
+    int rank = __popc(s.members[kLoraWarps * c + warp] & ((1u << lane) - 1u)) - first;
+    for (int w = 0; w < kLoraWarps * c + warp; ++w) rank += __popc(s.members[w]);
+    if (bin[c] == adapter && rank >= 0 && rank < kTileTokens) s.perm[rank] = tid + kThreads * c;
+  }
+  t.adapter = adapter < n ? adapter : -1, t.count = min(kTileTokens, s.bin[adapter] - first);
+  __syncthreads();
   return t;
 }
 
@@ -456,14 +528,18 @@ __device__ __forceinline__ void copy_rows(const gptoss_lora_args &g, const Work 
 // in the order of the CTAs, each CTA then takes an eighth of the outputs.  RN: tiles of 8 ranks, at least rank / 8.
 template <int RN>
 __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1)
-    lora_kernel(gptoss_lora_args g, LoraPlan p, bool direct) {
+    lora_kernel(gptoss_lora_args g, LoraPlan p) {
   extern __shared__ __align__(16) float smem_f[];
+  __shared__ __align__(16) BlockGroup group_s;
   float *acc_s = smem_f;                          // [8 warps][16][8 RN], of which the first [tokens][8 RN] become the sums
   float *u_s = acc_s + kTileTokens * 8 * RN;      // u, where the last warps' sums were
   float *y_s = acc_s + kLoraWarps * 16 * 8 * RN;  // ring
   const int cta = blockIdx.x % kClusterCtas;
   pdl_wait();
-  const Work k(find_tile(g, p, direct, blockIdx.x / kClusterCtas));
+  const int tile = blockIdx.x / kClusterCtas;
+  const Work k(g.T <= kDirectTokens ? vote_tile(g, p.skip_idle, tile)
+               : sorts(g)             ? sorted_tile(p, tile)
+                                      : block_tile(g, p.skip_idle, tile, group_s));
   int n_first, n_end;
   output_range(g.n_out, cta, kClusterCtas, n_first, n_end);
   if (k.t.count == 0 || k.t.adapter < 0) {  // the whole cluster
@@ -528,7 +604,7 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
   extern __shared__ __align__(16) uint8_t smem_b[];
   pdl_wait();
   pdl_launch_dependents();
-  const Tile t = find_tile(g, p, false, blockIdx.x / kWideSplits);
+  const Tile t = sorted_tile(p, blockIdx.x / kWideSplits);
   if (t.count == 0 || t.adapter < 0) return;
   const int part = blockIdx.x % kWideSplits;
   const int steps_all = (g.K + kShrinkStep - 1) / kShrinkStep, per = (steps_all + kWideSplits - 1) / kWideSplits;
@@ -669,6 +745,7 @@ LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
   // every adapter with tokens ends with one tile that is not full
   const long long full = g.T / kTileTokens, bins = (long long)g.n_adapters + 1;
   p.max_tiles = (int)(full + (bins < g.T ? bins : g.T));
+  if (!sorts(g)) return p;
   auto take = [&](uint64_t n) {
     char *here = static_cast<char *>(g.workspace) + bytes;
     bytes += (n + 255) & ~255ull;
@@ -687,13 +764,13 @@ cudaError_t allow_smem(K kernel, int bytes) {
   return bytes > 48 * 1024 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) : cudaSuccess;
 }
 template <int RN>
-cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, bool direct, cudaStream_t s) {
+cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, cudaStream_t s) {
   constexpr int acc = kLoraWarps * 16 * 8 * RN * (int)sizeof(float), ring = Expand<RN, false>::kRingBytes;
   const dim3 block(32 * kLoraWarps);
   cudaError_t e;
   if (!p.wide) {
     if ((e = allow_smem(lora_kernel<RN>, acc + ring)) != cudaSuccess) return e;
-    return launch_chain(lora_kernel<RN>, dim3(p.max_tiles * kClusterCtas), block, acc + ring, s, g, p, direct);
+    return launch_chain(lora_kernel<RN>, dim3(p.max_tiles * kClusterCtas), block, acc + ring, s, g, p);
   }
   constexpr int wide_ring = Expand<RN, true>::kRingBytes > ring ? Expand<RN, true>::kRingBytes : ring;
   constexpr int expand = kTileTokens * 8 * RN * (int)sizeof(float) + wide_ring;
@@ -741,13 +818,12 @@ extern "C" int gptoss_lora_apply(const gptoss_lora_args *args, void *stream) {
   if (need && (!g.workspace || !aligned16(g.workspace) || g.workspace_bytes < need))
     return serving_fail(GPTOSS_ERR_BAD_ARG, "workspace missing, misaligned or below gptoss_lora_workspace()");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool direct = g.T <= kDirectTokens;
   cudaError_t e = cudaSuccess;
-  if (!direct) e = launch_chain(lora_sort_kernel, dim3(1), dim3(1024), (g.n_adapters + 1) * sizeof(int), s, g.ids, g.T, g.n_adapters, p);
+  if (sorts(g)) e = launch_chain(lora_sort_kernel, dim3(1), dim3(1024), (g.n_adapters + 1) * sizeof(int), s, g.ids, g.T, g.n_adapters, p);
   if (e == cudaSuccess)
-    e = g.rank <= 16   ? launch_lora<2>(g, p, direct, s)
-        : g.rank <= 32 ? launch_lora<4>(g, p, direct, s)
-        : g.rank <= 64 ? launch_lora<8>(g, p, direct, s)
-                       : launch_lora<16>(g, p, direct, s);
+    e = g.rank <= 16   ? launch_lora<2>(g, p, s)
+        : g.rank <= 32 ? launch_lora<4>(g, p, s)
+        : g.rank <= 64 ? launch_lora<8>(g, p, s)
+                       : launch_lora<16>(g, p, s);
   return e == cudaSuccess ? GPTOSS_OK : serving_fail(GPTOSS_ERR_CUDA, "adapter launch", e);
 }

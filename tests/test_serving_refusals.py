@@ -80,7 +80,7 @@ def lora_args(**kw):
     dict(T=-1), dict(K=0), dict(K=60), dict(n_out=0), dict(n_out=30), dict(K=(1 << 30) + 8), dict(n_out=(1 << 30) + 8), dict(rank=0), dict(rank=12), dict(rank=136),
     dict(n_adapters=0), dict(n_adapters=8193), dict(out_stride=36, out=A, y=A), dict(x=None), dict(a=None), dict(b=None), dict(ids=None), dict(y=None), dict(out=None), dict(x=A + 2),
     dict(a=A + 8), dict(b=A + 8), dict(y=A + 4), dict(out=A + 8), dict(x_stride=68), dict(x_stride=56), dict(y_stride=33),
-    dict(y_stride=28), dict(out_stride=28), dict(T=33, workspace=None), dict(T=33, workspace=A + 4), dict(T=33, workspace_bytes=4)])
+    dict(y_stride=28), dict(out_stride=28), dict(T=513, workspace=None), dict(T=513, workspace=A + 4), dict(T=513, workspace_bytes=4)])
 def test_lora_refuses(lib, bad):
     assert lib.gptoss_lora_apply(C.byref(lora_args(**bad)), None) == capi.ERR_BAD_ARG
     assert lib.gptoss_serving_last_error()
