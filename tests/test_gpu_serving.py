@@ -279,6 +279,13 @@ def check_lora(serving, c, **kw):
     return got
 
 
+@pytest.mark.parametrize("hd", [32, 64])
+@pytest.mark.parametrize("nodes,ctx", [([5], [20011]), ([1], [700]), ([130], [9000]), ([3, 2], [15000, 40])])
+def test_tree_attention_many_shares(serving, nodes, ctx, hd):
+    """One kv head: the context is cut into up to as many shares as the GPU has room for."""
+    check_tree(serving, tree_case(serving, nodes, ctx, 2, 1, hd, seed=hd + ctx[0]), max(nodes), max(ctx))
+
+
 @pytest.mark.parametrize("T,K,n_out,rank,n", [
     (1, 2880, 5120, 16, 3), (1, 8, 8, 8, 1), (2, 64, 96, 8, 1), (3, 2880, 2880, 24, 5), (16, 72, 40, 128, 2), (17, 520, 1000, 40, 3),
     (31, 4096, 2880, 64, 40), (64, 2880, 5120, 32, 7), (257, 4096, 2880, 32, 48), (1000, 136, 264, 16, 1), (1025, 200, 2312, 8, 300),
