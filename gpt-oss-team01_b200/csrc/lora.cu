@@ -12,7 +12,7 @@
 //   lora_kernel       a cluster of 8 CTAs per tile: each computes u = A x over an eighth of K, the partial sums meet in
 //                     distributed shared memory, and each CTA adds s B u to an eighth of the outputs.  One launch, no
 //                     intermediate in memory.
-//   lora_shrink_kernel, lora_expand_kernel  from 2048 tokens on: the two products as two kernels
+//   lora_shrink_kernel, lora_expand_kernel  from 1536 tokens on: the two products as two kernels
 // u is not rounded: its fp32 value enters the second product as three bf16 terms (24 bits).
 #include "serving.cuh"
 
@@ -25,8 +25,11 @@ constexpr int kDirectTokens = 32;     // up to here a warp vote replaces the sor
 constexpr int kBlockTokens = 512, kBlockBins = 1024;  // and up to here, with fewer adapters, each CTA finds its tile by itself
 constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
-constexpr int kWideSplits = 2;        // parts of K with many tiles
-constexpr int kWideTokens = 2048;     // from here on a batch counts as many tiles
+constexpr int kMinSplits = 2, kMaxSplits = 8;  // parts of K with many tiles
+constexpr int kRoom = 2 * kSmCountFallback;
+// From here on a batch counts as many tiles.  Two kernels and one, at 1024 tokens: rank 16, 16 adapters 22.8 and 23.4 us, 64
+// adapters 27.0 and 23.7, rank 128 44.7 and 36.2; at 1500 (rank 32) 29.6 and 30.5; at 2047 (rank 16) 32.7 and 38.2.
+constexpr int kWideTokens = 1536;
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
 constexpr int kColBlock = 128;        // outputs of a tile that go to one CTA as a whole, with many tiles
 constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all
@@ -35,10 +38,10 @@ struct LoraPlan {
   int4 *tiles;   // {adapter or -1, first position in perm, tokens, cost of the tiles before}
   int *perm;     // tokens ordered by adapter
   int *n_tiles;  // number of tiles, cost of them all
-  float *u;       // many tiles: [kWideSplits][T][rank up to 16, 32, 64 or 128]
-  int max_tiles;
-  bool wide;      // many tiles
-  int skip_idle;  // out is y: tokens without an adapter need no work
+  float *u;      // many tiles: [splits][T][rank up to 16, 32, 64 or 128]
+  int max_tiles, splits;
+  bool wide;     // many tiles
+  int skip_idle; // out is y: tokens without an adapter need no work
 };
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -584,7 +587,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 }
 
 // Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
-// do not need: they fill the GPU without splitting a tile's K by more than kWideSplits.
+// do not need: they fill the GPU without splitting a tile's K much.
 // Shrink: a CTA takes 64 tokens and a part of K, x and A come through a ring of 64-element steps in shared memory; the warps are 4
 // across the rows and 2 across the ranks, so no sums have to be joined.
 template <int RN>
@@ -604,10 +607,10 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
   extern __shared__ __align__(16) uint8_t smem_b[];
   pdl_wait();
   pdl_launch_dependents();
-  const Tile t = sorted_tile(p, blockIdx.x / kWideSplits);
+  const Tile t = sorted_tile(p, blockIdx.x / p.splits);
   if (t.count == 0 || t.adapter < 0) return;
-  const int part = blockIdx.x % kWideSplits;
-  const int steps_all = (g.K + kShrinkStep - 1) / kShrinkStep, per = (steps_all + kWideSplits - 1) / kWideSplits;
+  const int part = blockIdx.x % p.splits;
+  const int steps_all = (g.K + kShrinkStep - 1) / kShrinkStep, per = (steps_all + p.splits - 1) / p.splits;
   const int first = part * per, steps = min(per, steps_all - first);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, row = lane >> 2, c = lane & 3;
   const int piece = threadIdx.x & 7, r0 = threadIdx.x >> 3;  // this thread's 16-byte piece of rows r0, r0 + 32, ...
@@ -671,6 +674,21 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
     if (m0 + row + 8 < t.count) *reinterpret_cast<float2 *>(u + 8 * (8 * RN) + 8 * j) = make_float2(acc[j][2], acc[j][3]);
   }
 }
+// u of a tile: its parts (MOST at most), added in their order; MOST * UNROLL loads are under way.
+template <int MOST, int UNROLL, int RN>
+__device__ __forceinline__ void add_parts(const float4 *u, int T, int parts, int count, float4 *u_s) {
+#pragma unroll UNROLL
+  for (int i = threadIdx.x; i < count * 2 * RN; i += 32 * kLoraWarps) {
+    float4 v[MOST];
+#pragma unroll
+    for (int part = 0; part < MOST; ++part)
+      v[part] = part < parts ? u[(size_t)part * T * (2 * RN) + i] : make_float4(0.f, 0.f, 0.f, 0.f);
+    float4 sum = v[0];
+#pragma unroll
+    for (int part = 1; part < MOST; ++part) sum.x += v[part].x, sum.y += v[part].y, sum.z += v[part].z, sum.w += v[part].w;
+    u_s[i] = sum;
+  }
+}
 template <int RN, bool BRING>
 __device__ __forceinline__ void wide_expand(const gptoss_lora_args &g, const LoraPlan &p, const Work &k, float *u_s, float *y_s, int n_first,
                                             int n_end) {
@@ -678,16 +696,10 @@ __device__ __forceinline__ void wide_expand(const gptoss_lora_args &g, const Lor
   expand.start();
   if (!BRING) expand.fetch_w(n_first + 16 * k.k);
   const float4 *u = reinterpret_cast<const float4 *>(p.u) + (size_t)(k.t.perm - p.perm) * (2 * RN);
-#pragma unroll 2
-  for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += 32 * kLoraWarps) {
-    float4 sum = u[i];
-#pragma unroll
-    for (int part = 1; part < kWideSplits; ++part) {
-      const float4 v = u[(size_t)part * g.T * (2 * RN) + i];
-      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-    }
-    reinterpret_cast<float4 *>(u_s)[i] = sum;
-  }
+  if (p.splits == 2)
+    add_parts<2, 4, RN>(u, g.T, 2, k.t.count, reinterpret_cast<float4 *>(u_s));
+  else
+    add_parts<kMaxSplits, 1, RN>(u, g.T, p.splits, k.t.count, reinterpret_cast<float4 *>(u_s));
   __syncthreads();
   expand.run(u_s);
 }
@@ -755,7 +767,17 @@ LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
   p.perm = reinterpret_cast<int *>(take((uint64_t)g.T * sizeof(int)));
   p.n_tiles = reinterpret_cast<int *>(take(2 * sizeof(int)));
   p.wide = g.T >= kWideTokens;
-  if (p.wide) p.u = reinterpret_cast<float *>(take((uint64_t)kWideSplits * g.T * padded_rank(g.rank) * sizeof(float)));
+  if (p.wide) {
+    // as many parts of K as two CTAs per SM have room for, of some six steps at least: the second product adds the parts up
+    // (2047 tokens, rank 128, K = 512: 67 us with 2 parts, 83 with 8; rank 16, K = 2880: 36.6 and 32.7)
+    const int tiles = g.T / kTileTokens, long_enough = g.K / (6 * kShrinkStep);
+    const int fit = kRoom / tiles < long_enough ? kRoom / tiles : long_enough;
+    p.splits = fit < kMinSplits ? kMinSplits : fit > kMaxSplits ? kMaxSplits : fit;
+    // at least splits * T rows, and never less for more tokens: who keeps a workspace asks for the largest batch
+    const uint64_t most = (uint64_t)kMaxSplits * g.T, enough = kRoom * kTileTokens + kMaxSplits * kTileTokens, least = (uint64_t)kMinSplits * g.T;
+    const uint64_t rows = most < enough ? most : (least > enough ? least : enough);
+    p.u = reinterpret_cast<float *>(take(rows * padded_rank(g.rank) * sizeof(float)));
+  }
   return p;
 }
 
@@ -776,7 +798,7 @@ cudaError_t launch_lora(const gptoss_lora_args &g, const LoraPlan &p, cudaStream
   constexpr int expand = kTileTokens * 8 * RN * (int)sizeof(float) + wide_ring;
   constexpr int shrink = ShrinkRing<RN>::kStages * ShrinkRing<RN>::kStageBytes;
   if ((e = allow_smem(lora_shrink_kernel<RN>, shrink)) != cudaSuccess || (e = allow_smem(lora_expand_kernel<RN>, expand)) != cudaSuccess) return e;
-  if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * kWideSplits), block, shrink, s, g, p)) != cudaSuccess) return e;
+  if ((e = launch_chain(lora_shrink_kernel<RN>, dim3(p.max_tiles * p.splits), block, shrink, s, g, p)) != cudaSuccess) return e;
   int device = 0, sms = kSmCountFallback;
   if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
   return launch_chain(lora_expand_kernel<RN>, dim3((RN <= 8 ? 2 : 1) * sms), block, expand, s, g, p);

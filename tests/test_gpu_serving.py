@@ -290,7 +290,7 @@ def test_tree_attention_many_shares(serving, nodes, ctx, hd):
     (1, 2880, 5120, 16, 3), (1, 8, 8, 8, 1), (2, 64, 96, 8, 1), (3, 2880, 2880, 24, 5), (16, 72, 40, 128, 2), (17, 520, 1000, 40, 3),
     (31, 4096, 2880, 64, 40), (64, 2880, 5120, 32, 7), (257, 4096, 2880, 32, 48), (1000, 136, 264, 16, 1), (1025, 200, 2312, 8, 300),
     (4099, 256, 512, 64, 6), (129, 64, 64, 128, 129), (2048, 72, 1000, 128, 3), (2100, 1032, 40, 24, 90), (3001, 8, 8, 8, 1),
-    (2500, 200, 328, 16, 2000), (5000, 64, 2048, 16, 4500), (2051, 64, 8, 64, 40), (400, 64, 96, 16, 1500), (300, 64, 96, 16, 1023), (32, 264, 136, 48, 4), (33, 264, 136, 48, 4)])
+    (2500, 200, 328, 16, 2000), (5000, 64, 2048, 16, 4500), (2051, 64, 8, 64, 40), (1536, 2880, 264, 16, 5), (1600, 3080, 72, 40, 3), (2400, 2000, 136, 16, 7), (400, 64, 96, 16, 1500), (300, 64, 96, 16, 1023), (32, 264, 136, 48, 4), (33, 264, 136, 48, 4)])
 def test_lora(serving, T, K, n_out, rank, n):
     check_lora(serving, lora_case(T, K, n_out, rank, n, seed=T + rank))
 
@@ -308,7 +308,7 @@ def test_lora_orders_ids_and_in_place(serving):
     assert serving.lora_apply(**c) is c["y"] and torch.equal(c["y"], want)
 
 
-@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 2047, 2048, 2111])
+@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 1535, 1536, 2047, 2111])
 def test_lora_groups_of_every_size(serving, T):
     """Runs of one adapter, one adapter for all, none at all, an adapter each, 64 and 65 tokens each; in place and not."""
     n = 70
