@@ -50,6 +50,13 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same with a sum of zero to start from
+__device__ __forceinline__ void mma_16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 // What a tile costs, for cutting the work of many tiles into equal shares: its 16-row blocks and the start.
 __host__ __device__ __forceinline__ int tile_cost(int tokens) { return (tokens + 15) / 16 + 1; }
 
@@ -414,6 +421,14 @@ struct Expand {
                       : make_uint4(0u, 0u, 0u, 0u);
   }
   __device__ __forceinline__ void start() {
+    if (BRING) {  // ranks beyond the adapter's
+      const int pad = 4 * KS - g.rank / 8;
+      for (int i = threadIdx.x; i < kYStages * 32 * BL * pad; i += 32 * kLoraWarps) {
+        const int r = i / pad;
+        *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(y_s + kYStages * kYStageFloats) + r * kBStride + 2 * g.rank + 16 * (i - r * pad)) =
+            make_uint4(0u, 0u, 0u, 0u);
+      }
+    }
 #pragma unroll
     for (int i = 0; i < kYStages - 1; ++i) fetch(i);
   }
@@ -455,16 +470,10 @@ struct Expand {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
               for (int i = 0; i < KS; ++i)
-                w[j][i] = 32 * i + 8 * k.c < g.rank
-                              ? *reinterpret_cast<const uint4 *>(b_s + stage * kBStageBytes + (16 * bl + 2 * j) * kBStride + 64 * i)
-                              : make_uint4(0u, 0u, 0u, 0u);
+                w[j][i] = *reinterpret_cast<const uint4 *>(b_s + stage * kBStageBytes + (16 * bl + 2 * j) * kBStride + 64 * i);
           }
           // a sum per term of u: the products of one sum wait for each other
           float part[3][2][4], acc[2][4];
-#pragma unroll
-          for (int term = 0; term < 3; ++term)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) part[term][j][0] = part[term][j][1] = part[term][j][2] = part[term][j][3] = 0.f;
 #pragma unroll
           for (int i = 0; i < KS; ++i)
 #pragma unroll
@@ -472,9 +481,13 @@ struct Expand {
 #pragma unroll
               for (int term = 0; term < 3; ++term)
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
-                  mma_16816(part[term][j], u0[i][2 * h][term], u1[i][2 * h][term], u0[i][2 * h + 1][term], u1[i][2 * h + 1][term],
-                            h ? w[j][i].z : w[j][i].x, h ? w[j][i].w : w[j][i].y);
+                for (int j = 0; j < 2; ++j) {
+                  const uint32_t w0 = h ? w[j][i].z : w[j][i].x, w1 = h ? w[j][i].w : w[j][i].y;
+                  if (i == 0 && h == 0)
+                    mma_16816_first(part[term][j], u0[i][0][term], u1[i][0][term], u0[i][1][term], u1[i][1][term], w0, w1);
+                  else
+                    mma_16816(part[term][j], u0[i][2 * h][term], u1[i][2 * h][term], u0[i][2 * h + 1][term], u1[i][2 * h + 1][term], w0, w1);
+                }
 #pragma unroll
           for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -587,7 +600,10 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 }
 
 // Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
-// do not need: they fill the GPU without splitting a tile's K much.
+// do not need: they fill the GPU without splitting a tile's K much.  8192 tokens, K = 2880, 5120 outputs, rank 64: 111 us (sort
+// 8, shrink 18, expand 85; floor 58, of which y and out 51).  The second product is bound by the issue of its instructions
+// and what they wait for each other (44 % of the issue slots, tensor pipe 34 %, DRAM 3.9 of 6.6 TB/s): with one term of u instead
+// of three it takes 10 us less, without its stores 12; a plain copy of y to out in the same pattern takes 55.
 // Shrink: a CTA takes 64 tokens and a part of K, x and A come through a ring of 64-element steps in shared memory; the warps are 4
 // across the rows and 2 across the ranks, so no sums have to be joined.
 template <int RN>
@@ -769,7 +785,7 @@ LoraPlan plan_lora(const gptoss_lora_args &g, uint64_t &bytes) {
   p.wide = g.T >= kWideTokens;
   if (p.wide) {
     // as many parts of K as two CTAs per SM have room for, of some six steps at least: the second product adds the parts up
-    // (2047 tokens, rank 128, K = 512: 67 us with 2 parts, 83 with 8; rank 16, K = 2880: 36.6 and 32.7)
+    // (2047 tokens, rank 128, K = 512: 51 us with 2 parts, 16 more with 8; rank 16, K = 2880: 4 less)
     const int tiles = g.T / kTileTokens, long_enough = g.K / (6 * kShrinkStep);
     const int fit = kRoom / tiles < long_enough ? kRoom / tiles : long_enough;
     p.splits = fit < kMinSplits ? kMinSplits : fit > kMaxSplits ? kMaxSplits : fit;
