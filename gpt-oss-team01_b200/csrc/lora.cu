@@ -601,7 +601,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 
 // Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
 // do not need: they fill the GPU without splitting a tile's K much.  8192 tokens, K = 2880, 5120 outputs, rank 64: 111 us (sort
-// 8, shrink 18, expand 85; floor 58, of which y and out 51).  The second product is bound by the issue of its instructions
+// and shrink 25, expand 86; floor 58, of which y and out 51).  The second product is bound by the issue of its instructions
 // and what they wait for each other (44 % of the issue slots, tensor pipe 34 %, DRAM 3.9 of 6.6 TB/s): with one term of u instead
 // of three it takes 10 us less, without its stores 12; a plain copy of y to out in the same pattern takes 55.
 // Shrink: a CTA takes 64 tokens and a part of K, x and A come through a ring of 64-element steps in shared memory; the warps are 4
