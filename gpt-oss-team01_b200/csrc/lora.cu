@@ -355,7 +355,7 @@ struct Expand {
   static constexpr int BL = BRING ? 2 : 1;
   static constexpr int kYStages = BRING ? 3 : 4;
   // 16 wm rows of 16 wn BL + 16 floats (the padding keeps 16-byte reads of 2 rows apart); the wide kernel has wm = 4
-  static constexpr int kYStageFloats = BRING ? 64 * 80 : 3072;
+  static constexpr int kYStageFloats = 64 * (BRING ? 80 : 48);
   static constexpr int kBStageBytes = 32 * BL * kBStride;
   static constexpr int kRingBytes = kYStages * (4 * kYStageFloats + (BRING ? kBStageBytes : 0));
   static constexpr int YP = 2 * BL;  // 16-byte pieces of a step's y per thread
