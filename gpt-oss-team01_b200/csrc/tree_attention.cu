@@ -36,7 +36,9 @@ thread_local char g_serving_error[256] = "";
 // unit's 16 results per cycle and SM make 172 us of it, and each warp's row of dependent steps (S from TMEM, maximum,
 // exponentials, P to TMEM, hand-over) keeps that unit 55 % busy.  No gain: 128-slot tiles with two rows of S (370 us), four
 // CTAs of 128 rows (312 us), two threads per row (319 us), S in two halves with the products one half ahead (311 us), no
-// maximum unless the tile's sum asks for it (spills: 388 us).
+// maximum unless the tile's sum asks for it (spills: 388 us), P in shared memory so that S is free for the next tile as soon as
+// it is in registers (384 us: with N = 64 the A operand's way from shared memory takes twice the product's time; in TMEM there
+// is no room for P beside S and O of four groups).
 //
 // Tiles that every row sees whole skip all masking.  In the others (the window's edge, the drafted slots, the end) each
 // thread builds a mask of its row, 32 slots to a word.  What a row must not see still goes through P V as 0 * V, so in those
