@@ -270,7 +270,9 @@ __global__ void __launch_bounds__(128) expert_choice_kernel(const __grid_constan
     const float gap = 2.f * err + 0x1p-19f * largest;  // the slot took the place of three bits of each choice
     float before = INFINITY;
     const float floor = by_logits ? (softmax ? mx : 0.f) - 700.f : -INFINITY;
-    for (int j = 0; j <= a.k; ++j) {  // the one after the last tells whether the last is sure
+#pragma unroll
+    for (int j = 0; j <= kMaxTopK; ++j) {  // the one after the last tells whether the last is sure
+      if (j > a.k) break;
       const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
       if (top == 0u) break;
       const uint32_t who = __ballot_sync(0xffffffffu, key[0] == top);
@@ -280,8 +282,8 @@ __global__ void __launch_bounds__(128) expert_choice_kernel(const __grid_constan
       if (lane == j) my_e = 32 * (int)(top & 7u) + __ffs(who) - 1;
       if (key[0] == top) {
 #pragma unroll
-        for (int s = 0; s + 1 < SLOTS; ++s) key[s] = key[s + 1];
-        key[SLOTS - 1] = 0u;
+        for (int s = 0; s + 1 < SLOTS && s < kMaxTopK - j; ++s) key[s] = key[s + 1];  // as many as can still be asked for
+        if (SLOTS <= kMaxTopK - j) key[SLOTS - 1] = 0u;
       }
     }
   }
