@@ -163,7 +163,7 @@ __device__ __forceinline__ void sort_keys(uint32_t (&k)[N]) {
 // One warp per token.  The choice is made in fp32 with a bound on its error, and taken if every comparison that decides it
 // (kept against dropped groups, each chosen expert against the next one) is wider than that bound; otherwise - ties, near
 // ties, infinities, NaN - the token is done again in fp64.  With everything in fp64, 8192 tokens x 256 experts in 8 groups
-// took 30 us.  What bounds the kernel is the number of instructions per token: each lane sorts its experts once (the key of
+// took 30 us (17.3 now).  What bounds the kernel is the number of instructions per token: each lane sorts its experts once (the key of
 // an expert is its choice with the slot in the three lowest bits), so that a round is one warp-wide maximum.
 template <int SLOTS>
 __global__ void __launch_bounds__(128) expert_choice_kernel(const __grid_constant__ gptoss_expert_choice_args a, uint32_t group_magic) {
