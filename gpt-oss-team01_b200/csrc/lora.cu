@@ -12,7 +12,7 @@
 //   lora_kernel       a cluster of 8 CTAs per tile: each computes u = A x over an eighth of K, the partial sums meet in
 //                     distributed shared memory, and each CTA adds s B u to an eighth of the outputs.  One launch, no
 //                     intermediate in memory.
-//   lora_shrink_kernel, lora_expand_kernel  from 1536 tokens on: the two products as two kernels
+//   lora_shrink_kernel, lora_expand_kernel  from 1280 tokens on: the two products as two kernels
 // u is not rounded: its fp32 value enters the second product as three bf16 terms (24 bits).
 #include "serving.cuh"
 
@@ -27,9 +27,9 @@ constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
 constexpr int kMinSplits = 2, kMaxSplits = 8;  // parts of K with many tiles
 constexpr int kRoom = 2 * kSmCountFallback;
-// From here on a batch counts as many tiles.  Two kernels and one, at 1024 tokens: rank 16, 16 adapters 22.8 and 23.4 us, 64
-// adapters 27.0 and 23.7, rank 128 44.7 and 36.2; at 1500 (rank 32) 29.6 and 30.5; at 2047 (rank 16) 32.7 and 38.2.
-constexpr int kWideTokens = 1536;
+// From here on a batch counts as many tiles.  Two kernels and one, at 1024 tokens: rank 16, 16 adapters 22.8 and 24.8 us, 64
+// adapters 27.0 and 24.1, rank 128 44.7 and 37.7; at 1500 (rank 32) 29.6 and 33.2; at 2047 (rank 16) 32.3 and 38.2.
+constexpr int kWideTokens = 1280;
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
 constexpr int kColBlock = 128;        // outputs of a tile that go to one CTA as a whole, with many tiles
 constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all
@@ -74,9 +74,11 @@ __device__ __forceinline__ int bin_of(const int *__restrict__ ids, int t, int T,
 // One block.  Bins 0..n-1 are the adapters, bin n the tokens without one.
 __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__ ids, int T, int n, LoraPlan p) {
   extern __shared__ int bin_s[];  // [n + 1] counts, then cursors
-  __shared__ int warp_tok[32], warp_tile[32], warp_cost[32];
+  __shared__ int warp_tok[32], warp_tile[32], warp_cost[32], n_several;
+  __shared__ int2 several[kWideTokens / kTileTokens];  // adapters with several tiles: bin, first position
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int i = tid; i <= n; i += 1024) bin_s[i] = 0;
+  if (tid == 0) n_several = 0;
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
@@ -117,6 +119,10 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   for (int b = b0; b < b1; ++b) {
     const int c = bin_s[b];
     bin_s[b] = tok_at;
+    if (c > kTileTokens && b < n && !p.wide) {
+      several[atomicAdd(&n_several, 1)] = make_int2(b, tok_at);
+      bin_s[b] = -1;
+    }
     if (b < bins)
       for (int j = 0; j < c; j += kTileTokens) {
         p.tiles[til_at++] = make_int4(b < n ? b : -1, tok_at + j, min(kTileTokens, c - j), cost_at);
@@ -125,7 +131,24 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
     tok_at += c;
   }
   __syncthreads();
-  // where a token stands among those of its adapter varies from run to run; its result does not depend on it
+  // Where a token stands among those of its adapter may vary from run to run: that moves it to another row of a tile, where
+  // its sums are the same.  With several tiles it could move it to another tile, and the last one, with fewer rows, is summed
+  // in another order (except in the kernels for many tiles): those adapters' tokens are taken in their order, by a warp each.
+  for (int i = warp; i < n_several; i += 32) {
+    const int2 d = several[i];
+    int at = d.y;
+    for (int t0 = 0; t0 < T; t0 += 8 * 32) {
+      int bin[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) bin[j] = bin_of(ids, t0 + 32 * j + lane, T, n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t members = __ballot_sync(0xffffffffu, bin[j] == d.x);
+        if (bin[j] == d.x) p.perm[at + __popc(members & ((1u << lane) - 1u))] = t0 + 32 * j + lane;
+        at += __popc(members);
+      }
+    }
+  }
   for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
     int bin[8];
 #pragma unroll
@@ -136,9 +159,10 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
       const uint32_t same = __match_any_sync(0xffffffffu, bin[i]);
       const int leader = __ffs(same) - 1;
       int at = 0;
-      if (bin[i] >= 0 && lane == leader) at = atomicAdd(&bin_s[bin[i]], __popc(same));
+      const bool mine = bin[i] >= 0 && bin_s[bin[i]] >= 0;
+      if (mine && lane == leader) at = atomicAdd(&bin_s[bin[i]], __popc(same));
       at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
-      if (bin[i] >= 0) p.perm[at] = t0 + 1024 * i + tid;
+      if (mine) p.perm[at] = t0 + 1024 * i + tid;
     }
   }
 }

@@ -308,7 +308,7 @@ def test_lora_orders_ids_and_in_place(serving):
     assert serving.lora_apply(**c) is c["y"] and torch.equal(c["y"], want)
 
 
-@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 1535, 1536, 2047, 2111])
+@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 1279, 1280, 1535, 2047, 2111])
 def test_lora_groups_of_every_size(serving, T):
     """Runs of one adapter, one adapter for all, none at all, an adapter each, 64 and 65 tokens each; in place and not."""
     n = 70
@@ -318,6 +318,23 @@ def test_lora_groups_of_every_size(serving, T):
         got = check_lora(serving, c)
         y = c["y"].clone()
         assert torch.equal(serving.lora_apply(**{**c, "y": y}), got)
+
+
+@pytest.mark.parametrize("T,rank,n", [(20, 16, 2), (300, 32, 3), (567, 64, 3), (1200, 16, 5), (1279, 128, 2), (700, 16, 1100), (3000, 32, 7)])
+def test_lora_gives_the_same_bits_every_time(serving, T, rank, n):
+    """Also when other work runs beside it, which changes the order in which the tokens' threads come."""
+    c = lora_case(T, 1736, 520, rank, n, seed=T)
+    if n > 1000:
+        c["ids"] = torch.where(torch.arange(T, device="cuda") % 3 == 0, c["ids"], c["ids"] % 2)
+    want = serving.lora_apply(**c, out=torch.empty_like(c["y"]))
+    side, load = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda")
+    outs = []
+    for i in range(60):
+        with torch.cuda.stream(side):
+            load = torch.sin(load)
+        outs.append(serving.lora_apply(**c, out=torch.empty_like(c["y"])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
 
 
 def test_lora_strides_zeros_and_what_is_not_served(serving):
