@@ -282,6 +282,7 @@ const char *gptoss_noalloc_last_error(void);
  * device, are asynchronous on `stream`, allocate nothing, keep nothing between calls and can be captured into a CUDA
  * graph.  Arguments are checked on the host; counts and indices that live on the device are bounded by the kernels, so
  * that a bad one never reaches memory outside the tensors, but what it yields is not specified beyond what is said here.
+ * The same call on the same inputs gives the same bits.
  * A workspace belongs to one call at a time: two calls (or captured graphs) that may overlap need two. */
 /* Message of the last failing call of these operators on this host thread ("" if none). */
 const char *gptoss_serving_last_error(void);

@@ -286,6 +286,22 @@ def test_tree_attention_many_shares(serving, nodes, ctx, hd):
     check_tree(serving, tree_case(serving, nodes, ctx, 2, 1, hd, seed=hd + ctx[0]), max(nodes), max(ctx))
 
 
+@pytest.mark.parametrize("nodes,ctx,nq,nkv,window", [([24] * 6, [900] * 6, 16, 2, 128), ([13, 7], [9000, 4000], 8, 1, 0), ([64] * 8, [500] * 8, 64, 8, 0)])
+def test_tree_attention_gives_the_same_bits_every_time(serving, nodes, ctx, nq, nkv, window):
+    c = tree_case(serving, nodes, ctx, nq, nkv, 64, seed=77)
+    c["v_cache"][:, :, ctx[0] + 2, 5] = math.nan  # a masked row for most of the tokens
+    call = lambda: serving.tree_attention(**c, window=window, max_nodes=max(nodes), max_ctx=max(ctx))  # noqa: E731
+    want = call()
+    side, load = torch.cuda.Stream(), torch.randn(2048, 2048, device="cuda")
+    outs = []
+    for _ in range(40):
+        with torch.cuda.stream(side):
+            load = torch.sin(load)
+        outs.append(call())
+    torch.cuda.synchronize()
+    assert all(torch.equal(o.view(torch.int16), want.view(torch.int16)) for o in outs)
+
+
 @pytest.mark.parametrize("T,K,n_out,rank,n", [
     (1, 2880, 5120, 16, 3), (1, 8, 8, 8, 1), (2, 64, 96, 8, 1), (3, 2880, 2880, 24, 5), (16, 72, 40, 128, 2), (17, 520, 1000, 40, 3),
     (31, 4096, 2880, 64, 40), (64, 2880, 5120, 32, 7), (257, 4096, 2880, 32, 48), (1000, 136, 264, 16, 1), (1025, 200, 2312, 8, 300),

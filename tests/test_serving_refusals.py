@@ -109,7 +109,7 @@ def test_expert_choice_of_nothing_is_a_no_op(lib):
     assert lib.gptoss_expert_choice(C.byref(choice_args(T=0, logits=None)), None) == capi.OK
 
 
-def test_python_layer_refuses_host_tensors_and_wrong_types():
+def test_python_layer_refuses_host_tensors_and_wrong_types(lib):
     from gptoss_b200 import moe, serving
     q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
     c = torch.zeros(1, 2, 8, 64, dtype=torch.bfloat16)
