@@ -335,7 +335,8 @@ int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_ro
 /* Adapters beside a shared projection: out[t] = y[t] + scale[a] * B_a (A_a x[t]) with a = ids[t]; a token whose id is
  * outside [0, n_adapters) has no adapter (out[t] = y[t]).  x [T][K] bf16, a [n_adapters][rank][K] bf16,
  * b [n_adapters][n_out][rank] bf16, scale [n_adapters] fp32 or NULL for 1, y and out [T][n_out] fp32; out may be y.
- * Products accumulate in fp32 and the intermediate A x is not rounded.  K and n_out multiples of 8 (up to 2^30), rank a
+ * Products accumulate in fp32 and the intermediate A x is not rounded.  The order of the sums, hence a token's last bits,
+ * depends on how many tokens the call has and how many of them share the adapter.  K and n_out multiples of 8 (up to 2^30), rank a
  * multiple of 8 up to GPTOSS_LORA_MAX_RANK (adapters of lower rank: zero rows of A, zero columns of B), at most 8192
  * adapters.  What adapters that no token uses and rows of x without an adapter hold does not matter. */
 #define GPTOSS_LORA_MAX_RANK 128
@@ -486,7 +487,9 @@ int gptoss_model_lora_create(gptoss_model *m, int n_adapters, int rank);
  * the model's stream. */
 int gptoss_model_lora_load(gptoss_model *m, int adapter, int layer, const float *a_qkv, const float *b_qkv, const float *a_o,
                            const float *b_o, float scale);
-/* The sequence in cache row `row` uses this adapter from its next step on (-1: none, the state of every row at first). */
+/* The sequence in cache row `row` uses this adapter from its next step on (-1: none, the state of every row at first).  Rows
+ * without one keep the bits that they have in any batch; those of a row with one depend on how many rows share its adapter
+ * (gptoss_lora_apply). */
 int gptoss_model_lora_bind(gptoss_model *m, int row, int adapter);
 /* The phases of gptoss_model_step, which runs begin, then per layer attention / moe_dispatch / moe_push / moe_combine,
  * then end.  In a group, B is the batch of the group and tokens_host / next_tokens_host hold this rank's sequences only.
