@@ -12,7 +12,7 @@
 //   lora_kernel       a cluster of 8 CTAs per tile: each computes u = A x over an eighth of K, the partial sums meet in
 //                     distributed shared memory, and each CTA adds s B u to an eighth of the outputs.  One launch, no
 //                     intermediate in memory.
-//   lora_shrink_kernel, lora_expand_kernel  from 1280 tokens on: the two products as two kernels
+//   lora_shrink_kernel, lora_expand_kernel  from 768 tokens on: the two products as two kernels
 // u is not rounded: its fp32 value enters the second product as three bf16 terms (24 bits).
 #include "serving.cuh"
 
@@ -27,9 +27,10 @@ constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
 constexpr int kMinSplits = 2, kMaxSplits = 8;  // parts of K with many tiles
 constexpr int kRoom = 2 * kSmCountFallback;
-// From here on a batch counts as many tiles.  Two kernels and one, at 1024 tokens: rank 16, 16 adapters 22.8 and 24.8 us, 64
-// adapters 27.0 and 24.1, rank 128 44.7 and 37.7; at 1500 (rank 32) 29.6 and 33.2; at 2047 (rank 16) 32.3 and 38.2.
-constexpr int kWideTokens = 1280;
+// From here on a batch counts as many tiles.  Two kernels and one: 600 tokens, rank 16, 16 adapters 19.9 and 18.6 us; 800 tokens,
+// rank 64, 8 adapters 27.7 and 32.7, rank 8, 200 adapters 34.2 and 37.0; 1024 tokens, rank 16, 64 adapters 25.9 and 24.0, rank
+// 128, 4 adapters 32.6 and 37.8; 1200 tokens, rank 128, 8 adapters 45.8 and 65.8.
+constexpr int kWideTokens = 768;
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
 constexpr int kColBlock = 128;        // outputs of a tile that go to one CTA as a whole, with many tiles
 constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all

@@ -324,7 +324,7 @@ def test_lora_orders_ids_and_in_place(serving):
     assert serving.lora_apply(**c) is c["y"] and torch.equal(c["y"], want)
 
 
-@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 1279, 1280, 1535, 2047, 2111])
+@pytest.mark.parametrize("T", [33, 64, 65, 255, 256, 257, 300, 511, 512, 513, 767, 768, 1279, 1535, 2047, 2111])
 def test_lora_groups_of_every_size(serving, T):
     """Runs of one adapter, one adapter for all, none at all, an adapter each, 64 and 65 tokens each; in place and not."""
     n = 70
@@ -336,7 +336,7 @@ def test_lora_groups_of_every_size(serving, T):
         assert torch.equal(serving.lora_apply(**{**c, "y": y}), got)
 
 
-@pytest.mark.parametrize("T,rank,n", [(20, 16, 2), (300, 32, 3), (567, 64, 3), (1200, 16, 5), (1279, 128, 2), (700, 16, 1100), (3000, 32, 7)])
+@pytest.mark.parametrize("T,rank,n", [(20, 16, 2), (300, 32, 3), (567, 64, 3), (767, 16, 11), (1200, 16, 5), (1279, 128, 2), (700, 16, 1100), (3000, 32, 7)])
 def test_lora_gives_the_same_bits_every_time(serving, T, rank, n):
     """Also when other work runs beside it, which changes the order in which the tokens' threads come."""
     c = lora_case(T, 1736, 520, rank, n, seed=T)
