@@ -84,16 +84,19 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
   pdl_wait();
   pdl_launch_dependents();
   // neighbours often share an adapter: one atomic per adapter and warp.  Eight loads are under way at a time.
-  for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
-    int bin[8];
+  int bin[8];
+  uint32_t same[8];  // the lanes of the warp with the same bin
+  const auto load = [&](int t0) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) bin[i] = bin_of(ids, t0 + 1024 * i + tid, T, n);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (t0 + 1024 * i >= T) break;
-      const uint32_t same = __match_any_sync(0xffffffffu, bin[i]);
-      if (bin[i] >= 0 && lane == __ffs(same) - 1) atomicAdd(&bin_s[bin[i]], __popc(same));
-    }
+    for (int i = 0; i < 8; ++i) same[i] = t0 + 1024 * i < T ? __match_any_sync(0xffffffffu, bin[i]) : 0u;
+  };
+  for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
+    load(t0);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (bin[i] >= 0 && lane == __ffs(same[i]) - 1) atomicAdd(&bin_s[bin[i]], __popc(same[i]));
   }
   __syncthreads();
   // exclusive prefix of the counts (positions) and of the tile counts; a thread owns `per` consecutive bins
@@ -139,30 +142,27 @@ __global__ void __launch_bounds__(1024) lora_sort_kernel(const int *__restrict__
     const int2 d = several[i];
     int at = d.y;
     for (int t0 = 0; t0 < T; t0 += 8 * 32) {
-      int bin[8];
+      int of[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) bin[j] = bin_of(ids, t0 + 32 * j + lane, T, n);
+      for (int j = 0; j < 8; ++j) of[j] = bin_of(ids, t0 + 32 * j + lane, T, n);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t members = __ballot_sync(0xffffffffu, bin[j] == d.x);
-        if (bin[j] == d.x) p.perm[at + __popc(members & ((1u << lane) - 1u))] = t0 + 32 * j + lane;
+        const uint32_t members = __ballot_sync(0xffffffffu, of[j] == d.x);
+        if (of[j] == d.x) p.perm[at + __popc(members & ((1u << lane) - 1u))] = t0 + 32 * j + lane;
         at += __popc(members);
       }
     }
   }
   for (int t0 = 0; t0 < T; t0 += 8 * 1024) {
-    int bin[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) bin[i] = bin_of(ids, t0 + 1024 * i + tid, T, n);
+    if (T > 8 * 1024) load(t0);  // else they are still there
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if (t0 + 1024 * i >= T) break;
-      const uint32_t same = __match_any_sync(0xffffffffu, bin[i]);
-      const int leader = __ffs(same) - 1;
+      const int leader = __ffs(same[i]) - 1;
       int at = 0;
       const bool mine = bin[i] >= 0 && bin_s[bin[i]] >= 0;
-      if (mine && lane == leader) at = atomicAdd(&bin_s[bin[i]], __popc(same));
-      at = __shfl_sync(0xffffffffu, at, leader) + __popc(same & ((1u << lane) - 1u));
+      if (mine && lane == leader) at = atomicAdd(&bin_s[bin[i]], __popc(same[i]));
+      at = __shfl_sync(0xffffffffu, at, leader) + __popc(same[i] & ((1u << lane) - 1u));
       if (mine) p.perm[at] = t0 + 1024 * i + tid;
     }
   }
@@ -625,7 +625,7 @@ __global__ void __cluster_dims__(kClusterCtas, 1, 1) __launch_bounds__(32 * kLor
 }
 
 // Many tiles: two kernels.  Meeting three times costs a CTA of a cluster some 10 us, which few tiles cannot avoid and many
-// do not need: they fill the GPU without splitting a tile's K much.  8192 tokens, K = 2880, 5120 outputs, rank 64: 111 us (sort
+// do not need: they fill the GPU without splitting a tile's K much.  8192 tokens, K = 2880, 5120 outputs, rank 64: 110 us (sort
 // and shrink 25, expand 86; floor 58, of which y and out 51).  The second product is bound by the issue of its instructions
 // and what they wait for each other (44 % of the issue slots, tensor pipe 34 %, DRAM 3.9 of 6.6 TB/s): with one term of u instead
 // of three it takes 10 us less, without its stores 12; a plain copy of y to out in the same pattern takes 55.

@@ -306,7 +306,7 @@ def test_tree_attention_gives_the_same_bits_every_time(serving, nodes, ctx, nq, 
     (1, 2880, 5120, 16, 3), (1, 8, 8, 8, 1), (2, 64, 96, 8, 1), (3, 2880, 2880, 24, 5), (16, 72, 40, 128, 2), (17, 520, 1000, 40, 3),
     (31, 4096, 2880, 64, 40), (64, 2880, 5120, 32, 7), (257, 4096, 2880, 32, 48), (1000, 136, 264, 16, 1), (1025, 200, 2312, 8, 300),
     (4099, 256, 512, 64, 6), (129, 64, 64, 128, 129), (2048, 72, 1000, 128, 3), (2100, 1032, 40, 24, 90), (3001, 8, 8, 8, 1),
-    (2500, 200, 328, 16, 2000), (5000, 64, 2048, 16, 4500), (2051, 64, 8, 64, 40), (1536, 2880, 264, 16, 5), (1600, 3080, 72, 40, 3), (2400, 2000, 136, 16, 7), (400, 64, 96, 16, 1500), (300, 64, 96, 16, 1023), (32, 264, 136, 48, 4), (33, 264, 136, 48, 4)])
+    (2500, 200, 328, 16, 2000), (5000, 64, 2048, 16, 4500), (2051, 64, 8, 64, 40), (9001, 64, 72, 8, 3), (17000, 32, 40, 8, 4000), (1536, 2880, 264, 16, 5), (1600, 3080, 72, 40, 3), (2400, 2000, 136, 16, 7), (400, 64, 96, 16, 1500), (300, 64, 96, 16, 1023), (32, 264, 136, 48, 4), (33, 264, 136, 48, 4)])
 def test_lora(serving, T, K, n_out, rank, n):
     check_lora(serving, lora_case(T, K, n_out, rank, n, seed=T + rank))
 
