@@ -155,7 +155,8 @@ cudaError_t launch_residual_rmsnorm(float *x, const float *add, const float *w, 
 cudaError_t launch_qkv_rope_store(const float *qkv, const float *cos_t, const float *sin_t, int pos, int B, int nq, int nkv,
                                   int hd, int S, float *q_out, __nv_bfloat16 *k_cache, __nv_bfloat16 *v_cache,
                                   const int *cache_rows, const int *pos_rows, cudaStream_t s);
-// drafted tokens: K, V of row b to slot slots[b] of cache row cache_rows[b], rotated for position rope_rows[b]; q as bf16
+// drafted tokens: K, V of row b to slot slots[b] of cache row cache_rows[b], rotated for position rope_rows[b]; q as
+// two bf16 terms: [B][nq][hd] of the first, then [B][nq][hd] of the second
 cudaError_t launch_qkv_rope_store_tree(const float *qkv, const float *cos_t, const float *sin_t, int B, int nq, int nkv, int hd, int S,
                                        __nv_bfloat16 *q_out, __nv_bfloat16 *k_cache, __nv_bfloat16 *v_cache, const int *cache_rows,
                                        const int *slots, const int *rope_rows, cudaStream_t s);

@@ -534,7 +534,7 @@ int gptoss_model_layer_attention(gptoss_model *m, int layer) {
       a.q = q16, a.k_cache = kc, a.v_cache = vc, a.out = m->att, a.sinks = m->sinks + l * nq;
       a.window = c.sliding_window > 0 && l % 2 == 0 ? c.sliding_window : 0;  // run.cpp:582
       a.workspace = m->tree_work, a.workspace_bytes = m->tree_work_bytes;
-      if ((rc = gptoss_tree_attention(&a, s))) return m->fail(rc, gptoss_serving_last_error());
+      if ((rc = tree_attention_fine(a, q16 + (size_t)B * qd, s))) return m->fail(rc, gptoss_serving_last_error());
     } else {
       MK(launch_qkv_rope_store(m->qkv, m->cos_t, m->sin_t, pos, B, nq, nkv, hd, (int)S, m->q, kc, vc, m->step_rows,
                                m->step_pos_rows, s));
@@ -817,9 +817,9 @@ int gptoss_model_step_tree(gptoss_model *m, int n_seqs, const int *rows_host, co
     a.cache_rows = m->max_local, a.max_seq = m->S, a.n_q_heads = m->c.n_attn_heads, a.n_kv_heads = m->c.n_kv_heads;
     a.head_dim = m->c.head_dim, a.scale = 1.0f / sqrtf((float)m->c.head_dim);
     m->tree_args = a;
-    uint64_t need = gptoss_tree_attention_workspace(&a);
+    uint64_t need = tree_attention_fine_workspace(a);
     a.window = m->c.sliding_window;  // a shorter context may be cut into more, smaller shares
-    const uint64_t need_windowed = gptoss_tree_attention_workspace(&a);
+    const uint64_t need_windowed = tree_attention_fine_workspace(a);
     if (need_windowed > need) need = need_windowed;
     if (need > m->tree_work_bytes) {
       MK(cudaStreamSynchronize(m->stream));

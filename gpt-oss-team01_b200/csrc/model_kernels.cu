@@ -52,11 +52,20 @@ __global__ void __launch_bounds__(256) residual_rmsnorm_kernel(float *__restrict
   pdl_launch_dependents();
 }
 
+// (x, y) -> bf16 pair of the rounded values (hi) and of the remainders (lo); x in the low half
+__device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint32_t &lo) {
+  const __nv_bfloat16 xh = __float2bfloat16_rn(x), yh = __float2bfloat16_rn(y);
+  const __nv_bfloat16 xl = __float2bfloat16_rn(x - __bfloat162float(xh)), yl = __float2bfloat16_rn(y - __bfloat162float(yh));
+  hi = (uint32_t)__bfloat16_as_ushort(xh) | ((uint32_t)__bfloat16_as_ushort(yh) << 16);
+  lo = (uint32_t)__bfloat16_as_ushort(xl) | ((uint32_t)__bfloat16_as_ushort(yl) << 16);
+}
+
 // qkv[b, :] = (q heads | k heads | v heads), bias already added (run.cpp:534-557).  Rotates q and k with the
 // cos/sin of position `pos` (half-split pairs: element i pairs with i + hd/2), writes q as fp32 and k, v as
 // bf16 into the caches at [b, kv_head, pos, i]: the rows that one (sequence, kv head) attends to are contiguous.
 // TREE: row b is a drafted token, cached in slot pos_rows[b] of row cache_rows[b] but rotated for position rope_rows[b]
-// (siblings share a position), and q goes out as bf16, the type of the tree attention's products.
+// (siblings share a position), and q goes out as two bf16 terms, the type of the tree attention's products: the first terms of
+// all rows, then the second ones.
 template <bool TREE>
 __global__ void __launch_bounds__(256) qkv_rope_store_kernel(const float *__restrict__ qkv, const float *__restrict__ cos_t,
                                                              const float *__restrict__ sin_t, int pos, int nq, int nkv,
@@ -84,9 +93,10 @@ __global__ void __launch_bounds__(256) qkv_rope_store_kernel(const float *__rest
     const float2 o1 = make_float2(x1.x * c.x - x2.x * s.x, x1.y * c.y - x2.y * s.y);
     const float2 o2 = make_float2(x2.x * c.x + x1.x * s.x, x2.y * c.y + x1.y * s.y);
     if (TREE && h < nq) {
-      __nv_bfloat16 *dst = reinterpret_cast<__nv_bfloat16 *>(q_out) + (size_t)b * qdim + h * hd + j;
-      *reinterpret_cast<__nv_bfloat162 *>(dst) = __floats2bfloat162_rn(o1.x, o1.y);
-      *reinterpret_cast<__nv_bfloat162 *>(dst + half) = __floats2bfloat162_rn(o2.x, o2.y);
+      uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<__nv_bfloat16 *>(q_out) + (size_t)b * qdim + h * hd + j);
+      uint32_t *low = dst + (size_t)gridDim.x * qdim / 2;
+      split_pair(o1.x, o1.y, dst[0], low[0]);
+      split_pair(o2.x, o2.y, dst[half / 2], low[half / 2]);
     } else if (h < nq) {
       float *dst = q_out + (size_t)b * qdim + h * hd + j;
       *reinterpret_cast<float2 *>(dst) = o1;
@@ -133,14 +143,6 @@ __device__ __forceinline__ void mma_bf16_16816(float (&c)[4], uint32_t a0, uint3
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// (x, y) -> bf16 pair of the rounded values (hi) and of the remainders (lo); x in the low half
-__device__ __forceinline__ void split_pair(float x, float y, uint32_t &hi, uint32_t &lo) {
-  const __nv_bfloat16 xh = __float2bfloat16_rn(x), yh = __float2bfloat16_rn(y);
-  const __nv_bfloat16 xl = __float2bfloat16_rn(x - __bfloat162float(xh)), yl = __float2bfloat16_rn(y - __bfloat162float(yh));
-  hi = (uint32_t)__bfloat16_as_ushort(xh) | ((uint32_t)__bfloat16_as_ushort(yh) << 16);
-  lo = (uint32_t)__bfloat16_as_ushort(xl) | ((uint32_t)__bfloat16_as_ushort(yl) << 16);
-}
-
 template <int HD, int G>
 __global__ void __launch_bounds__(128) attention_kernel(const float *__restrict__ q, const __nv_bfloat16 *__restrict__ k_cache,
                                                         const __nv_bfloat16 *__restrict__ v_cache,

@@ -21,11 +21,14 @@ thread_local char g_serving_error[256] = "";
 // group) pair, so a tree of n tokens with g heads per kv head gives n g rows that all read the same K and V; a query tile
 // has 128 of them.  Per tile of 64 slots:
 //   S = Q K^T             tcgen05, accumulator in TMEM
-//   P = 2^(c S - m)       c = scale log2(e); in the registers of one thread per row, as bf16 back to TMEM in place of S
+//   P = 2^(c S - m)       c = scale log2(e); in the registers of one thread per row, back to TMEM in place of S
 //   O += P V              tcgen05, A operand from TMEM, V as it lies in the cache (its N index innermost)
 // m is a running reference, not the running maximum: it moves (and O is rescaled in TMEM) only when the maximum has grown
 // by more than 2^8, so that most tiles leave O alone; P and O stay below 2^8 times their usual range.  P is rounded to
-// bf16, the type of V (both operands of the product have the same type); the denominator adds the unrounded values.
+// bf16, the type of V (both operands of the product have the same type); the denominator adds the unrounded values.  For
+// outputs that are bf16 themselves the two roundings are alike (2-norm of the error 1.8e-3 to 2.3e-3, 1.7e-3 without that of P);
+// a second bf16 term of P would take that one away, at 399 instead of 320 us for 64 x 64 over 4096.  The model's own steps
+// have it (LOW below), as drafted decoding has to give the tokens of one-token decoding.
 //
 // Two groups of four softmax warps work side by side, so that one's exponentials cover the other's products: on a query tile
 // each (K and V tiles are then fetched once for 256 rows: with 128 rows per CTA the L2 reads alone took 247 of 310 us for
@@ -72,7 +75,8 @@ constexpr size_t kAttSmem = 2 * kAttQBytes + kAttTileBytes * 2 * kAttStages + 10
 struct AttParams {
   CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 64, 1}
   gptoss_tree_attention_args a;
-  int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
+  const void *q_low;         // second bf16 term of the queries, laid out like a.q (the kernel with LOW)
+  int group, nodes_per_tile, nodes_per_cta, q_blocks, n_splits, tiles_per_split;
   bool in_cluster;           // the shares of the context are a cluster and join in shared memory
   float c;                   // scale * log2(e)
 };
@@ -121,6 +125,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
         "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+               "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+               : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // D[tmem] (+)= A[tmem] * B[smem], bf16, M = 128, K = 16
@@ -223,7 +232,11 @@ __device__ __forceinline__ bool elect_one() {
   return ok != 0;
 }
 
-template <int HD>
+// LOW: queries and weights of two bf16 terms each (16 bits), for steps that have to follow one-token decoding, whose attention
+// keeps them so: with one term the drafted greedy decoding of the 7m fixture left the reference's tokens at the 16th.  The
+// queries' second term takes the second query tile's place in shared memory, S is the sum of the products with both, and the
+// groups always share out the slot tiles; the weights' second term takes the other half of S's columns in TMEM.
+template <int HD, bool LOW>
 __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_kernel(const __grid_constant__ AttParams p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -235,8 +248,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   int x = blockIdx.x;
   const int split = x % p.n_splits;
   x /= p.n_splits;
-  const int pair = x % p.q_pairs;
-  x /= p.q_pairs;
+  const int block = x % p.q_blocks;
+  x /= p.q_blocks;
   const int kvh = x % a.n_kv_heads, b = x / a.n_kv_heads;
   // what does not depend on the kernels before
   if (threadIdx.x == 0) {
@@ -258,13 +271,13 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
   const int first = a.offsets[b], n = min(min(a.offsets[b + 1], a.n_tokens) - first, a.max_nodes);
   const int row = a.rows ? a.rows[b] : b;
   int ctx = min(max(a.ctx_len[b], 0), a.max_seq);
-  const int n0 = 2 * pair * p.nodes_per_tile, nodes = min(n - n0, 2 * p.nodes_per_tile);
+  const int n0 = block * p.nodes_per_cta, nodes = min(n - n0, p.nodes_per_cta);
   if (first < 0 || nodes <= 0) {  // with all CTAs of its cluster
     pdl_launch_dependents();
     if (warp == 8) tmem_dealloc(tmem, kAttTmemCols);
     return;
   }
-  const bool by_rows = nodes > p.nodes_per_tile;  // a query tile for each group, else the slot tiles are dealt out to them
+  const bool by_rows = !LOW && nodes > p.nodes_per_tile;  // a query tile for each group, else the slot tiles are dealt out to them
   int len = min(ctx + n, a.max_seq);
   if (row < 0 || row >= a.cache_rows) ctx = len = 0;
   const int slab = row * a.n_kv_heads + kvh;
@@ -326,6 +339,11 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k)
           umma_bf16(tmem + grp * kTmemGroup + kTmemS, e + (uint64_t)(2 * k), d + (uint64_t)(2 * k), idesc_s, k > 0);
+        if (LOW) {
+#pragma unroll
+          for (int k = 0; k < HD / 16; ++k)
+            umma_bf16(tmem + grp * kTmemGroup + kTmemS, dq + (kAttQBytes >> 4) + (uint64_t)(2 * k), d + (uint64_t)(2 * k), idesc_s, 1u);
+        }
         umma_commit(s_full + 8 * grp);
       };
       auto output = [&](int grp, int stage, bool add) {
@@ -334,6 +352,11 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
 #pragma unroll
         for (int c = 0; c < kAttTile / 16; ++c)  // 16 slots: 8 TMEM columns of P, 2048 bytes of V
           umma_bf16_ts(t + kTmemO, t + kTmemS + 8 * c, d + (uint64_t)(128 * c), idesc_o, add || c > 0);
+        if (LOW) {
+#pragma unroll
+          for (int c = 0; c < kAttTile / 16; ++c)
+            umma_bf16_ts(t + kTmemO, t + kTmemS + kAttTile / 2 + 8 * c, d + (uint64_t)(128 * c), idesc_o, 1u);
+        }
       };
       int stage = 0, ahead = 0;          // of tile i; of the next tile whose S is wanted
       uint32_t ahead_phase = 0;
@@ -392,8 +415,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     const int node = (by_rows ? g * p.nodes_per_tile : 0) + r / p.group, head = kvh * p.group + r % p.group;
     const bool valid = r < p.nodes_per_tile * p.group && node < nodes;
     const int tok = first + n0 + (valid ? node : 0);
-    if (valid && (by_rows || g == 0)) {
-      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
+    if (valid && (LOW || by_rows || g == 0)) {
+      const uint4 *src = reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(LOW && g ? p.q_low : a.q) + (size_t)tok * a.q_stride + (size_t)head * HD);
       uint4 q[HD / 8];
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c) q[c] = src[c];
@@ -484,10 +507,27 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         const float base = fabsf(top) < INFINITY || top == -INFINITY ? (m == -INFINITY ? 0.f : m) : NAN;
         float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
         const float2 c2 = make_float2(p.c, p.c), base2 = make_float2(-base, -base);
+        if (LOW) {
+#pragma unroll
+          for (int h = 0; h < kAttTile; h += 16) {
+            uint32_t hi[8], lo[8];
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float2 x = fma2(make_float2(s[h + j], s[h + j + 1]), c2, base2);
+              const float2 e = make_float2(ex2(x.x), ex2(x.y));
+              sum[(j >> 1) & 1] = add2(sum[(j >> 1) & 1], e);
+              const uint32_t top16 = pack_bf16(e.x, e.y);
+              const float2 rest = add2(e, make_float2(-__uint_as_float(top16 << 16), -__uint_as_float(top16 & 0xffff0000u)));
+              hi[j >> 1] = top16, lo[j >> 1] = pack_bf16(rest.x, rest.y);
+            }
+            tmem_st8(ts + (h >> 1), hi);
+            tmem_st8(ts + ((kAttTile + h) >> 1), lo);
+          }
+        }
         // Every eighth pair goes through the FMA units instead of the exponential unit, which takes 8 cycles for a warp's 32
         // (64 x 64 tokens over 4096: 293 us instead of 300).
 #pragma unroll
-        for (int h = 0; h < kAttTile; h += 32) {
+        for (int h = 0; h < (LOW ? 0 : kAttTile); h += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
@@ -757,16 +797,17 @@ namespace {
 // fill two CTAs on every SM.
 constexpr int kJoinTiles = 4, kMergeTiles = 8;
 struct AttPlan {
-  int group, nodes_per_tile, q_pairs, n_splits, tiles_per_split;
+  int group, nodes_per_tile, nodes_per_cta, q_blocks, n_splits, tiles_per_split;
 };
-AttPlan plan_of(const gptoss_tree_attention_args &a) {
+AttPlan plan_of(const gptoss_tree_attention_args &a, bool low) {
   AttPlan p;
   p.group = a.n_q_heads / a.n_kv_heads;
   p.nodes_per_tile = kAttRows / p.group;
-  p.q_pairs = (a.max_nodes + 2 * p.nodes_per_tile - 1) / (2 * p.nodes_per_tile);
+  p.nodes_per_cta = (low ? 1 : 2) * p.nodes_per_tile;
+  p.q_blocks = (a.max_nodes + p.nodes_per_cta - 1) / p.nodes_per_cta;
   int device = 0, sms = kSmCountFallback;
   if (cudaGetDevice(&device) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-  const long long items = (long long)a.n_seqs * a.n_kv_heads * p.q_pairs;
+  const long long items = (long long)a.n_seqs * a.n_kv_heads * p.q_blocks;
   // the cached tokens that a tree can reach: with a window, as many as its first token sees
   const long long reach = a.window > 0 && a.window - 1 < a.max_ctx ? a.window - 1 : a.max_ctx;
   const long long tiles = (reach + a.max_nodes + kAttTile - 1) / kAttTile;
@@ -795,18 +836,18 @@ uint64_t workspace_of(const gptoss_tree_attention_args &a, int n_splits) {
   return n_splits <= kMaxClusterSplits ? 0 : (uint64_t)n_splits * a.n_tokens * a.n_q_heads * (a.head_dim + 2) * sizeof(float);
 }
 
-template <int HD>
+template <int HD, bool LOW>
 cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
   static std::atomic<uint64_t> configured{0};  // devices (of the first 64) on which the kernel may have its shared memory
   int device = 0;
   cudaError_t e = cudaGetDevice(&device);
   if (e == cudaSuccess && (device >= 64 || !(configured.load(std::memory_order_relaxed) >> device & 1))) {
-    e = cudaFuncSetAttribute(tree_attention_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
+    e = cudaFuncSetAttribute(tree_attention_kernel<HD, LOW>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kAttSmem);
     if (e == cudaSuccess && device < 64) configured.fetch_or(1ull << device, std::memory_order_relaxed);
   }
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_pairs * p.n_splits));
+  cfg.gridDim = dim3((unsigned)(p.a.n_seqs * p.a.n_kv_heads * p.q_blocks * p.n_splits));
   cfg.blockDim = dim3(kAttThreads);
   cfg.dynamicSmemBytes = kAttSmem;
   cfg.stream = s;
@@ -825,34 +866,13 @@ cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
   cfg.attrs = attr;
   cfg.numAttrs = n;
   count_launch();
-  e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<HD>, p);
+  e = cudaLaunchKernelEx(&cfg, tree_attention_kernel<HD, LOW>, p);
   if (e != cudaSuccess || p.n_splits <= kMaxClusterSplits) return e;
   return launch_chain(tree_merge_kernel<HD>, dim3(p.a.n_seqs * p.a.max_nodes, (p.a.n_q_heads + 7) / 8), dim3(256), 0, s,
                       p.a, p.n_splits);
 }
 
-}  // namespace
-
-extern "C" uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *a) {
-  return a && countable(*a) ? workspace_of(*a, plan_of(*a).n_splits) : 0;
-}
-
-extern "C" int gptoss_serving_status(void) {
-  int st[kStatusWords];
-  cudaError_t e = cudaDeviceSynchronize();
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(st, g_serving_status, sizeof st);
-  if (e != cudaSuccess) return serving_fail(GPTOSS_ERR_CUDA, "gptoss_serving_status", e);
-  if (st[0] == 0) return GPTOSS_OK;
-  char msg[128];
-  snprintf(msg, sizeof msg, "device-side bounded wait gave up in a serving operator (site 0x%x)", st[1]);
-  memset(st, 0, sizeof st);
-  cudaMemcpyToSymbol(g_serving_status, st, sizeof st);
-  return serving_fail(GPTOSS_ERR_TIMEOUT, msg);
-}
-
-extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream) {
-  if (!args) return serving_fail(GPTOSS_ERR_BAD_ARG, "null arguments");
-  const gptoss_tree_attention_args &a = *args;
+int tree_attention(const gptoss_tree_attention_args &a, const void *q_low, cudaStream_t stream) {
   if (a.n_seqs < 0 || a.n_tokens < 0 || a.max_nodes < 0 || a.max_ctx < 0)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "negative count");
   if (a.head_dim != 32 && a.head_dim != 64) return serving_fail(GPTOSS_ERR_BAD_ARG, "head_dim must be 32 or 64");
@@ -871,24 +891,65 @@ extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, voi
     return serving_fail(GPTOSS_ERR_BAD_ARG, "q, caches and out must be 16-byte aligned, token strides multiples of 8 elements");
   if (a.q_stride < (int64_t)a.n_q_heads * a.head_dim || a.out_stride < (int64_t)a.n_q_heads * a.head_dim)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "token stride below n_q_heads * head_dim");
-  const AttPlan plan = plan_of(a);
+  const AttPlan plan = plan_of(a, q_low != nullptr);
   const uint64_t need = workspace_of(a, plan.n_splits);
   if (need && (!a.workspace || !aligned16(a.workspace) || a.workspace_bytes < need))
     return serving_fail(GPTOSS_ERR_BAD_ARG, "workspace missing, misaligned or below gptoss_tree_attention_workspace()");
-  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff || (int64_t)a.n_seqs * a.n_kv_heads * plan.q_pairs * plan.n_splits > 0x7fffffff ||
+  if ((int64_t)a.n_seqs * a.max_nodes > 0x7fffffff || (int64_t)a.n_seqs * a.n_kv_heads * plan.q_blocks * plan.n_splits > 0x7fffffff ||
       (int64_t)a.cache_rows * a.n_kv_heads > 0x7fffffff)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "too many drafted tokens or cache rows");
   AttParams p;
   p.a = a;
-  p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.q_pairs = plan.q_pairs;
+  p.q_low = q_low;
+  p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.nodes_per_cta = plan.nodes_per_cta, p.q_blocks = plan.q_blocks;
   p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
   p.in_cluster = plan.n_splits > 1 && plan.n_splits <= kMaxClusterSplits;
   p.c = a.scale * 1.44269504f;
   const uint64_t slabs = (uint64_t)a.cache_rows * a.n_kv_heads;
   cudaError_t e = encode_map_3d(&p.map_k, a.k_cache, a.head_dim, a.max_seq, slabs, kAttTile);
   if (e == cudaSuccess) e = encode_map_3d(&p.map_v, a.v_cache, a.head_dim, a.max_seq, slabs, kAttTile);
-  if (e == cudaSuccess) e = a.head_dim == 64 ? launch_tree<64>(p, static_cast<cudaStream_t>(stream)) : launch_tree<32>(p, static_cast<cudaStream_t>(stream));
+  if (e == cudaSuccess) {
+    if (q_low)
+      e = a.head_dim == 64 ? launch_tree<64, true>(p, stream) : launch_tree<32, true>(p, stream);
+    else
+      e = a.head_dim == 64 ? launch_tree<64, false>(p, stream) : launch_tree<32, false>(p, stream);
+  }
   return e == cudaSuccess ? GPTOSS_OK : serving_fail(GPTOSS_ERR_CUDA, "tree attention launch", e);
+}
+
+}  // namespace
+
+namespace gptoss {
+
+uint64_t tree_attention_fine_workspace(const gptoss_tree_attention_args &a) { return countable(a) ? workspace_of(a, plan_of(a, true).n_splits) : 0; }
+
+int tree_attention_fine(const gptoss_tree_attention_args &a, const void *q_low, cudaStream_t stream) {
+  if (!q_low || !aligned16(q_low)) return serving_fail(GPTOSS_ERR_BAD_ARG, "second term of the queries missing or misaligned");
+  return tree_attention(a, q_low, stream);
+}
+
+}  // namespace gptoss
+
+extern "C" uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_args *a) {
+  return a && countable(*a) ? workspace_of(*a, plan_of(*a, false).n_splits) : 0;
+}
+
+extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream) {
+  if (!args) return serving_fail(GPTOSS_ERR_BAD_ARG, "null arguments");
+  return tree_attention(*args, nullptr, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int gptoss_serving_status(void) {
+  int st[kStatusWords];
+  cudaError_t e = cudaDeviceSynchronize();
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(st, g_serving_status, sizeof st);
+  if (e != cudaSuccess) return serving_fail(GPTOSS_ERR_CUDA, "gptoss_serving_status", e);
+  if (st[0] == 0) return GPTOSS_OK;
+  char msg[128];
+  snprintf(msg, sizeof msg, "device-side bounded wait gave up in a serving operator (site 0x%x)", st[1]);
+  memset(st, 0, sizeof st);
+  cudaMemcpyToSymbol(g_serving_status, st, sizeof st);
+  return serving_fail(GPTOSS_ERR_TIMEOUT, msg);
 }
 
 extern "C" int gptoss_cache_commit(void *k_cache, void *v_cache, int n_layers, int cache_rows, int n_kv_heads, int max_seq,

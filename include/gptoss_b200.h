@@ -295,8 +295,8 @@ int gptoss_serving_status(void);
  * in the cache, drafted token i in slot ctx_len[b] + i.  Query i attends to every cached token and to the drafted tokens
  * j whose bit is set in its mask (bit j & 31 of word j >> 5; its own bit included, if it shall see itself).  With a
  * window > 0 it attends only to tokens less than `window` positions before its own, the position of a drafted token
- * being ctx_len[b] + depth (run.cpp:582).  Softmax in fp32, the sink joins the denominator only (run.cpp:588-591); a
- * query that attends to nothing gets zeros.  K and V rows that no query of the tree attends to, and masked ones, may
+ * being ctx_len[b] + depth (run.cpp:582).  Softmax in fp32, the sink joins the denominator only (run.cpp:588-591); the weights are
+ * rounded to bf16 for their product with V.  A query that attends to nothing gets zeros.  K and V rows that no query of the tree attends to, and masked ones, may
  * hold anything, NaN included.  Rows of out behind offsets[n_seqs] are left as they were.
  * bf16: q [n_tokens][n_q_heads][head_dim], token stride q_stride elements (a multiple of 8); caches
  * [cache_rows][n_kv_heads][max_seq][head_dim]; out like q.  All 16-byte aligned.  head_dim 32 or 64, 1 to 8 query heads
@@ -470,8 +470,9 @@ int gptoss_model_step_seqs(gptoss_model *m, const int *tokens_host, const int *r
  * last cached token.  Every drafted token is run at position ctx + depth, seeing the cached tokens, its ancestors and
  * itself; next_tokens_host (may be NULL) gets the greedy token that follows each of them.  Their K and V stay in the slots
  * behind the cached ones until gptoss_model_accept keeps some.  With a chain per sequence this is also a prompt in pieces.
- * The attention rounds queries and weights to bf16 (the one-token step keeps them in two terms), so logits agree with those
- * of one-token steps to bf16 rounding, not bit for bit.  Single-GPU models only. */
+ * The attention keeps queries and weights in two bf16 terms as the one-token step does (gptoss_tree_attention: one), but adds
+ * in another order, so logits agree with those of one-token steps to fp32 rounding, not bit for bit; where the difference
+ * carries a value over the edge of its rounding to bf16, to that.  Single-GPU models only. */
 int gptoss_model_step_tree(gptoss_model *m, int n_seqs, const int *rows_host, const int *ctx_host, const int *offsets_host,
                            const int *tokens_host, const int *parents_host, int *next_tokens_host);
 /* Keeps the drafted tokens path_host[offsets_host[b] .. offsets_host[b+1]) (ascending indices of the tree of the last
