@@ -906,9 +906,10 @@ int gptoss_model_lora_create(gptoss_model *m, int n_adapters, int rank) {
   cudaError_t e = cudaSuccess;
   for (auto &x : parts) {
     if (e == cudaSuccess) e = cudaMalloc(x.p, x.bytes);
-    if (e == cudaSuccess) e = cudaMemset(*x.p, 0, x.bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(*x.p, 0, x.bytes, m->stream);  // ahead of any step, which runs there too
   }
   if (e != cudaSuccess) {
+    cudaStreamSynchronize(m->stream);
     for (auto &x : parts) {
       cudaFree(*x.p);
       *x.p = nullptr;
