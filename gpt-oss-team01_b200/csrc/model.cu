@@ -534,7 +534,7 @@ int gptoss_model_layer_attention(gptoss_model *m, int layer) {
       a.q = q16, a.k_cache = kc, a.v_cache = vc, a.out = m->att, a.sinks = m->sinks + l * nq;
       a.window = c.sliding_window > 0 && l % 2 == 0 ? c.sliding_window : 0;  // run.cpp:582
       a.workspace = m->tree_work, a.workspace_bytes = m->tree_work_bytes;
-      if ((rc = tree_attention_fine(a, q16 + (size_t)B * qd, s))) return m->fail(rc, gptoss_serving_last_error());
+      if ((rc = tree_attention_fine(a, q16 + (size_t)B * qd, m->status, s))) return m->fail(rc, gptoss_serving_last_error());
     } else {
       MK(launch_qkv_rope_store(m->qkv, m->cos_t, m->sin_t, pos, B, nq, nkv, hd, (int)S, m->q, kc, vc, m->step_rows,
                                m->step_pos_rows, s));
@@ -645,7 +645,7 @@ int gptoss_model_step_end(gptoss_model *m, int *next_tokens_host) {
   m->step_B = 0;
   if (st[0] != 0) {
     cudaMemset(m->status, 0, sizeof st);
-    return m->fail(GPTOSS_ERR_TIMEOUT, "device-side bounded wait gave up in a dense GEMM");
+    return m->fail(GPTOSS_ERR_TIMEOUT, "device-side bounded wait gave up in a dense GEMM or in the attention of drafted tokens");
   }
   rc = gptoss_ctx_status(m->moe);
   return rc ? m->fail(rc, gptoss_last_error(m->moe)) : GPTOSS_OK;
@@ -836,18 +836,9 @@ int gptoss_model_step_tree(gptoss_model *m, int n_seqs, const int *rows_host, co
     if ((rc = gptoss_model_layer_attention(m, l))) break;
     rc = gptoss_model_layer_moe_push(m, l);
   }
-  int waits[kStatusWords] = {};
-  if (!rc) {
-    const cudaError_t e = serving_status_async(waits, m->stream);
-    if (e != cudaSuccess) rc = m->fail(GPTOSS_ERR_CUDA, "status of the attention", e);
-  }
   if (!rc) rc = gptoss_model_step_end(m, next_tokens_host);  // synchronises the stream
   m->step_B = 0;
   m->step_tree = false;
-  if (!rc && waits[0] != 0) {
-    gptoss_serving_status();  // takes the report back
-    rc = m->fail(GPTOSS_ERR_TIMEOUT, "device-side bounded wait gave up in the tree attention");
-  }
   return rc;
 }
 

@@ -76,6 +76,7 @@ struct AttParams {
   CUtensorMap map_k, map_v;  // 3-D (dim, slot, cache row * kv head), box {64, 64, 1}
   gptoss_tree_attention_args a;
   const void *q_low;         // second bf16 term of the queries, laid out like a.q (the kernel with LOW)
+  int *status;               // where a wait that gives up is noted; null: in g_serving_status
   int group, nodes_per_tile, nodes_per_cta, q_blocks, n_splits, tiles_per_split;
   bool in_cluster;           // the shares of the context are a cluster and join in shared memory
   float c;                   // scale * log2(e)
@@ -205,19 +206,20 @@ __device__ __forceinline__ uint32_t bf16_finite_part(uint32_t pair) {
 }
 
 // mbar_wait in line: around a call the compiler would spill the row of scores that a softmax thread holds.
-__device__ __forceinline__ void wait_addr(uint32_t addr, uint32_t parity, volatile int *abort_flag, int site) {
+__device__ __forceinline__ void wait_addr(uint32_t addr, uint32_t parity, volatile int *abort_flag, int *status, int site) {
   uint32_t i = 0;
   while (!mbar_try_wait(addr, parity)) {
     if (*abort_flag) return;
     if (++i == kSpinLimit) {
       *abort_flag = 1;
-      if (atomicCAS(g_serving_status, 0, kDevErrTimeout) == 0) g_serving_status[1] = site, g_serving_status[2] = (int)blockIdx.x;
+      if (status == nullptr) status = g_serving_status;
+      if (atomicCAS(status, 0, kDevErrTimeout) == 0) status[1] = site, status[2] = (int)blockIdx.x;
       return;
     }
   }
 }
-__device__ __forceinline__ void wait_warp(uint64_t *bar, uint32_t parity, int *abort_flag, int site) {
-  wait_addr(smem_u32(bar), parity, abort_flag, site);
+__device__ __forceinline__ void wait_warp(uint64_t *bar, uint32_t parity, int *abort_flag, int *status, int site) {
+  wait_addr(smem_u32(bar), parity, abort_flag, status, site);
   __syncwarp();
 }
 
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
     int i = 0;
     for (; i < n_tiles; ++i) {
       const int st = i % kAttStages;
-      if (i >= kAttStages) wait_warp(&ctrl->empty[st], ((i / kAttStages) & 1) ^ 1, &ctrl->abort, 0x2000 | st);
+      if (i >= kAttStages) wait_warp(&ctrl->empty[st], ((i / kAttStages) & 1) ^ 1, &ctrl->abort, p.status, 0x2000 | st);
       if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int *>(&ctrl->abort))) break;
       if (elect_one()) {
         const uint32_t full = smem_u32(&ctrl->full[st]);
@@ -364,7 +366,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         if (++ahead == kAttStages) ahead = 0, ahead_phase ^= 1;
       };
       for (int grp = 0; grp < 2 && (by_rows ? 0 : grp) < n_tiles; ++grp) {
-        if (grp == 0 || !by_rows) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2200);
+        if (grp == 0 || !by_rows) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, p.status, 0x2200);
         tc_fence_after();
         scores(grp, ahead);
         if (grp == 1 || !by_rows) advance();
@@ -372,12 +374,12 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
       if (by_rows) {
         for (int i = 0; i < n_tiles; ++i) {
           const bool more = i + 1 < n_tiles;
-          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2201);
-          wait_addr(p_full, i & 1, &ctrl->abort, 0x2500);
+          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, p.status, 0x2201);
+          wait_addr(p_full, i & 1, &ctrl->abort, p.status, 0x2500);
           tc_fence_after();
           output(0, stage, i > 0);
           if (more) scores(0, ahead);
-          wait_addr(p_full + 8, i & 1, &ctrl->abort, 0x2501);
+          wait_addr(p_full + 8, i & 1, &ctrl->abort, p.status, 0x2501);
           tc_fence_after();
           output(1, stage, i > 0);
           umma_commit(empty + 8 * stage);
@@ -390,8 +392,8 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
       } else {
         for (int i = 0; i < n_tiles; ++i) {
           const bool more = i + 2 < n_tiles;
-          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, 0x2202);
-          wait_addr(p_full + 8 * (i & 1), (i >> 1) & 1, &ctrl->abort, 0x2502);
+          if (more) wait_addr(full + 8 * ahead, ahead_phase, &ctrl->abort, p.status, 0x2202);
+          wait_addr(p_full + 8 * (i & 1), (i >> 1) & 1, &ctrl->abort, p.status, 0x2502);
           tc_fence_after();
           output(i & 1, stage, i > 1);
           umma_commit(empty + 8 * stage);
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         // half of slot r / 2 of this tile: non-finite elements of V become zeros, and the slot is noted if anyone can see it
         // (two groups on one tile both look at all of it: what the second still finds, the first has written as well)
         const int st = i % kAttStages;
-        wait_warp(&ctrl->full[st], (i / kAttStages) & 1, &ctrl->abort, 0x2700);
+        wait_warp(&ctrl->full[st], (i / kAttStages) & 1, &ctrl->abort, p.status, 0x2700);
         uint4 *vr = reinterpret_cast<uint4 *>(smem + 2 * kAttQBytes + (kAttStages + st) * kAttTileBytes + r * 64);
         int bad = 0;
 #pragma unroll
@@ -467,7 +469,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      wait_addr(s_full, k & 1, &ctrl->abort, 0x2600);
+      wait_addr(s_full, k & 1, &ctrl->abort, p.status, 0x2600);
       __syncwarp();
       tc_fence_after();
       if (live) {
@@ -546,7 +548,7 @@ __global__ void __launch_bounds__(kAttThreads, kAttCtasPerSm) tree_attention_ker
       if (lane == 0) mbar_arrive(p_full);
     }
     // ---- result of this share of the context ----
-    wait_warp(&ctrl->retired, 0, &ctrl->abort, 0x2900);
+    wait_warp(&ctrl->retired, 0, &ctrl->abort, p.status, 0x2900);
     tc_fence_after();
     float o[HD];
 #pragma unroll
@@ -773,10 +775,6 @@ __global__ void __launch_bounds__(128) cache_commit_kernel(uint4 *__restrict__ k
 
 }  // namespace
 
-cudaError_t serving_status_async(int *host, cudaStream_t s) {
-  return cudaMemcpyFromSymbolAsync(host, g_serving_status, kStatusWords * sizeof(int), 0, cudaMemcpyDeviceToHost, s);
-}
-
 int serving_fail(int code, const char *msg, cudaError_t e) {
   if (e != cudaSuccess)
     snprintf(g_serving_error, sizeof g_serving_error, "%s: %s (%s)", msg, cudaGetErrorName(e), cudaGetErrorString(e));
@@ -872,7 +870,7 @@ cudaError_t launch_tree(const AttParams &p, cudaStream_t s) {
                       p.a, p.n_splits);
 }
 
-int tree_attention(const gptoss_tree_attention_args &a, const void *q_low, cudaStream_t stream) {
+int tree_attention(const gptoss_tree_attention_args &a, const void *q_low, int *status, cudaStream_t stream) {
   if (a.n_seqs < 0 || a.n_tokens < 0 || a.max_nodes < 0 || a.max_ctx < 0)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "negative count");
   if (a.head_dim != 32 && a.head_dim != 64) return serving_fail(GPTOSS_ERR_BAD_ARG, "head_dim must be 32 or 64");
@@ -900,7 +898,7 @@ int tree_attention(const gptoss_tree_attention_args &a, const void *q_low, cudaS
     return serving_fail(GPTOSS_ERR_BAD_ARG, "too many drafted tokens or cache rows");
   AttParams p;
   p.a = a;
-  p.q_low = q_low;
+  p.q_low = q_low, p.status = status;
   p.group = plan.group, p.nodes_per_tile = plan.nodes_per_tile, p.nodes_per_cta = plan.nodes_per_cta, p.q_blocks = plan.q_blocks;
   p.n_splits = plan.n_splits, p.tiles_per_split = plan.tiles_per_split;
   p.in_cluster = plan.n_splits > 1 && plan.n_splits <= kMaxClusterSplits;
@@ -923,9 +921,9 @@ namespace gptoss {
 
 uint64_t tree_attention_fine_workspace(const gptoss_tree_attention_args &a) { return countable(a) ? workspace_of(a, plan_of(a, true).n_splits) : 0; }
 
-int tree_attention_fine(const gptoss_tree_attention_args &a, const void *q_low, cudaStream_t stream) {
+int tree_attention_fine(const gptoss_tree_attention_args &a, const void *q_low, int *status, cudaStream_t stream) {
   if (!q_low || !aligned16(q_low)) return serving_fail(GPTOSS_ERR_BAD_ARG, "second term of the queries missing or misaligned");
-  return tree_attention(a, q_low, stream);
+  return tree_attention(a, q_low, status, stream);
 }
 
 }  // namespace gptoss
@@ -936,7 +934,7 @@ extern "C" uint64_t gptoss_tree_attention_workspace(const gptoss_tree_attention_
 
 extern "C" int gptoss_tree_attention(const gptoss_tree_attention_args *args, void *stream) {
   if (!args) return serving_fail(GPTOSS_ERR_BAD_ARG, "null arguments");
-  return tree_attention(*args, nullptr, static_cast<cudaStream_t>(stream));
+  return tree_attention(*args, nullptr, nullptr, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int gptoss_serving_status(void) {
