@@ -6,18 +6,21 @@
 * ``lora_apply``      low-rank adapters of many requests at once beside a shared projection
 * ``route_experts``   experts from softmax / sigmoid scores with a balancing bias, groups, renormalised weights
                       (``MoEBlock.forward_routed`` runs the expert GEMMs on the result)
+* ``status``          whether the calls so far ran as they should (synchronises)
 
 Each call runs on the device of its tensors, asynchronously on ``stream`` (default: that device's current stream); scratch
 comes from torch's allocator, so calls on different streams and captured graphs have their own.  As with torch's own
 operators, a tensor that belongs to another stream than the one it is used on is the caller's to keep alive and to order
-(``record_stream``, ``wait_stream``); what a call returns belongs to the stream it ran on.  Errors raise ``GptossError``.
-Nothing is kept between calls.
+(``record_stream``, ``wait_stream``); what a call returns belongs to the stream it ran on.  Refused arguments and failed launches
+raise ``GptossError``; a wait on the GPU that gives up (its results mean nothing then) is noted there, and ``status`` raises it.
+Nothing else is kept between calls.
 
 The calls are short on the GPU (from 2 us), so their host side counts: csrc/serving_torch.cpp looks the tensors over,
 allocates and calls the C ABI (3 to 5 us a call; in Python that was 8 to 13).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import importlib.util
 
@@ -58,6 +61,16 @@ def _on(stream, t, call, *args):
         _bad("the stream belongs to another device than the tensors")
     with torch.cuda.stream(stream):
         return call(t, *args)
+
+
+def status(device=None):
+    """Waits for all work of a device (default: the current one) and raises GptossError if a kernel of these operators gave up on a
+    bounded wait since the last such call, or if the device reports an error."""
+    lib = capi.load()
+    with contextlib.nullcontext() if device is None else torch.cuda.device(device):
+        rc = lib.gptoss_serving_status()
+    if rc != capi.OK:
+        raise GptossError(rc, lib.gptoss_serving_last_error().decode())
 
 
 def tree_masks(parents, max_nodes=None):
