@@ -167,8 +167,13 @@ class Model:
         """Greedy continuations of ``prompts`` (lists of ids, any lengths) in steps over drafted tokens.  ``draft(history)``
         proposes what may follow the ids seen so far: (tokens, parents), parents counting within the proposal, -1 for a
         token that follows the history directly.  Returns int32 [B, n_generate]; the number of steps does not change the
-        result (up to bf16 rounding of near-ties), only the time."""
+        result (up to bf16 rounding of near-ties), only the time.  More prompts than max_batch are taken in turn."""
         B = len(prompts)
+        if B == 0 or n_generate == 0:
+            return np.zeros((B, n_generate), np.int32)
+        if B > self.max_batch:
+            return np.concatenate([self.generate_drafted(prompts[i:i + self.max_batch], n_generate, draft)
+                                   for i in range(0, B, self.max_batch)])
         hist, ctx = [list(map(int, p)) for p in prompts], np.zeros(B, np.int32)
         room = max(1, min(256, self.max_batch // B))
         goal = [len(h) + n_generate for h in hist]
