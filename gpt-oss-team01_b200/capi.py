@@ -5,8 +5,10 @@ There is no CPU fallback: if the library has not been built, ``load()`` raises.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.metadata
 import importlib.util
 import subprocess
+import sys
 import sysconfig
 from pathlib import Path
 
@@ -21,8 +23,18 @@ SOURCES = ["routing.cu", "router.cu", "grouped_gemm.cu", "grouped_gemm_pair.cu",
 HEADERS = ["common.cuh", "kernels.cuh", "serving.cuh", "tcgen05.cuh", "gemm_tile.cuh", "../../include/gptoss_b200.h"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-shared", "--threads", "4"]
-# the serving operators' binding to torch tensors (serving.py), a Python module
-TORCH_LIB_PATH = CSRC / "_serving_torch.so"
+
+
+def _torch_lib_path():
+    """The serving operators' binding to torch tensors (serving.py), a Python module; named after the Python and the torch it is
+    compiled against, as it works with no other.  None without torch: the library itself does not need it."""
+    try:
+        return CSRC / f"_serving_torch.{sys.implementation.cache_tag}-torch{importlib.metadata.version('torch')}.so"
+    except importlib.metadata.PackageNotFoundError:
+        return None
+
+
+TORCH_LIB_PATH = _torch_lib_path()
 TORCH_SOURCES = ["serving_torch.cpp"]
 
 OK, ERR_BAD_ARG, ERR_CUDA, ERR_TIMEOUT, ERR_UNSUPPORTED, ERR_STATE = range(6)
@@ -100,7 +112,7 @@ def _lib_stale() -> bool:
 
 
 def _torch_lib_stale() -> bool:
-    return _stale(TORCH_LIB_PATH, TORCH_SOURCES + HEADERS[-1:])
+    return TORCH_LIB_PATH is not None and _stale(TORCH_LIB_PATH, TORCH_SOURCES + HEADERS[-1:])
 
 
 def needs_build() -> bool:
@@ -115,12 +127,12 @@ def _nvcc(args):
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compiles the library for sm_100a and the torch binding with nvcc (works without a GPU)."""
+    """Compiles the library for sm_100a and, where torch is installed, its binding to torch with nvcc (works without a GPU)."""
     if force or _lib_stale():
         out = _nvcc([*(["-Xptxas", "-v"] if verbose else []), *NVCC_FLAGS, "-o", str(LIB_PATH), *SOURCES])
         if verbose:
             print(out)
-    if force or _torch_lib_stale():
+    if TORCH_LIB_PATH is not None and (force or _torch_lib_stale()):
         torch_dir = Path(importlib.util.find_spec("torch").origin).parent
         _nvcc(["-x", "c++", "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-shared", "-I", sysconfig.get_paths()["include"],
                "-I", str(torch_dir / "include"), "-o", str(TORCH_LIB_PATH), *TORCH_SOURCES, "-L", str(torch_dir / "lib"),

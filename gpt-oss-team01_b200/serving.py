@@ -38,8 +38,8 @@ _binding = None
 def _bind():
     """The compiled binding, with the C functions of the loaded library."""
     global _binding
-    if not capi.TORCH_LIB_PATH.exists():
-        raise RuntimeError(f"{capi.TORCH_LIB_PATH} is missing: run `python -c 'import __graft_entry__ as e; e.build()'` first")
+    if capi.TORCH_LIB_PATH is None or not capi.TORCH_LIB_PATH.exists():
+        raise RuntimeError(f"{capi.TORCH_LIB_PATH or 'the binding to torch'} is missing: run `python -c 'import __graft_entry__ as e; e.build()'` first")
     lib = capi.load()
     spec = importlib.util.spec_from_file_location("_serving_torch", capi.TORCH_LIB_PATH)
     mod = importlib.util.module_from_spec(spec)
