@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -39,10 +40,13 @@ struct NoGil {
   ~NoGil() { PyEval_RestoreThread(state); }
 };
 
-// o as a tensor of that type and number of dimensions on cuda device `dev` (-1: any)
+// o as a tensor of that type and number of dimensions on cuda device `dev` (-1: any).  The operators have no backward pass: as
+// torch's own operators without one refuse it, a tensor that asks for its gradient is refused, not silently left without.
 const at::Tensor &view(PyObject *o, const char *name, at::ScalarType type, int64_t ndim, int dev) {
   if (THPVariable_Check(o)) {
     const at::Tensor &t = THPVariable_Unpack(o);
+    if (t.requires_grad() && c10::GradMode::is_enabled())
+      bad(std::string(name) + " requires a gradient, which the serving operators do not give: detach it, or call under torch.no_grad()");
     if (t.layout() == at::kStrided && t.scalar_type() == type && t.dim() == ndim && t.is_cuda() && (dev < 0 || t.get_device() == dev)) return t;
   }
   bad(std::string(name) + " must be a " + at::toString(type) + " tensor of " + std::to_string(ndim) + " dimensions on " +

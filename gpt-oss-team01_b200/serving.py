@@ -13,7 +13,8 @@ comes from torch's allocator, so calls on different streams and captured graphs 
 operators, a tensor that belongs to another stream than the one it is used on is the caller's to keep alive and to order
 (``record_stream``, ``wait_stream``); what a call returns belongs to the stream it ran on.  Refused arguments and failed launches
 raise ``GptossError``; a wait on the GPU that gives up (its results mean nothing then) is noted there, and ``status`` raises it.
-Nothing else is kept between calls.
+Nothing else is kept between calls.  There is no backward pass: tensors that require a gradient are refused while gradients are
+recorded (they pass under ``torch.no_grad()``).
 
 The calls are short on the GPU (from 2 us), so their host side counts: csrc/serving_torch.cpp looks the tensors over,
 allocates and calls the C ABI (3 to 5 us a call; in Python that was 8 to 13).
