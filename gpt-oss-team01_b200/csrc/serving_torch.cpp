@@ -83,6 +83,11 @@ void check(int rc) {
   if (rc) throw Refused{rc, f_last_error()};
 }
 
+// A tensor of the caller's that the call has written: its version counts up, so that a graph that saved it notices.
+void written(const at::Tensor &t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // body(args) with C++ exceptions turned into Python's
 template <typename F>
 PyObject *guarded(Py_ssize_t n_args, Py_ssize_t want, F body) {
@@ -150,6 +155,7 @@ PyObject *tree_attention(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
       }
       check(f_tree(&a, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream()));
     }
+    if (given) written(out);
     return given ? Py_NewRef(o[13]) : THPVariable_Wrap(std::move(out));
   });
 }
@@ -178,6 +184,7 @@ PyObject *cache_commit(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
                      static_cast<const int *>(path.const_data_ptr()), n_path, max_path,
                      c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream()));
     }
+    written(k), written(v);
     Py_RETURN_NONE;
   });
 }
@@ -215,6 +222,7 @@ PyObject *lora_apply(PyObject *, PyObject *const *o, Py_ssize_t n_args) {
       }
       check(f_lora(&g, c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream()));
     }
+    written(out);
     return Py_NewRef(result);
   });
 }

@@ -59,3 +59,31 @@ def test_without_recording_everything_passes(op):
             got = call(**{k: t.clone().requires_grad_() if t.is_floating_point() else t.clone() for k, t in tensors.items()})
         for g, p in zip(*[r if isinstance(r, tuple) else (r,) for r in (got, plain)]):
             assert g is p or torch.equal(g, p)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("op,names", [("tree_attention", ("out",)), ("cache_commit", ("k_cache", "v_cache")), ("lora_apply", ("y",))])
+def test_what_a_call_writes_counts_its_version_up(op, names):
+    """A graph that saved such a tensor before the call refuses to run backward; the other tensors keep their versions."""
+    call, tensors = next((c, t) for n, c, t in calls("cuda") if n == op)
+    for name in names:
+        w = torch.ones_like(tensors[name], requires_grad=True)
+        loss = (w * tensors[name]).sum()  # saves the tensor
+        before = {k: t._version for k, t in tensors.items()}
+        call(**tensors)
+        for k, t in tensors.items():
+            assert t._version > before[k] if k in names else t._version == before[k], k
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    with torch.inference_mode():
+        call(**{k: t.clone() for k, t in tensors.items()})  # inference tensors have no version
+
+
+@pytest.mark.gpu
+def test_a_refused_call_writes_nothing():
+    from gptoss_b200 import moe
+    call, tensors = next((c, t) for n, c, t in calls("cuda") if n == "lora_apply")
+    before = tensors["y"]._version
+    with pytest.raises(moe.GptossError):
+        call(**{**tensors, "ids": tensors["ids"].long()})
+    assert tensors["y"]._version == before
