@@ -56,3 +56,34 @@ def test_drafted_decoding_follows_one_token_decoding(greedy, checkpoint, drafter
     out = m.generate_drafted([prompt] + [synth.uniform_ids(i, 9, 11 + i, cfg.vocab_size).tolist() for i in range(others)], SURE, draft)
     assert out[0].tolist() == want[:SURE]
     m.close()
+
+
+@pytest.mark.parametrize("B,ctx", [(1, 3000), (3, 2500), (40, 1500), (80, 600)])
+def test_drafted_and_one_token_steps_agree_over_long_contexts(tmp_path, B, ctx):
+    """Both kinds of step on the same cache, whose contexts the attention of drafted tokens cuts into shares (by the number of
+    sequences: through memory, in clusters, not at all).  They differ by the order of fp32 sums, which now and then carries an element
+    over the edge of its rounding to bf16: less than the 4e-3 that bf16 rounding throughout is allowed in test_gpu_model.py."""
+    from gptoss_b200 import model
+    cfg = binfmt.config_7m(4096)
+    ckpt = tmp_path / "7m.bin"
+    binfmt.write_synthetic(str(ckpt), cfg, 21)
+    m = model.Model(cfg, max_batch=256, max_seq=4096)
+    m.load_bin(ckpt)
+    rows, at, length = np.arange(B), np.zeros(B, np.int32), np.array([ctx - 5 * b for b in range(B)])
+    ids = synth.uniform_ids(8, 3, B * (ctx + 1), cfg.vocab_size).reshape(B, ctx + 1).astype(np.int32)
+    while (at < length).any():  # the contexts, in pieces
+        live = np.flatnonzero(at < length)
+        n = [int(min(256 // len(live), length[b] - at[b])) for b in live]
+        m.step_tree([ids[b, at[b]:at[b] + k] for b, k in zip(live, n)], [list(range(-1, k - 1)) for k in n], live, at[live], need_next=False)
+        at[live] = m.accept(live, at[live], [list(range(k)) for k in n])
+    last = [int(ids[b, ctx]) for b in range(B)]
+    one = m.step_seqs(np.array(last, np.int32), rows, at)
+    want = [m.logits(b) for b in range(B)]
+    # the same token behind the context in each sequence, and a second child of the context, which sees neither it nor its child
+    nxt = m.step_tree([[t, 7, (t + 1) % cfg.vocab_size] for t in last], [[-1, 0, -1]] * B, rows, at)
+    for b in range(B):
+        assert float(np.abs(m.logits(3 * b) - want[b]).max()) <= 4e-3, b
+        top = np.sort(want[b])[-2:]
+        if top[1] - top[0] > 8e-3:
+            assert nxt[b][0] == one[b]
+    m.close()
