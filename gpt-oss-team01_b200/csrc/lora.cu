@@ -32,6 +32,7 @@ constexpr int kRoom = 2 * kSmCountFallback;
 // 128, 4 adapters 32.6 and 37.8; 1200 tokens, rank 128, 8 adapters 45.8 and 65.8.
 constexpr int kWideTokens = 768;
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
+constexpr int kSumSteps = 3;          // steps whose products the tensor core adds up
 constexpr int kColBlock = 128;        // outputs of a tile that go to one CTA as a whole, with many tiles
 constexpr int kSmallU = 256;          // pieces of 4 values of u up to which every CTA of a cluster sums up all
 
@@ -304,6 +305,10 @@ struct Work {
 
 // acc_s[m][r] = sum over this CTA's part of K (steps `part` of `parts`) of A[r, :] x[m, :], rows of 8 RN values (ranks beyond
 // the adapter's: zero); the warps' sums are added in their order.
+// The tensor core cuts off what falls below the last bit of a sum, always towards zero.  So a warp's sums stay in it for kSumSteps
+// steps only (three: K = 2880 in tiles of 64 tokens has no more) and are then added to those in shared memory, which rounds.  With the
+// whole part as one sum the error was 4.8e-7 of the result at K = 16384, 4.4e-6 at 65536; now 1.9e-7 and 2.1e-7.  Sums of a step each,
+// as in lora_shrink_kernel, are at 1.2e-7 and 1.8e-7, but their products wait for each other (600 tokens, rank 64: 45 us, now 39).
 template <int RN>
 __device__ __forceinline__ void partial_u(const gptoss_lora_args &g, const Work &k, int part, int parts, float *acc_s) {
   const int warp = threadIdx.x >> 5, row = k.row, c = k.c;
@@ -325,6 +330,20 @@ __device__ __forceinline__ void partial_u(const gptoss_lora_args &g, const Work 
   const int stride = parts * k.wn * kShrinkStep;
   int at0 = (part * k.wn + k.k) * kShrinkStep;
   load_x(at0);
+  // accumulator of tile j: rows row, row + 8, ranks 8j + 2c, + 1
+  float *mine = acc_s + (size_t)warp * 16 * (8 * RN) + row * (8 * RN) + 2 * c;
+  const auto put = [&](bool add) {
+#pragma unroll
+    for (int j = 0; j < RN; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float2 *p = reinterpret_cast<float2 *>(mine + 8 * h * (8 * RN) + 8 * j);
+        const float2 before = add ? *p : make_float2(0.f, 0.f);
+        *p = make_float2(before.x + acc[j][2 * h], before.y + acc[j][2 * h + 1]);
+      }
+  };
+  int step = 0;
+  bool put_before = false;
   for (; at0 < g.K; at0 += stride) {
     const uint4 ca[2] = {xa[0], xa[1]}, cb[2] = {xb[0], xb[1]};
     load_x(at0 + stride);
@@ -346,14 +365,14 @@ __device__ __forceinline__ void partial_u(const gptoss_lora_args &g, const Work 
           mma_16816(acc[j], ca[h].z, cb[h].z, ca[h].w, cb[h].w, w[j - j0][h].z, w[j - j0][h].w);
         }
     }
-  }
-  // accumulator of tile j: rows row, row + 8, ranks 8j + 2c, + 1
-  float *mine = acc_s + (size_t)warp * 16 * (8 * RN);
+    if (++step == kSumSteps && at0 + stride < g.K) {
+      put(put_before);
+      put_before = true, step = 0;
 #pragma unroll
-  for (int j = 0; j < RN; ++j) {
-    *reinterpret_cast<float2 *>(mine + row * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][0], acc[j][1]);
-    *reinterpret_cast<float2 *>(mine + (row + 8) * (8 * RN) + 8 * j + 2 * c) = make_float2(acc[j][2], acc[j][3]);
+      for (int j = 0; j < RN; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+    }
   }
+  put(put_before);
   __syncthreads();
   float4 *sum4 = reinterpret_cast<float4 *>(acc_s);  // the sums take the place of the first warps' ones
   for (int i = threadIdx.x; i < k.t.count * 2 * RN; i += blockDim.x) {
@@ -686,8 +705,7 @@ __global__ void __launch_bounds__(32 * kLoraWarps, RN <= 8 ? 2 : 1) lora_shrink_
     __syncthreads();
     fetch(step + Ring::kStages - 1);
     const uint8_t *ring = smem_b + (step % Ring::kStages) * Ring::kStageBytes + 16 * c;
-    // a step's products have a sum of their own: the tensor core cuts off what falls below the last bit of a sum, always
-    // towards zero, which over thousands of elements would show (errors of 4.8e-7 of the result instead of 5.6e-8 at 2880)
+    // a step's products have a sum of their own, for the reason in partial_u (errors of 5.6e-8 of the result instead of 4.8e-7 at 2880)
     float sum[NJ][4];
 #pragma unroll
     for (int j = 0; j < NJ; ++j) sum[j][0] = sum[j][1] = sum[j][2] = sum[j][3] = 0.f;
