@@ -77,7 +77,8 @@ __device__ __noinline__ void choose_exactly(const gptoss_expert_choice_args &a, 
       b2 = fmax(fmin(b1, o1), fmax(b2, o2));
       b1 = fmax(b1, o1);
     }
-    const double worth = __shfl_sync(0xffffffffu, a.group_top == 2 && gs > 1 ? b1 + b2 : b1, (lane << shift) & 31);
+    double worth = __shfl_sync(0xffffffffu, a.group_top == 2 && gs > 1 ? b1 + b2 : b1, (lane << shift) & 31);
+    if (worth != worth) worth = -INFINITY;  // infinities of both signs
     int ahead = 0;  // groups that come before this lane's
     for (int o = 0; o < a.n_groups; ++o) {
       const double other = __shfl_sync(0xffffffffu, worth, o);

@@ -359,7 +359,7 @@ int gptoss_lora_apply(const gptoss_lora_args *args, void *stream);
  * worth the sum of its group_top (1 or 2) largest choices, and only the topk_groups best groups take part.  The k largest
  * choices are taken, in descending order; of equal ones, of groups and of experts, the lowest index comes first.
  * topk_w = their scores (without the bias), divided by their sum with renormalize, times weight_scale.
- * A NaN logit scores 0, a NaN choice counts as -infinity.  Compared in fp64.  E <= 256, k <= 8, n_groups <= 32. */
+ * A NaN logit scores 0, a NaN choice and a NaN sum (infinities of both signs) count as -infinity.  Compared in fp64.  E <= 256, k <= 8, n_groups <= 32. */
 #define GPTOSS_SCORE_SOFTMAX 0
 #define GPTOSS_SCORE_SIGMOID 1
 typedef struct {
