@@ -879,6 +879,7 @@ int tree_attention(const gptoss_tree_attention_args &a, const void *q_low, int *
   if (a.max_nodes > GPTOSS_TREE_MAX_NODES) return serving_fail(GPTOSS_ERR_BAD_ARG, "more than 256 drafted tokens per sequence");
   if (a.n_seqs == 0 || a.n_tokens == 0 || a.max_nodes == 0) return GPTOSS_OK;
   if (a.cache_rows <= 0 || a.max_seq <= 0) return serving_fail(GPTOSS_ERR_BAD_ARG, "empty cache");
+  if (a.max_seq > 1 << 30) return serving_fail(GPTOSS_ERR_BAD_ARG, "max_seq goes up to 2^30");  // slots and positions are counted in int
   if (a.mask_words < (a.max_nodes + 31) / 32)
     return serving_fail(GPTOSS_ERR_BAD_ARG, "mask_words does not hold a bit for every drafted token");
   if (!a.q || !a.k_cache || !a.v_cache || !a.offsets || !a.ctx_len || !a.mask || !a.out)

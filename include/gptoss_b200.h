@@ -300,7 +300,7 @@ int gptoss_serving_status(void);
  * hold anything, NaN included.  Rows of out behind offsets[n_seqs] are left as they were.
  * bf16: q [n_tokens][n_q_heads][head_dim], token stride q_stride elements (a multiple of 8); caches
  * [cache_rows][n_kv_heads][max_seq][head_dim]; out like q.  All 16-byte aligned.  head_dim 32 or 64, 1 to 8 query heads
- * per kv head, up to GPTOSS_TREE_MAX_NODES drafted tokens per sequence, ctx_len[b] + n_b <= max_seq.
+ * per kv head, up to GPTOSS_TREE_MAX_NODES drafted tokens per sequence, ctx_len[b] + n_b <= max_seq <= 2^30.
  * max_nodes must not be below the largest n_b (further tokens of a sequence are not computed); max_ctx sizes the launch:
  * the result is right for any ctx_len, the work is spread best when max_ctx is the largest. */
 #define GPTOSS_TREE_MAX_NODES 256
