@@ -332,7 +332,7 @@ extern "C" int gptoss_expert_choice(const gptoss_expert_choice_args *args, void 
   if (a.T == 0) return GPTOSS_OK;
   if (!a.logits || !a.topk_w || !a.topk_i) return serving_fail(GPTOSS_ERR_BAD_ARG, "null pointer");
   if (a.stride < a.E) return serving_fail(GPTOSS_ERR_BAD_ARG, "row stride below n_experts");
-  const dim3 grid((a.T + 3) / 4);
+  const dim3 grid((a.T - 1) / 4 + 1);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const int slots = (a.E + 31) / 32;
   const uint32_t gs = a.E / a.n_groups, magic = gs == 1 ? 0u : 0xffffffffu / gs + 1;  // e / gs = high word of e * magic (0: e itself)
