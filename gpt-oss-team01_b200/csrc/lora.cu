@@ -26,10 +26,12 @@ constexpr int kBlockTokens = 512, kBlockBins = 1024;  // and up to here, with fe
 constexpr int kMaxAdapters = 8192;    // bins of the sort, in shared memory
 constexpr int kClusterCtas = 8, kLoraWarps = 8;
 constexpr int kMinSplits = 2, kMaxSplits = 8;  // parts of K with many tiles
-constexpr int kRoom = 2 * kSmCountFallback;
-// From here on a batch counts as many tiles.  Two kernels and one: 600 tokens, rank 16, 16 adapters 19.9 and 18.6 us; 800 tokens,
-// rank 64, 8 adapters 27.7 and 32.7, rank 8, 200 adapters 34.2 and 37.0; 1024 tokens, rank 16, 64 adapters 25.9 and 24.0, rank
-// 128, 4 adapters 32.6 and 37.8; 1200 tokens, rank 128, 8 adapters 45.8 and 65.8.
+constexpr int kRoom = 2 * kSmCountFallback;    // CTAs side by side; a constant, as a workspace may be asked for on any device
+// From here on a batch counts as many tiles.  Two kernels and one, in us: K = 4096, 2880 outputs: 600 tokens, rank 16, 16 adapters 20.2 and
+// 22.5, 200 adapters 44.7 and 44.7; 800 tokens, rank 8, 200 adapters 45.7 and 45.3; 1024 tokens, rank 16, 64 adapters 30.1 and 28.1.
+// K = 2880, 5120 outputs: 520 tokens, rank 16, 64 adapters 26.0 and 23.8.  K = 2880, 2880 outputs: 600 tokens, rank 16, 16 adapters
+// 19.6 and 21.6; 800 tokens, rank 64, 8 adapters 26.4 and 33.5; 1024 tokens, rank 128, 4 adapters 35.4 and 64.3.  So it is even somewhere
+// between 500 and 1000 tokens, by the number of tiles, which the host does not know.
 constexpr int kWideTokens = 768;
 constexpr int kShrinkStep = 64;       // elements of K that a warp takes per step
 constexpr int kSumSteps = 3;          // steps whose products the tensor core adds up

@@ -35,9 +35,10 @@ thread_local char g_serving_error[256] = "";
 // 64 sequences x 64 tokens over 4096), or, with up to 128 rows, on every other slot tile of the same rows.  One warp issues
 // the products, one the copies (a ring of four stages).  256 of the 512 TMEM columns and 111 KiB of shared memory: two CTAs,
 // hence 16 softmax warps, per SM.
-// What bounds it (64 x 64 over 4096: 293 us, 0.33 of the tensor peak; floors 97 us products, 70 us HBM): the exponential
-// unit's 16 results per cycle and SM make 172 us of it, and each warp's row of dependent steps (S from TMEM, maximum,
-// exponentials, P to TMEM, hand-over) keeps that unit 55 % busy.  No gain: 128-slot tiles with two rows of S (370 us), four
+// What bounds it (64 x 64 over 4096: 293 us at best, 302 in a replayed graph of calls, 320 to 328 from a host loop, which runs at lower
+// clocks; floors 97 us products, 70 us HBM): each warp's row of dependent steps (S from TMEM, maximum, exponentials, P to TMEM,
+// hand-over).  No unit is full: of the 6.7e8 exponentials seven eighths go through the exponential unit, whose 16 results per cycle
+// and SM make 126 us of them, and the captured kernel (lower clocks) has it 53 % busy.  No gain: 128-slot tiles with two rows of S (370 us), four
 // CTAs of 128 rows (312 us), two threads per row (319 us), S in two halves with the products one half ahead (311 us), no
 // maximum unless the tile's sum asks for it (spills: 388 us), P in shared memory so that S is free for the next tile as soon as
 // it is in registers (384 us: with N = 64 the A operand's way from shared memory takes twice the product's time; in TMEM there
