@@ -295,9 +295,9 @@ int gptoss_serving_status(void);
  * in the cache, drafted token i in slot ctx_len[b] + i.  Query i attends to every cached token and to the drafted tokens
  * j whose bit is set in its mask (bit j & 31 of word j >> 5; its own bit included, if it shall see itself).  With a
  * window > 0 it attends only to tokens less than `window` positions before its own, the position of a drafted token
- * being ctx_len[b] + depth (run.cpp:582).  Softmax in fp32, the sink joins the denominator only (run.cpp:588-591); the weights are
- * rounded to bf16 for their product with V.  A query that attends to nothing gets zeros.  K and V rows that no query of the tree attends to, and masked ones, may
- * hold anything, NaN included.  Rows of out behind offsets[n_seqs] are left as they were.
+ * being ctx_len[b] + depth (run.cpp:582).  Softmax in fp32, the sink joins the denominator only (run.cpp:588-591); the weights
+ * are rounded to bf16 for their product with V.  A query that attends to nothing gets zeros.  K and V rows that no query of the
+ * tree attends to, and masked ones, may hold anything, NaN included.  Rows of out behind offsets[n_seqs] are left as they were.
  * bf16: q [n_tokens][n_q_heads][head_dim], token stride q_stride elements (a multiple of 8); caches
  * [cache_rows][n_kv_heads][max_seq][head_dim]; out like q.  All 16-byte aligned.  head_dim 32 or 64, 1 to 8 query heads
  * per kv head, up to GPTOSS_TREE_MAX_NODES drafted tokens per sequence, ctx_len[b] + n_b <= max_seq <= 2^30.
@@ -359,7 +359,8 @@ int gptoss_lora_apply(const gptoss_lora_args *args, void *stream);
  * worth the sum of its group_top (1 or 2) largest choices, and only the topk_groups best groups take part.  The k largest
  * choices are taken, in descending order; of equal ones, of groups and of experts, the lowest index comes first.
  * topk_w = their scores (without the bias), divided by their sum with renormalize, times weight_scale.
- * A NaN logit scores 0, a NaN choice and a NaN sum (infinities of both signs) count as -infinity.  Compared in fp64.  E <= 256, k <= 8, n_groups <= 32. */
+ * A NaN logit scores 0, a NaN choice and a NaN sum (infinities of both signs) count as -infinity.  Compared in fp64.
+ * E <= 256, k <= 8, n_groups <= 32. */
 #define GPTOSS_SCORE_SOFTMAX 0
 #define GPTOSS_SCORE_SIGMOID 1
 typedef struct {
